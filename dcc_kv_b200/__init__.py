@@ -26,6 +26,9 @@ from .value_regression import fit_compact_value, ridge_regression_value
 from .compact_kv import CompactKV, build_compact_kv, build_compact_kv_batched
 from .attention import attention
 from .layer import DccKvSyncLayer
+from .rotary import Rotary, rotary_frequencies
+from .kv_cache import KvCache
+from .tree_attention import tree_attention, tree_mask
 
 __all__ = [
     "OnlineSoftmaxState", "online_softmax_from_attention", "merge_softmax_states",
@@ -36,4 +39,5 @@ __all__ = [
     "ridge_regression_value", "fit_compact_value",
     "CompactKV", "build_compact_kv", "build_compact_kv_batched",
     "attention", "DccKvSyncLayer",
+    "Rotary", "rotary_frequencies", "KvCache", "tree_attention", "tree_mask",
 ]

@@ -7,6 +7,7 @@ CUDA tensors and fails loudly when given anything else.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import os
 from typing import Optional
@@ -27,6 +28,14 @@ DCC_ERR_TIMEOUT = 7
 DCC_F32 = 0
 DCC_BF16 = 1
 DCC_F64 = 2
+
+DCC_ROTARY_HALF = 0
+DCC_ROTARY_INTERLEAVED = 1
+
+DCC_KV_BF16 = 0
+DCC_KV_F32 = 1
+DCC_KV_INT8 = 2
+DCC_KV_E4M3 = 3
 
 MAX_SEGMENTS = 16
 
@@ -68,6 +77,38 @@ class dcc_attn_problem(C.Structure):
                 ("n_seg", C.c_int32), ("causal", C.c_int32), ("causal_offset", C.c_int64),
                 ("seg", dcc_kv_segment * MAX_SEGMENTS),
                 ("o_init", C.c_void_p), ("lse_init", C.c_void_p), ("lse_init_head_stride", C.c_int64)]
+
+
+class dcc_rotary_tensor(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("y", C.c_void_p),
+                ("x_seq_stride", C.c_int64), ("x_head_stride", C.c_int64), ("x_row_stride", C.c_int64),
+                ("y_seq_stride", C.c_int64), ("y_head_stride", C.c_int64), ("y_row_stride", C.c_int64),
+                ("n_heads", C.c_int64)]
+
+
+class dcc_kv_pages(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("bias", C.c_void_p), ("n_pages", C.c_int64), ("page_size", C.c_int32),
+                ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32), ("format", C.c_int32)]
+
+
+class dcc_kv_tokens(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("bias", C.c_void_p),
+                ("k_seq_stride", C.c_int64), ("k_head_stride", C.c_int64), ("k_row_stride", C.c_int64),
+                ("v_seq_stride", C.c_int64), ("v_head_stride", C.c_int64), ("v_row_stride", C.c_int64),
+                ("bias_seq_stride", C.c_int64), ("bias_head_stride", C.c_int64),
+                ("start", C.c_void_p), ("counts", C.c_void_p), ("page_table", C.c_void_p),
+                ("table_stride", C.c_int64), ("T", C.c_int64), ("n_seqs", C.c_int32), ("max_pages", C.c_int32)]
+
+
+class dcc_tree_query(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("o", C.c_void_p), ("lse", C.c_void_p),
+                ("q_seq_stride", C.c_int64), ("q_head_stride", C.c_int64), ("q_row_stride", C.c_int64),
+                ("o_seq_stride", C.c_int64), ("o_head_stride", C.c_int64), ("o_row_stride", C.c_int64),
+                ("context", C.c_void_p), ("counts", C.c_void_p), ("tree", C.c_void_p),
+                ("tree_seq_stride", C.c_int64), ("page_table", C.c_void_p), ("table_stride", C.c_int64),
+                ("T", C.c_int64), ("n_seqs", C.c_int32), ("n_q_heads", C.c_int32), ("max_pages", C.c_int32),
+                ("reserved", C.c_int32)]
 
 
 _P = C.c_void_p
@@ -112,6 +153,11 @@ SIGNATURES = {
     "dcc_online_softmax_from_attention": (_I, [_P, _P, _P, _I64, _I64, _I64, _I64, _I, _P, _P, _P, _P]),
     "dcc_merge_softmax_states": (_I, [_P, _P, _P, _P, _P, _P, _I64, _I64, _I, _P, _P, _P, _P]),
     "dcc_merge_lse": (_I, [_P, _P, _I, _I64, _I64, _I, _P, _P, _P]),
+    "dcc_rotary": (_I, [_P, _I, _P, _I, _I64, _I64, _I64, _I64, _I, _I, _P, _D, _I, _I, _I, _P]),
+    "dcc_kv_cache_write": (_I, [C.POINTER(dcc_kv_pages), C.POINTER(dcc_kv_tokens), _I, _P]),
+    "dcc_kv_cache_read": (_I, [C.POINTER(dcc_kv_pages), C.POINTER(dcc_kv_tokens), _I, _P]),
+    "dcc_tree_attention_workspace_bytes": (_SZ, [C.POINTER(dcc_kv_pages), C.POINTER(dcc_tree_query), _I]),
+    "dcc_tree_attention": (_I, [C.POINTER(dcc_kv_pages), C.POINTER(dcc_tree_query), _D, _I, _P, _SZ, _P]),
 }
 
 _lib: Optional[C.CDLL] = None
@@ -161,6 +207,20 @@ def require_cuda(*tensors: torch.Tensor) -> None:
 
 def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def on_device(device: torch.device):
+    """Makes ``device`` the current one for a launch when it is not already
+    (a kernel launches on the current device)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def same_device(device: torch.device, **tensors: Optional[torch.Tensor]) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} is on {t.device}, expected {device}")
 
 
 def ptr(t: Optional[torch.Tensor]) -> Optional[int]:

@@ -50,7 +50,7 @@ const char* dcc_status_string(int status) {
 
 const char* dcc_last_error(void) { return dcc::g_last_error.c_str(); }
 
-int dcc_version(void) { return 2; }
+int dcc_version(void) { return 3; }
 
 size_t dcc_struct_size(const char* name) {
   if (!name) return 0;
@@ -59,6 +59,10 @@ size_t dcc_struct_size(const char* name) {
   if (n == "dcc_build_problem") return sizeof(dcc_build_problem);
   if (n == "dcc_kv_segment") return sizeof(dcc_kv_segment);
   if (n == "dcc_attn_problem") return sizeof(dcc_attn_problem);
+  if (n == "dcc_rotary_tensor") return sizeof(dcc_rotary_tensor);
+  if (n == "dcc_kv_pages") return sizeof(dcc_kv_pages);
+  if (n == "dcc_kv_tokens") return sizeof(dcc_kv_tokens);
+  if (n == "dcc_tree_query") return sizeof(dcc_tree_query);
   return 0;
 }
 

@@ -1,0 +1,314 @@
+// Writing keys and values into the paged cache (quantised on the way) and
+// reading them back.
+//
+// One group of lanes takes one row -- a token of a KV head -- of K and of V:
+// 16 lanes with 8 elements each for head_dim up to 128 (8 lanes up to 64), so
+// the loads are 16 bytes wide, the largest magnitude of the row is a shuffle
+// reduction over its lanes, and each element is read and written once: both
+// kernels are bound by memory.  Rows that are not made of aligned groups of 8
+// elements take a whole warp with one element per lane and load.
+#include <algorithm>
+#include <string>
+
+#include "kv_pages.cuh"
+
+namespace dcc {
+
+constexpr int kCacheThreads = 256;
+
+struct CacheParams {
+  dcc_kv_pages c;
+  dcc_kv_tokens t;
+};
+
+__device__ __forceinline__ uint32_t bits_abs(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
+template <int kFormat>
+__device__ __forceinline__ float scale_of(uint32_t top_bits) {
+  if (top_bits >= 0x7f800000u) return __uint_as_float(0x7fc00000u);
+  const float top = __uint_as_float(top_bits);
+  if constexpr (kFormat == DCC_KV_INT8) return fmaxf(__fdiv_rn(top, 127.f), kSmallestScale);
+  // smallest power of two s with top <= 448 s, 448 = 1.75 * 2^8
+  const int e = (int)(top_bits >> 23) - 8 + ((top_bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return __uint_as_float((uint32_t)max(e, 127 - 96) << 23);
+}
+
+// x / scale to the nearest whole number, ties to even, as the exact quotient
+// rounds: x * (1 / scale) in fp32 is within 3e-5 of it, so only a result next
+// to a tie needs the division in fp64.
+__device__ __forceinline__ int code_int8(float x, float scale, float inv) {
+  const float r = x * inv;
+  float n = rintf(r);
+  if (fabsf(r - n) > 0.4999f) n = (float)rint((double)x / (double)scale);
+  return (int)fminf(fmaxf(n, -127.f), 127.f);
+}
+
+// Codes of N elements (N = 8, or 1) of one row.
+template <int kFormat, int N>
+__device__ __forceinline__ void store_codes(void* base, int64_t at, const float* x, float scale) {
+  const bool good = scale == scale;  // a row with an infinity or NaN keeps zero codes
+  if constexpr (kFormat == DCC_KV_INT8) {
+    const float inv = 1.f / scale;
+    int8_t q[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) q[i] = good ? (int8_t)code_int8(x[i], scale, inv) : (int8_t)0;
+    if constexpr (N == 8) {
+      uint2 w;
+      w.x = (uint8_t)q[0] | (uint8_t)q[1] << 8 | (uint8_t)q[2] << 16 | (uint32_t)(uint8_t)q[3] << 24;
+      w.y = (uint8_t)q[4] | (uint8_t)q[5] << 8 | (uint8_t)q[6] << 16 | (uint32_t)(uint8_t)q[7] << 24;
+      *reinterpret_cast<uint2*>(static_cast<int8_t*>(base) + at) = w;
+    } else {
+      static_cast<int8_t*>(base)[at] = q[0];
+    }
+  } else if constexpr (kFormat == DCC_KV_E4M3) {
+    const float inv = 1.f / scale;  // exact: a power of two
+    if constexpr (N == 8) {
+      uint32_t h[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        h[i] = good ? __nv_cvt_float2_to_fp8x2(make_float2(x[2 * i] * inv, x[2 * i + 1] * inv), __NV_SATFINITE, __NV_E4M3)
+                    : 0u;
+      *reinterpret_cast<uint2*>(static_cast<uint8_t*>(base) + at) = make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
+    } else {
+      static_cast<uint8_t*>(base)[at] = good ? __nv_cvt_float_to_fp8(x[0] * inv, __NV_SATFINITE, __NV_E4M3) : 0;
+    }
+  } else if constexpr (kFormat == DCC_KV_BF16) {
+    __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(base) + at;
+    if constexpr (N == 8) {
+      __align__(16) __nv_bfloat162 h[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+      *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(h);
+    } else {
+      dst[0] = __float2bfloat16_rn(x[0]);
+    }
+  } else {
+    float* dst = static_cast<float*>(base) + at;
+#pragma unroll
+    for (int i = 0; i < N; ++i) dst[i] = x[i];
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* src, float* x) {
+  if constexpr (sizeof(T) == 2) {
+    const uint4 w = *reinterpret_cast<const uint4*>(src);
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = __uint_as_float(u[i] << 16);
+      x[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+    }
+  } else {
+    reinterpret_cast<float4*>(x)[0] = reinterpret_cast<const float4*>(src)[0];
+    reinterpret_cast<float4*>(x)[1] = reinterpret_cast<const float4*>(src)[1];
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* dst, const float* x) {
+  if constexpr (sizeof(T) == 2) {
+    __align__(16) __nv_bfloat162 h[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+    *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(h);
+  } else {
+    reinterpret_cast<float4*>(dst)[0] = reinterpret_cast<const float4*>(x)[0];
+    reinterpret_cast<float4*>(dst)[1] = reinterpret_cast<const float4*>(x)[1];
+  }
+}
+template <int kFormat>
+__device__ __forceinline__ void load_codes8(const void* base, int64_t at, float* x) {
+  if constexpr (kFormat == DCC_KV_BF16) {
+    load8(static_cast<const __nv_bfloat16*>(base) + at, x);
+  } else if constexpr (kFormat == DCC_KV_F32) {
+    load8(static_cast<const float*>(base) + at, x);
+  } else {
+    const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(base) + at);
+    if constexpr (kFormat == DCC_KV_INT8) {
+      decode_int8x4(w.x, x);
+      decode_int8x4(w.y, x + 4);
+    } else {
+      decode_e4m3x4(w.x, x);
+      decode_e4m3x4(w.y, x + 4);
+    }
+  }
+}
+
+// The row of this group of kLanes lanes: sequence, KV head, token and the
+// place in the cache (-1: none).
+struct RowAt {
+  int64_t b, t, at;
+  int h;
+  bool counted;
+};
+__device__ __forceinline__ RowAt row_at(const CacheParams& p, int64_t row) {
+  RowAt r;
+  r.t = row % p.t.T;
+  const int64_t bh = row / p.t.T;
+  r.h = (int)(bh % p.c.n_kv_heads);
+  r.b = bh / p.c.n_kv_heads;
+  r.counted = !p.t.counts || r.t < p.t.counts[r.b];
+  r.at = -1;
+  if (r.counted) {
+    const PageWalk w{p.t.page_table + r.b * p.t.table_stride, p.c.n_pages, p.c.page_size, p.t.max_pages};
+    int off = 0;
+    const int64_t page = w.page_of((int64_t)p.t.start[r.b] + r.t, off);
+    if (page >= 0) r.at = page_row(p.c, page, r.h, off);
+  }
+  return r;
+}
+
+template <typename T, int kFormat, int kLanes>  // kLanes 8 or 16: 8 elements a lane; 32: one element a load
+__global__ void __launch_bounds__(kCacheThreads) cache_write_kernel(const __grid_constant__ CacheParams p) {
+  constexpr bool kScaled = kFormat == DCC_KV_INT8 || kFormat == DCC_KV_E4M3;
+  constexpr bool kWide = kLanes < 32;
+  const int64_t row = (int64_t)blockIdx.x * (kCacheThreads / kLanes) + threadIdx.x / kLanes;
+  const int64_t rows = (int64_t)p.t.n_seqs * p.c.n_kv_heads * p.t.T;
+  const int lane = threadIdx.x % kLanes;
+  const int d = p.c.head_dim;
+  RowAt r{0, 0, -1, 0, false};
+  if (row < rows) r = row_at(p, row);
+  const bool live = r.at >= 0;  // the same for the lanes of a row; all lanes take part in the shuffles
+  const T* k = static_cast<const T*>(p.t.k) + r.b * p.t.k_seq_stride + r.h * p.t.k_head_stride + r.t * p.t.k_row_stride;
+  const T* v = static_cast<const T*>(p.t.v) + r.b * p.t.v_seq_stride + r.h * p.t.v_head_stride + r.t * p.t.v_row_stride;
+  __align__(16) float x[2][kWide ? 8 : 4];
+  uint32_t top[2] = {0u, 0u};
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    const T* src = s ? v : k;
+    if constexpr (kWide) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[s][i] = 0.f;
+      if (live && lane * 8 < d) load8(src + lane * 8, x[s]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[s][i] = live && lane + 32 * i < d ? to_f32<T>(src[lane + 32 * i]) : 0.f;
+    }
+  }
+  if constexpr (kScaled) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+#pragma unroll
+      for (int i = 0; i < (kWide ? 8 : 4); ++i) top[s] = max(top[s], bits_abs(x[s][i]));
+#pragma unroll
+      for (int o = kLanes / 2; o > 0; o >>= 1) top[s] = max(top[s], __shfl_xor_sync(0xffffffffu, top[s], o));
+    }
+  }
+  if (!live) return;
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    void* base = s ? p.c.v : p.c.k;
+    float scale = 1.f;
+    if constexpr (kScaled) {
+      scale = scale_of<kFormat>(top[s]);
+      if (lane == 0) (s ? p.c.v_scale : p.c.k_scale)[r.at] = scale;
+    }
+    if constexpr (kWide) {
+      if (lane * 8 < d) store_codes<kFormat, 8>(base, r.at * d + lane * 8, x[s], scale);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (lane + 32 * i < d) store_codes<kFormat, 1>(base, r.at * d + lane + 32 * i, &x[s][i], scale);
+    }
+  }
+  if (p.c.bias && lane == 0)
+    p.c.bias[r.at] = p.t.bias ? p.t.bias[r.b * p.t.bias_seq_stride + r.h * p.t.bias_head_stride + r.t] : 0.f;
+}
+
+template <typename T, int kFormat, int kLanes>
+__global__ void __launch_bounds__(kCacheThreads) cache_read_kernel(const __grid_constant__ CacheParams p) {
+  constexpr bool kScaled = kFormat == DCC_KV_INT8 || kFormat == DCC_KV_E4M3;
+  const int64_t row = (int64_t)blockIdx.x * (kCacheThreads / kLanes) + threadIdx.x / kLanes;
+  const int64_t rows = (int64_t)p.t.n_seqs * p.c.n_kv_heads * p.t.T;
+  if (row >= rows) return;
+  const int lane = threadIdx.x % kLanes;
+  const int d = p.c.head_dim;
+  const RowAt r = row_at(p, row);
+  T* k = static_cast<T*>(p.t.k) + r.b * p.t.k_seq_stride + r.h * p.t.k_head_stride + r.t * p.t.k_row_stride;
+  T* v = static_cast<T*>(p.t.v) + r.b * p.t.v_seq_stride + r.h * p.t.v_head_stride + r.t * p.t.v_row_stride;
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    const void* base = s ? p.c.v : p.c.k;
+    T* dst = s ? v : k;
+    float scale = 1.f;
+    if constexpr (kScaled)
+      if (r.at >= 0) scale = (s ? p.c.v_scale : p.c.k_scale)[r.at];
+    if constexpr (kLanes < 32) {
+      if (lane * 8 < d) {
+        __align__(16) float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (r.at >= 0) load_codes8<kFormat>(base, r.at * d + lane * 8, x);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] *= scale;
+        store8(dst + lane * 8, x);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (lane + 32 * i < d)
+          dst[lane + 32 * i] = from_f32<T>(r.at >= 0 ? load_code<kFormat>(base, r.at * d + lane + 32 * i) * scale : 0.f);
+    }
+  }
+  if (p.t.bias && lane == 0)
+    p.t.bias[r.b * p.t.bias_seq_stride + r.h * p.t.bias_head_stride + r.t] =
+        r.at >= 0 && p.c.bias ? p.c.bias[r.at] : 0.f;
+}
+
+template <bool kWrite, typename T, int kFormat, int kLanes>
+static int cache_launch(const CacheParams& p, cudaStream_t st) {
+  const int64_t rows = (int64_t)p.t.n_seqs * p.c.n_kv_heads * p.t.T;
+  const int64_t blocks = (rows + kCacheThreads / kLanes - 1) / (kCacheThreads / kLanes);
+  if (blocks > 2147483647LL) return fail(DCC_ERR_UNSUPPORTED, "kv_cache: too many rows");
+  if (kWrite) cache_write_kernel<T, kFormat, kLanes><<<(unsigned)blocks, kCacheThreads, 0, st>>>(p);
+  else cache_read_kernel<T, kFormat, kLanes><<<(unsigned)blocks, kCacheThreads, 0, st>>>(p);
+  return check_launch(kWrite ? "kv_cache_write" : "kv_cache_read");
+}
+
+template <bool kWrite, typename T, int kFormat>
+static int cache_lanes(const CacheParams& p, cudaStream_t st) {
+  const dcc_kv_tokens& t = p.t;
+  bool wide = p.c.head_dim % 8 == 0;
+  for (const void* q : {(const void*)t.k, (const void*)t.v, (const void*)p.c.k, (const void*)p.c.v})
+    wide = wide && (reinterpret_cast<uintptr_t>(q) & 15u) == 0;
+  for (int64_t s : {t.k_seq_stride, t.k_head_stride, t.k_row_stride, t.v_seq_stride, t.v_head_stride, t.v_row_stride})
+    wide = wide && s % 8 == 0;
+  if (!wide) return cache_launch<kWrite, T, kFormat, 32>(p, st);
+  return p.c.head_dim <= 64 ? cache_launch<kWrite, T, kFormat, 8>(p, st) : cache_launch<kWrite, T, kFormat, 16>(p, st);
+}
+
+template <bool kWrite, typename T>
+static int cache_format(const CacheParams& p, cudaStream_t st) {
+  switch (p.c.format) {
+    case DCC_KV_BF16: return cache_lanes<kWrite, T, DCC_KV_BF16>(p, st);
+    case DCC_KV_F32: return cache_lanes<kWrite, T, DCC_KV_F32>(p, st);
+    case DCC_KV_INT8: return cache_lanes<kWrite, T, DCC_KV_INT8>(p, st);
+    default: return cache_lanes<kWrite, T, DCC_KV_E4M3>(p, st);
+  }
+}
+
+template <bool kWrite>
+static int cache_call(const dcc_kv_pages* cache, const dcc_kv_tokens* tokens, int dtype, void* stream) {
+  const char* what = kWrite ? "kv_cache_write" : "kv_cache_read";
+  DCC_CHECK(check_pages(cache, what));
+  if (!tokens || tokens->T < 0 || tokens->n_seqs < 0 || tokens->max_pages < 0)
+    return fail(DCC_ERR_INVALID_ARGUMENT, std::string(what) + ": bad tokens");
+  if (dtype != DCC_F32 && dtype != DCC_BF16) return fail(DCC_ERR_DTYPE, std::string(what) + ": unsupported dtype");
+  if (kWrite && tokens->bias && !cache->bias)
+    return fail(DCC_ERR_INVALID_ARGUMENT, "kv_cache_write: the cache holds no logit bias");
+  if (tokens->T == 0 || tokens->n_seqs == 0) return DCC_OK;
+  if (!tokens->k || !tokens->v || !tokens->start || (tokens->max_pages > 0 && !tokens->page_table))
+    return fail(DCC_ERR_INVALID_ARGUMENT, std::string(what) + ": null tensor");
+  CacheParams p{*cache, *tokens};
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return dtype == DCC_F32 ? cache_format<kWrite, float>(p, st) : cache_format<kWrite, __nv_bfloat16>(p, st);
+}
+
+}  // namespace dcc
+
+using namespace dcc;
+
+extern "C" int dcc_kv_cache_write(const dcc_kv_pages* cache, const dcc_kv_tokens* tokens, int dtype, void* stream) {
+  return cache_call<true>(cache, tokens, dtype, stream);
+}
+extern "C" int dcc_kv_cache_read(const dcc_kv_pages* cache, const dcc_kv_tokens* tokens, int dtype, void* stream) {
+  return cache_call<false>(cache, tokens, dtype, stream);
+}

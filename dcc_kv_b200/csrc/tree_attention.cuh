@@ -1,0 +1,178 @@
+// Work of the tree attention and its division among CTAs.
+//
+// The rows of one sequence and KV head -- T newest tokens x `group` query
+// heads, row = t * group + g -- are cut into tiles of `n_rows`, its cached
+// tokens into tiles of 128 keys.  An item is (sequence, KV head, row tile) with
+// all its key tiles.  The key tiles of all items, in that order, form one
+// line that is cut into n_ctas equal spans (+-1 tile; one tile each where there
+// are fewer tiles), whatever the lengths: a CTA walks over its span, and an item that does not lie in one span leaves
+// unnormalised partial results (O, max, sum), which tree_merge_kernel adds in
+// the order of the CTAs -- no atomics, so results repeat bit for bit.  The
+// lengths are read on the device: neither the launch nor a captured graph
+// depends on them.
+#pragma once
+
+#include "kv_pages.cuh"
+
+namespace dcc {
+
+constexpr int kTreeKeys = 128;
+constexpr int kTreePartCols = 128;
+constexpr int64_t kTreeMaxT = 4096;
+
+struct TreeParams {
+  dcc_kv_pages c;
+  dcc_tree_query q;
+  int group;    // query heads per KV head
+  int n_rows;   // rows per row tile
+  int n_row_tiles;
+  int n_ctas;
+  float scale;
+  float* part_o;   // [n_ctas][2][n_rows][kTreePartCols]
+  float* part_ml;  // [n_ctas][2][n_rows][2]: max, sum
+};
+
+struct SeqTokens {
+  int64_t ctx;    // positions before the newest
+  int64_t total;  // positions that are looked at (0 when no row asks)
+  int cnt;        // newest tokens
+};
+__device__ __forceinline__ SeqTokens tree_tokens(const TreeParams& p, int b) {
+  SeqTokens s;
+  s.ctx = max(p.q.context[b], 0);
+  const int64_t T = p.q.T;
+  s.cnt = (int)(p.q.counts ? min(max((int64_t)p.q.counts[b], (int64_t)0), T) : T);
+  const int64_t cap = (int64_t)p.q.max_pages * p.c.page_size;
+  s.total = s.cnt > 0 ? min(s.ctx + s.cnt, cap) : 0;
+  return s;
+}
+__device__ __forceinline__ int64_t tree_key_tiles(const SeqTokens& s) { return (s.total + kTreeKeys - 1) / kTreeKeys; }
+
+__device__ __forceinline__ bool tree_sees(const TreeParams& p, int b, int64_t t, int64_t i) {
+  return p.q.tree ? p.q.tree[b * p.q.tree_seq_stride + t * p.q.T + i] != 0 : i <= t;
+}
+
+// n spans of `total` >= n tiles, none empty.
+__device__ __forceinline__ int span_count(int64_t total, int n_ctas) { return (int)(total < n_ctas ? total : n_ctas); }
+__device__ __forceinline__ int64_t span_begin(int64_t total, int i, int n) { return total * i / n; }
+// The span that holds tile g.
+__device__ __forceinline__ int span_owner(int64_t total, int64_t g, int n) { return (int)(((g + 1) * n - 1) / total); }
+
+// Where a CTA begins: the sequence that holds tile `begin` and the number of
+// its first tile.
+struct TreePlan {
+  int64_t total, begin, end, seq_off;
+  int seq;
+};
+struct TreePlanSmem {
+  int64_t warp[32];
+  TreePlan plan;
+};
+// All threads of the block; ends with a __syncthreads.
+__device__ __forceinline__ void tree_plan(const TreeParams& p, int cta, TreePlanSmem& sm) {
+  const int n_thr = blockDim.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, n_warps = (n_thr + 31) >> 5;
+  const int64_t items = (int64_t)p.c.n_kv_heads * p.n_row_tiles;
+  int64_t sum = 0;
+  for (int b = tid; b < p.q.n_seqs; b += n_thr) sum += items * tree_key_tiles(tree_tokens(p, b));
+  sum = warp_sum(sum);
+  if (lane == 0) sm.warp[warp] = sum;
+  __syncthreads();
+  int64_t total = 0;
+  for (int w = 0; w < n_warps; ++w) total += sm.warp[w];
+  const int n = span_count(total, p.n_ctas);
+  const int64_t begin = cta < n ? span_begin(total, cta, n) : 0, end = cta < n ? span_begin(total, cta + 1, n) : 0;
+  if (tid == 0) sm.plan = TreePlan{total, begin, end, 0, 0};
+  if (begin < end) {  // the same for every thread
+    int64_t carry = 0;
+    for (int b0 = 0; b0 < p.q.n_seqs && carry <= begin; b0 += n_thr) {
+      const int b = b0 + tid;
+      const int64_t w = b < p.q.n_seqs ? items * tree_key_tiles(tree_tokens(p, b)) : 0;
+      int64_t incl = w;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += up;
+      }
+      __syncthreads();
+      if (lane == 31) sm.warp[warp] = incl;
+      __syncthreads();
+      int64_t before = carry;
+      for (int i = 0; i < n_warps; ++i) {
+        if (i < warp) before += sm.warp[i];
+        carry += sm.warp[i];
+      }
+      const int64_t off = before + incl - w;
+      if (off <= begin && begin < off + w) {
+        sm.plan.seq = b;
+        sm.plan.seq_off = off;
+      }
+    }
+  }
+  __syncthreads();
+}
+
+// The pieces of a CTA's span, one item (or the part of it in the span) after
+// the other.  Every role of a CTA walks the same pieces.
+struct TreePiece {
+  int b, hk, rt;
+  int64_t k0, k1;  // key tiles
+  SeqTokens s;
+  int part;        // -1: the whole item, else the partial slot (0: begun by an earlier CTA, 1: begun here)
+};
+struct TreeWalk {
+  int64_t g, end, off, tiles;  // next tile, end of span, first tile of sequence b, key tiles of b
+  int b;
+  SeqTokens s;
+  __device__ __forceinline__ void start(const TreeParams& p, const TreePlan& pl) {
+    g = pl.begin;
+    end = pl.end;
+    off = pl.seq_off;
+    b = pl.seq;
+    if (g < end) {
+      s = tree_tokens(p, b);
+      tiles = tree_key_tiles(s);
+    }
+  }
+  __device__ __forceinline__ bool next(const TreeParams& p, TreePiece& o) {
+    if (g >= end) return false;
+    const int64_t items = (int64_t)p.c.n_kv_heads * p.n_row_tiles;
+    while (g >= off + items * tiles) {  // ends: g < end <= the tiles of all sequences
+      off += items * tiles;
+      s = tree_tokens(p, ++b);
+      tiles = tree_key_tiles(s);
+    }
+    const int64_t item = (g - off) / tiles, first = off + item * tiles, last = first + tiles;
+    const int64_t stop = last < end ? last : end;
+    o.b = b;
+    o.hk = (int)(item / p.n_row_tiles);
+    o.rt = (int)(item - (int64_t)o.hk * p.n_row_tiles);
+    o.k0 = g - first;
+    o.k1 = stop - first;
+    o.s = s;
+    o.part = o.k0 > 0 ? 0 : (o.k1 < tiles ? 1 : -1);
+    g = stop;
+    return true;
+  }
+};
+
+// q row of the tile: token, query head; valid when it exists.
+struct TreeRow {
+  int64_t t;
+  int h;
+  bool exists;
+};
+__device__ __forceinline__ TreeRow tree_row(const TreeParams& p, int hk, int rt, int r) {
+  const int64_t row = (int64_t)rt * p.n_rows + r;
+  TreeRow o;
+  o.t = row / p.group;
+  o.h = hk * p.group + (int)(row - o.t * p.group);
+  o.exists = o.t < p.q.T;
+  return o;
+}
+
+template <typename T>
+__device__ __forceinline__ T* tree_out_row(const TreeParams& p, int b, const TreeRow& r) {
+  return static_cast<T*>(p.q.o) + b * p.q.o_seq_stride + r.h * p.q.o_head_stride + r.t * p.q.o_row_stride;
+}
+
+}  // namespace dcc

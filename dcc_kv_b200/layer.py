@@ -410,3 +410,27 @@ class DccKvSyncLayer:
         bp = min(self.budgets[(s, r)], self.L)
         return CompactKV(self.ck[r][h, o:o + bp], self.cb[r][h, o:o + bp], self.cv[r][h, o:o + bp],
                          self.ci[r][h, o:o + bp])
+
+    def write_cache(self, cache, page_table: torch.Tensor, r: int, k: torch.Tensor, v: torch.Tensor) -> int:
+        """Puts what block r attended to in the last forward (same k, v
+        [nb, H_kv, L, d]) into one sequence of a :class:`KvCache`, so that
+        decoding goes on where the prefill stopped: the compact keys of the
+        sources s < r with their logit bias, then block r's own keys.
+        ``page_table`` [1, max_pages] int32 with room for all of them.
+        Returns the number of tokens: the ``context_lens`` of
+        :func:`tree_attention` for the tokens that follow."""
+        if not 0 <= r < self.nb:
+            raise ValueError(f"block {r} of {self.nb}")
+        self.check_inputs(self.out, k, v)
+        n = self.total[r] + self.L
+        if page_table.shape[-1] * cache.page_size < n:
+            raise ValueError(f"the page table holds {page_table.shape[-1] * cache.page_size} tokens, need {n}")
+        if self.total[r] > 0:
+            if cache.logit_bias is None:
+                raise ValueError("compact keys have a logit bias; make the cache with logit_bias=True")
+            cache.write(self.ck[r][None], self.cv[r][None], page_table, 0, logit_bias=self.cb[r][None])
+        cache.write(k[r][None], v[r][None], page_table, self.total[r])
+        if self._host_stream is not None and self._last_call_host:
+            # the next host-buffer call builds on its own stream: not before the compact keys are read
+            self._host_stream.wait_stream(torch.cuda.current_stream(self.device))
+        return n

@@ -43,10 +43,12 @@ enum { DCC_F32 = 0, DCC_BF16 = 1, DCC_F64 = 2 };
 
 const char* dcc_status_string(int status);
 const char* dcc_last_error(void);
-/* ABI version: 2 added the initial state of dcc_attn_problem. */
+/* ABI version: 2 added the initial state of dcc_attn_problem, 3 the decoding
+ * entry points at the end of this file. */
 int dcc_version(void);
 /* sizeof of an ABI struct by its name ("dcc_query_set", "dcc_build_problem",
- * "dcc_kv_segment", "dcc_attn_problem"), 0 for an unknown name -- lets a
+ * "dcc_kv_segment", "dcc_attn_problem", "dcc_rotary_tensor", "dcc_kv_pages",
+ * "dcc_kv_tokens", "dcc_tree_query"), 0 for an unknown name -- lets a
  * foreign-function binding check its struct layouts. */
 size_t dcc_struct_size(const char* name);
 
@@ -279,6 +281,123 @@ int dcc_merge_softmax_states(const void* m_a, const void* l_a, const void* o_a, 
  * lse_parts[p] [R] float32; out [R, D] (dtype), lse_out [R] (may be NULL). */
 int dcc_merge_lse(const void* const* o_parts, const float* const* lse_parts, int n_parts, int64_t R,
                   int64_t D, int dtype, void* out, float* lse_out, void* stream);
+
+/* ---- decoding behind the prefill -------------------------------------------
+ * No counterpart in the reference, which stops after the prefill: rotary
+ * positions, a paged KV cache that is quantised as it is written, and the
+ * attention of the newest tokens (one per sequence, or a tree of drafted
+ * ones) over that cache. */
+
+/* Rotary positions.  Pair i of the first 2 * n_freqs elements of a head is
+ * turned by 2 pi position turns[i] and scaled by `magnitude`:
+ *   y1 = magnitude (x1 cos a - x2 sin a),  y2 = magnitude (x1 sin a + x2 cos a)
+ * with (x1, x2) = elements (i, i + n_freqs) (DCC_ROTARY_HALF) or (2i, 2i + 1)
+ * (DCC_ROTARY_INTERLEAVED); the rest of the head is copied.  `inverse` turns by
+ * -a: the transpose of the forward map, so its gradient.  One or two tensors
+ * (queries, keys) [n_seqs, n_heads, T, head_dim] share the positions
+ * [n_seqs, T] (element strides, a zero sequence stride shares one row).  y may
+ * be x itself (same strides).  turns: n_freqs <= 128 doubles in host memory,
+ * read during the call. */
+enum { DCC_ROTARY_HALF = 0, DCC_ROTARY_INTERLEAVED = 1 };
+typedef struct dcc_rotary_tensor {
+  const void* x;
+  void* y;
+  int64_t x_seq_stride, x_head_stride, x_row_stride;
+  int64_t y_seq_stride, y_head_stride, y_row_stride;
+  int64_t n_heads;
+} dcc_rotary_tensor;
+int dcc_rotary(const dcc_rotary_tensor* tensors, int n_tensors, const void* positions,
+               int positions_are_int64, int64_t pos_seq_stride, int64_t pos_row_stride, int64_t n_seqs,
+               int64_t T, int head_dim, int n_freqs, const double* turns, double magnitude, int layout,
+               int inverse, int dtype, void* stream);
+
+/* Paged KV cache.  A page holds page_size tokens of every KV head:
+ * k, v [n_pages, n_kv_heads, page_size, head_dim] contiguous codes, k_scale and
+ * v_scale [n_pages, n_kv_heads, page_size] float (DCC_KV_INT8, DCC_KV_E4M3
+ * only), bias [n_pages, n_kv_heads, page_size] float logit bias or NULL.
+ * Row = one token of one KV head; value = code * scale:
+ *   DCC_KV_INT8: scale = max(amax / 127, 2^-96) in float, code = x / scale
+ *     rounded to nearest even and clamped to +-127
+ *   DCC_KV_E4M3: scale = the smallest power of two >= amax / 448, at least
+ *     2^-96, code = e4m3(x / scale), rounded to nearest even
+ *   DCC_KV_BF16, DCC_KV_F32: code = x.
+ * A quantised row with an infinity or NaN gets scale NaN and zero codes, so
+ * all of it reads as NaN.  head_dim <= 128. */
+enum { DCC_KV_BF16 = 0, DCC_KV_F32 = 1, DCC_KV_INT8 = 2, DCC_KV_E4M3 = 3 };
+typedef struct dcc_kv_pages {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  float* bias;
+  int64_t n_pages;
+  int32_t page_size;
+  int32_t n_kv_heads;
+  int32_t head_dim;
+  int32_t format;
+} dcc_kv_pages;
+
+/* T tokens of each of n_seqs sequences: token t < counts[s] (NULL: every t)
+ * of sequence s stands at position start[s] + t, row position % page_size of
+ * page page_table[s * table_stride + position / page_size].  Positions below
+ * zero or behind max_pages pages, and page numbers outside [0, n_pages), hold
+ * nothing: a write skips them, a read gives zeros, as for t >= counts[s].
+ * k, v [n_seqs, n_kv_heads, T, head_dim] (DCC_F32 or DCC_BF16), bias
+ * [n_seqs, n_kv_heads, T] with unit row stride. */
+typedef struct dcc_kv_tokens {
+  void* k;
+  void* v;
+  float* bias;
+  int64_t k_seq_stride, k_head_stride, k_row_stride;
+  int64_t v_seq_stride, v_head_stride, v_row_stride;
+  int64_t bias_seq_stride, bias_head_stride;
+  const int32_t* start;
+  const int32_t* counts;
+  const int32_t* page_table;
+  int64_t table_stride;
+  int64_t T;
+  int32_t n_seqs;
+  int32_t max_pages;
+} dcc_kv_tokens;
+/* Quantises tokens into the cache.  Two tokens of one call at the same row
+ * leave that row undefined.  tokens->bias NULL writes a zero bias. */
+int dcc_kv_cache_write(const dcc_kv_pages* cache, const dcc_kv_tokens* tokens, int dtype, void* stream);
+/* Reads tokens back: code * scale rounded once to `dtype`. */
+int dcc_kv_cache_read(const dcc_kv_pages* cache, const dcc_kv_tokens* tokens, int dtype, void* stream);
+
+/* Attention of the T newest tokens of each sequence over its cached ones.
+ * Sequence s holds context[s] + counts[s] tokens (counts NULL: T); the last
+ * counts[s] are the newest, and token t sees every position before them and
+ * newest token i when tree[s * tree_seq_stride + t * T + i] is non-zero (tree
+ * NULL: i <= t).  With x = scale q.k + bias over what it sees,
+ * o = softmax(x) v and lse = log sum exp(x); a row that sees nothing, and rows
+ * t >= counts[s], give o = 0 and lse = -inf.  Positions without a page (see
+ * dcc_kv_tokens) are not seen.  q, o [n_seqs, n_q_heads, T, head_dim] in
+ * `dtype` (DCC_BF16 or DCC_F32), lse [n_seqs, n_q_heads, T] contiguous or NULL.
+ * Query head h reads KV head h / (n_q_heads / n_kv_heads).  T <= 4096.
+ * A row that sees a key or value with an infinity or NaN is not finite;
+ * rows that do not see it are unaffected. */
+typedef struct dcc_tree_query {
+  const void* q;
+  void* o;
+  float* lse;
+  int64_t q_seq_stride, q_head_stride, q_row_stride;
+  int64_t o_seq_stride, o_head_stride, o_row_stride;
+  const int32_t* context;
+  const int32_t* counts;
+  const uint8_t* tree;
+  int64_t tree_seq_stride;
+  const int32_t* page_table;
+  int64_t table_stride;
+  int64_t T;
+  int32_t n_seqs;
+  int32_t n_q_heads;
+  int32_t max_pages;
+  int32_t reserved;
+} dcc_tree_query;
+size_t dcc_tree_attention_workspace_bytes(const dcc_kv_pages* cache, const dcc_tree_query* query, int dtype);
+int dcc_tree_attention(const dcc_kv_pages* cache, const dcc_tree_query* query, double scale, int dtype,
+                       void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
