@@ -608,6 +608,12 @@ bool attn_tc05_supported(const dcc_attn_problem& p, const AttnParams& prm) {
 
 int score_error_flag_address(unsigned int** out);
 
+// Device address of the attention's bounded-wait error word on the current
+// device, which the tree attention shares.
+int attn_error_flag_address(unsigned int** out) {
+  return check_cuda(cudaGetSymbolAddress(reinterpret_cast<void**>(out), g_attn_error), "attention flag address");
+}
+
 // Both error words to host memory by a posted write from the device (pinned
 // host memory is device-accessible under unified addressing), so reading
 // them needs neither a copy engine nor a synchronisation.

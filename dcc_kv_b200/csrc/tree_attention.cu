@@ -14,7 +14,8 @@ constexpr int kSimtCtasPerSm = 6;
 // Online softmax over key tiles of 128: thread = key for the scores (q rows
 // from shared memory), thread = column for the values.  fp32 throughout.
 // Bound by instruction issue (2 fused multiply-adds per row, key and column);
-// it serves every type, format and head_dim.
+// it serves fp32 queries and caches and the head_dims that the tensor-core
+// kernel does not take.
 template <typename T, int kFormat>
 __global__ void __launch_bounds__(kSimtThreads) tree_simt_kernel(const __grid_constant__ TreeParams p) {
   constexpr bool kScaled = kFormat == DCC_KV_INT8 || kFormat == DCC_KV_E4M3;
@@ -26,128 +27,131 @@ __global__ void __launch_bounds__(kSimtThreads) tree_simt_kernel(const __grid_co
   __shared__ float vscale_s[kTreeKeys];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int d = p.c.head_dim;
-  tree_plan(p, blockIdx.x, ps);
-  TreeWalk walk;
-  walk.start(p, ps.plan);
-  TreePiece w;
-  while (walk.next(p, w)) {
-    __syncthreads();
-    if (tid < kSimtRows) {
-      m_s[tid] = -INFINITY;
-      l_s[tid] = 0.f;
-    }
-    for (int i = tid; i < kSimtRows * d; i += kSimtThreads) {
-      const int r = i / d, c = i - r * d;
-      const TreeRow row = tree_row(p, w.hk, w.rt, r);
-      q_s[c][r] = row.exists ? to_f32<T>(static_cast<const T*>(p.q.q)[w.b * p.q.q_seq_stride + row.h * p.q.q_head_stride +
-                                                                      row.t * p.q.q_row_stride + c])
-                             : 0.f;
-    }
-    float o[kSimtRows];
-#pragma unroll
-    for (int r = 0; r < kSimtRows; ++r) o[r] = 0.f;
-    const PageWalk pages{p.q.page_table + w.b * p.q.table_stride, p.c.n_pages, p.c.page_size, p.q.max_pages};
-    for (int64_t kt = w.k0; kt < w.k1; ++kt) {
+  const int span = blockIdx.x / p.n_groups;
+  tree_plan(p, span, ps);
+  for (int rt = blockIdx.x % p.n_groups; rt < p.n_row_tiles; rt += p.n_groups) {
+    TreeWalk walk;
+    walk.start(p, ps.plan);
+    TreePiece w;
+    while (walk.next(p, w)) {
       __syncthreads();
-      {
-        const int64_t pos = kt * kTreeKeys + tid;
-        int off = 0;
-        const int64_t page = pos < w.s.total ? pages.page_of(pos, off) : -1;
-        const int64_t at = page >= 0 ? page_row(p.c, page, w.hk, off) : -1;
-        row_s[tid] = at;
-        float x[kSimtRows];
-#pragma unroll
-        for (int r = 0; r < kSimtRows; ++r) x[r] = 0.f;
-        float bias = 0.f, ks = 1.f;
-        if (at >= 0) {
-          for (int c = 0; c < d; ++c) {
-            const float kv = load_code<kFormat>(p.c.k, at * d + c);
-#pragma unroll
-            for (int r = 0; r < kSimtRows; ++r) x[r] = fmaf(q_s[c][r], kv, x[r]);
-          }
-          if (p.c.bias) bias = p.c.bias[at];
-          if (kScaled) {
-            ks = p.c.k_scale[at];
-            vscale_s[tid] = p.c.v_scale[at];
-          }
-        }
-        const int64_t i = pos - w.s.ctx;  // >= 0: newest token i
-#pragma unroll
-        for (int r = 0; r < kSimtRows; ++r) {
-          const TreeRow row = tree_row(p, w.hk, w.rt, r);
-          const bool sees = at >= 0 && row.exists && row.t < w.s.cnt && (i < 0 || tree_sees(p, w.b, row.t, i));
-          x_s[tid][r] = sees ? fmaf(x[r] * ks, p.scale, bias) : __uint_as_float(0xffffffffu);  // mark: not seen
-        }
+      if (tid < kSimtRows) {
+        m_s[tid] = -INFINITY;
+        l_s[tid] = 0.f;
       }
-      __syncthreads();
-      // rows 2 warp, 2 warp + 1
-#pragma unroll
-      for (int rr = 0; rr < 2; ++rr) {
-        const int r = 2 * warp + rr;
-        float x[4], mt = -INFINITY;
-        bool seen[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          x[i] = x_s[lane + 32 * i][r];
-          seen[i] = __float_as_uint(x[i]) != 0xffffffffu;
-          if (seen[i]) mt = fmaxf(mt, x[i]);
-        }
-        const float m_old = m_s[r];
-        const float m_new = fmaxf(m_old, warp_max(mt));
-        const float msub = m_new == -INFINITY ? 0.f : m_new;
-        float sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float e = seen[i] ? expf(x[i] - msub) : 0.f;
-          sum += e;
-          float pv = e;
-          if (kScaled && seen[i]) pv *= vscale_s[lane + 32 * i];
-          x_s[lane + 32 * i][r] = seen[i] ? pv : -0.f;
-        }
-        sum = warp_sum(sum);
-        if (lane == 0) {
-          const float corr = m_old == -INFINITY ? 0.f : expf(m_old - m_new);
-          m_s[r] = m_new;
-          l_s[r] = l_s[r] * corr + sum;
-          corr_s[r] = corr;
-        }
+      for (int i = tid; i < kSimtRows * d; i += kSimtThreads) {
+        const int r = i / d, c = i - r * d;
+        const TreeRow row = tree_row(p, w.hk, rt, r);
+        q_s[c][r] = row.exists ? to_f32<T>(static_cast<const T*>(p.q.q)[w.b * p.q.q_seq_stride + row.h * p.q.q_head_stride +
+                                                                        row.t * p.q.q_row_stride + c])
+                               : 0.f;
       }
-      __syncthreads();
-      if (tid < d) {
+      float o[kSimtRows];
 #pragma unroll
-        for (int r = 0; r < kSimtRows; ++r) o[r] *= corr_s[r];
-        const int64_t left = w.s.total - kt * kTreeKeys;
-        const int n = left < kTreeKeys ? (int)left : kTreeKeys;
-#pragma unroll 4
-        for (int j = 0; j < n; ++j) {
-          const int64_t at = row_s[j];
-          if (at < 0) continue;
-          const float vv = load_code<kFormat>(p.c.v, at * d + tid);
+      for (int r = 0; r < kSimtRows; ++r) o[r] = 0.f;
+      const PageWalk pages{p.q.page_table + w.b * p.q.table_stride, p.c.n_pages, p.c.page_size, p.q.max_pages};
+      for (int kt = w.k0; kt < w.k1; ++kt) {
+        __syncthreads();
+        {
+          const int64_t pos = (int64_t)kt * kTreeKeys + tid;
+          int off = 0;
+          const int64_t page = pos < w.s.total ? pages.page_of(pos, off) : -1;
+          const int64_t at = page >= 0 ? page_row(p.c, page, w.hk, off) : -1;
+          row_s[tid] = at;
+          float x[kSimtRows];
+#pragma unroll
+          for (int r = 0; r < kSimtRows; ++r) x[r] = 0.f;
+          float bias = 0.f, ks = 1.f;
+          if (at >= 0) {
+            for (int c = 0; c < d; ++c) {
+              const float kv = load_code<kFormat>(p.c.k, at * d + c);
+#pragma unroll
+              for (int r = 0; r < kSimtRows; ++r) x[r] = fmaf(q_s[c][r], kv, x[r]);
+            }
+            if (p.c.bias) bias = p.c.bias[at];
+            if (kScaled) {
+              ks = p.c.k_scale[at];
+              vscale_s[tid] = p.c.v_scale[at];
+            }
+          }
+          const int64_t i = pos - w.s.ctx;  // >= 0: newest token i
 #pragma unroll
           for (int r = 0; r < kSimtRows; ++r) {
-            const float pr = x_s[j][r];
-            if (__float_as_uint(pr) != 0x80000000u) o[r] = fmaf(pr, vv, o[r]);  // nothing of a key that is not seen
+            const TreeRow row = tree_row(p, w.hk, rt, r);
+            const bool sees = at >= 0 && row.exists && row.t < w.s.cnt && (i < 0 || tree_sees(p, w.b, row.t, i));
+            x_s[tid][r] = sees ? fmaf(x[r] * ks, p.scale, bias) : __uint_as_float(0xffffffffu);  // mark: not seen
+          }
+        }
+        __syncthreads();
+        // rows 2 warp, 2 warp + 1
+#pragma unroll
+        for (int rr = 0; rr < 2; ++rr) {
+          const int r = 2 * warp + rr;
+          float x[4], mt = -INFINITY;
+          bool seen[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            x[i] = x_s[lane + 32 * i][r];
+            seen[i] = __float_as_uint(x[i]) != 0xffffffffu;
+            if (seen[i]) mt = fmaxf(mt, x[i]);
+          }
+          const float m_old = m_s[r];
+          const float m_new = fmaxf(m_old, warp_max(mt));
+          const float msub = m_new == -INFINITY ? 0.f : m_new;
+          float sum = 0.f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float e = seen[i] ? expf(x[i] - msub) : 0.f;
+            sum += e;
+            float pv = e;
+            if (kScaled && seen[i]) pv *= vscale_s[lane + 32 * i];
+            x_s[lane + 32 * i][r] = seen[i] ? pv : -0.f;
+          }
+          sum = warp_sum(sum);
+          if (lane == 0) {
+            const float corr = m_old == -INFINITY ? 0.f : expf(m_old - m_new);
+            m_s[r] = m_new;
+            l_s[r] = l_s[r] * corr + sum;
+            corr_s[r] = corr;
+          }
+        }
+        __syncthreads();
+        if (tid < d) {
+#pragma unroll
+          for (int r = 0; r < kSimtRows; ++r) o[r] *= corr_s[r];
+          const int64_t left = w.s.total - (int64_t)kt * kTreeKeys;
+          const int n = left < kTreeKeys ? (int)left : kTreeKeys;
+#pragma unroll 4
+          for (int j = 0; j < n; ++j) {
+            const int64_t at = row_s[j];
+            if (at < 0) continue;
+            const float vv = load_code<kFormat>(p.c.v, at * d + tid);
+#pragma unroll
+            for (int r = 0; r < kSimtRows; ++r) {
+              const float pr = x_s[j][r];
+              if (__float_as_uint(pr) != 0x80000000u) o[r] = fmaf(pr, vv, o[r]);  // nothing of a key that is not seen
+            }
           }
         }
       }
-    }
-    __syncthreads();
+      __syncthreads();
 #pragma unroll
-    for (int r = 0; r < kSimtRows; ++r) {
-      if (w.part >= 0) {
-        const int64_t slot = ((int64_t)blockIdx.x * 2 + w.part) * kSimtRows + r;
-        if (tid < d) p.part_o[slot * kTreePartCols + tid] = o[r];
-        if (tid == 0) {
-          p.part_ml[slot * 2] = m_s[r];
-          p.part_ml[slot * 2 + 1] = l_s[r];
+      for (int r = 0; r < kSimtRows; ++r) {
+        if (w.part >= 0) {
+          const int64_t slot = p.part_row(span, rt, w.part, r);
+          if (tid < d) p.part_o[slot * kTreePartCols + tid] = o[r];
+          if (tid == 0) {
+            p.part_ml[slot * 2] = m_s[r];
+            p.part_ml[slot * 2 + 1] = l_s[r];
+          }
+        } else {
+          const TreeRow row = tree_row(p, w.hk, rt, r);
+          if (!row.exists) continue;
+          const float l = l_s[r];
+          if (tid < d) tree_out_row<T>(p, w.b, row)[tid] = from_f32<T>(l == 0.f ? 0.f : o[r] / l);
+          if (tid == 0 && p.q.lse)
+            p.q.lse[((int64_t)w.b * p.q.n_q_heads + row.h) * p.q.T + row.t] = l == 0.f ? -INFINITY : m_s[r] + logf(l);
         }
-      } else {
-        const TreeRow row = tree_row(p, w.hk, w.rt, r);
-        if (!row.exists) continue;
-        const float l = l_s[r];
-        if (tid < d) tree_out_row<T>(p, w.b, row)[tid] = from_f32<T>(l == 0.f ? 0.f : o[r] / l);
-        if (tid == 0 && p.q.lse)
-          p.q.lse[((int64_t)w.b * p.q.n_q_heads + row.h) * p.q.T + row.t] = l == 0.f ? -INFINITY : m_s[r] + logf(l);
       }
     }
   }
@@ -164,9 +168,10 @@ __global__ void __launch_bounds__(kMergeWarps * 32) tree_merge_kernel(const __gr
   const int64_t items = (int64_t)p.c.n_kv_heads * p.n_row_tiles;
   const int b = (int)(blockIdx.x / items);
   const int item = (int)(blockIdx.x - b * items);
+  const int hk = item / p.n_row_tiles, rt = item - hk * p.n_row_tiles;
   int64_t before = 0, all = 0;
   for (int i = threadIdx.x; i < p.q.n_seqs; i += kMergeWarps * 32) {
-    const int64_t w = items * tree_key_tiles(tree_tokens(p, i));
+    const int64_t w = p.c.n_kv_heads * tree_key_tiles(tree_tokens(p, i));
     all += w;
     if (i < b) before += w;
   }
@@ -183,20 +188,19 @@ __global__ void __launch_bounds__(kMergeWarps * 32) tree_merge_kernel(const __gr
     all += sums[1][i];
   }
   const SeqTokens s = tree_tokens(p, b);
-  const int64_t tiles = tree_key_tiles(s), first = before + item * tiles;
+  const int64_t tiles = tree_key_tiles(s), first = before + hk * tiles;
   int i0 = 0, i1 = -1;
   if (tiles > 0) {
-    const int n = span_count(all, p.n_ctas);
+    const int n = span_count(all, p.n_spans);
     i0 = span_owner(all, first, n);
     i1 = span_owner(all, first + tiles - 1, n);
     if (i0 == i1) return;
   }
-  const int hk = item / p.n_row_tiles, rt = item - hk * p.n_row_tiles;
   const int r = blockIdx.y * kMergeWarps + warp;
   if (r >= p.n_rows) return;
   const TreeRow row = tree_row(p, hk, rt, r);
   if (!row.exists) return;
-  auto slot = [&](int i) { return ((int64_t)i * 2 + (i == i0 ? 1 : 0)) * p.n_rows + r; };
+  auto slot = [&](int i) { return p.part_row(i, rt, i == i0 ? 1 : 0, r); };
   float m = -INFINITY;
   for (int i = i0 + lane; i <= i1; i += 32) m = fmaxf(m, p.part_ml[slot(i) * 2]);
   m = warp_max(m);
@@ -224,17 +228,23 @@ __global__ void __launch_bounds__(kMergeWarps * 32) tree_merge_kernel(const __gr
         l == 0.f ? -INFINITY : m + logf(l);
 }
 
-static void tree_params(const dcc_kv_pages& c, const dcc_tree_query& q, TreeParams& p) {
+static bool tree_params(const dcc_kv_pages& c, const dcc_tree_query& q, int dtype, TreeParams& p) {
   p.c = c;
   p.q = q;
   p.group = q.n_q_heads / c.n_kv_heads;
-  p.n_rows = kSimtRows;
-  p.n_row_tiles = (int)((q.T * p.group + p.n_rows - 1) / p.n_rows);
-  p.n_ctas = num_sms() * kSimtCtasPerSm;
+  const bool tc = tree_tc05_supported(c, q, dtype);
+  const int64_t rows = q.T * p.group;
+  p.n_rows = tc ? tree_tc05_rows(rows) : kSimtRows;
+  p.n_row_tiles = (int)((rows + p.n_rows - 1) / p.n_rows);
+  const int ctas = num_sms() * (tc ? 1 : kSimtCtasPerSm);
+  const int rounds = (p.n_row_tiles + ctas - 1) / ctas;
+  p.n_groups = rounds > 0 ? (p.n_row_tiles + rounds - 1) / rounds : 1;
+  p.n_spans = ctas / p.n_groups;
+  return tc;
 }
 
 static size_t tree_carve(TreeParams& p, Workspace& ws) {
-  const size_t slots = (size_t)p.n_ctas * 2 * p.n_rows;
+  const size_t slots = p.n_spans > 1 ? (size_t)p.part_row(p.n_spans, 0, 0, 0) : 0;  // one span leaves no parts
   p.part_o = ws.take<float>(slots * kTreePartCols);
   p.part_ml = ws.take<float>(slots * 2);
   return align_up(ws.used, 256);
@@ -255,10 +265,10 @@ static int tree_check(const dcc_kv_pages* cache, const dcc_tree_query* q, int dt
 template <typename T>
 static void tree_simt_launch(const TreeParams& p, cudaStream_t st) {
   switch (p.c.format) {
-    case DCC_KV_BF16: tree_simt_kernel<T, DCC_KV_BF16><<<p.n_ctas, kSimtThreads, 0, st>>>(p); break;
-    case DCC_KV_F32: tree_simt_kernel<T, DCC_KV_F32><<<p.n_ctas, kSimtThreads, 0, st>>>(p); break;
-    case DCC_KV_INT8: tree_simt_kernel<T, DCC_KV_INT8><<<p.n_ctas, kSimtThreads, 0, st>>>(p); break;
-    default: tree_simt_kernel<T, DCC_KV_E4M3><<<p.n_ctas, kSimtThreads, 0, st>>>(p); break;
+    case DCC_KV_BF16: tree_simt_kernel<T, DCC_KV_BF16><<<p.n_groups * p.n_spans, kSimtThreads, 0, st>>>(p); break;
+    case DCC_KV_F32: tree_simt_kernel<T, DCC_KV_F32><<<p.n_groups * p.n_spans, kSimtThreads, 0, st>>>(p); break;
+    case DCC_KV_INT8: tree_simt_kernel<T, DCC_KV_INT8><<<p.n_groups * p.n_spans, kSimtThreads, 0, st>>>(p); break;
+    default: tree_simt_kernel<T, DCC_KV_E4M3><<<p.n_groups * p.n_spans, kSimtThreads, 0, st>>>(p); break;
   }
 }
 
@@ -269,7 +279,7 @@ using namespace dcc;
 extern "C" size_t dcc_tree_attention_workspace_bytes(const dcc_kv_pages* cache, const dcc_tree_query* query, int dtype) {
   if (tree_check(cache, query, dtype) != DCC_OK) return 0;
   TreeParams p{};
-  tree_params(*cache, *query, p);
+  tree_params(*cache, *query, dtype, p);
   Workspace ws(nullptr, 0);
   return tree_carve(p, ws);
 }
@@ -282,7 +292,7 @@ extern "C" int dcc_tree_attention(const dcc_kv_pages* cache, const dcc_tree_quer
   if (!q.q || !q.o || !q.context || (q.max_pages > 0 && !q.page_table))
     return fail(DCC_ERR_INVALID_ARGUMENT, "tree_attention: null tensor");
   TreeParams p{};
-  tree_params(*cache, q, p);
+  const bool tc = tree_params(*cache, q, dtype, p);
   p.scale = (float)scale;
   Workspace ws(workspace, workspace_bytes);
   tree_carve(p, ws);
@@ -290,9 +300,13 @@ extern "C" int dcc_tree_attention(const dcc_kv_pages* cache, const dcc_tree_quer
   const int64_t items = (int64_t)q.n_seqs * cache->n_kv_heads * p.n_row_tiles;
   if (items > 2147483647LL) return fail(DCC_ERR_UNSUPPORTED, "tree_attention: too many sequences");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype == DCC_BF16) tree_simt_launch<__nv_bfloat16>(p, st);
-  else tree_simt_launch<float>(p, st);
-  DCC_CHECK(check_launch("tree_attention"));
+  if (tc) {
+    DCC_CHECK(launch_tree_tc05(p, st));
+  } else {
+    if (dtype == DCC_BF16) tree_simt_launch<__nv_bfloat16>(p, st);
+    else tree_simt_launch<float>(p, st);
+    DCC_CHECK(check_launch("tree_attention"));
+  }
   const int rows = (int)std::min<int64_t>(p.n_rows, q.T * p.group);
   const dim3 grid((unsigned)items, (unsigned)((rows + kMergeWarps - 1) / kMergeWarps));
   if (dtype == DCC_BF16) tree_merge_kernel<__nv_bfloat16><<<grid, kMergeWarps * 32, 0, st>>>(p);

@@ -2,14 +2,16 @@
 //
 // The rows of one sequence and KV head -- T newest tokens x `group` query
 // heads, row = t * group + g -- are cut into tiles of `n_rows`, its cached
-// tokens into tiles of 128 keys.  An item is (sequence, KV head, row tile) with
-// all its key tiles.  The key tiles of all items, in that order, form one
-// line that is cut into n_ctas equal spans (+-1 tile; one tile each where there
-// are fewer tiles), whatever the lengths: a CTA walks over its span, and an item that does not lie in one span leaves
-// unnormalised partial results (O, max, sum), which tree_merge_kernel adds in
-// the order of the CTAs -- no atomics, so results repeat bit for bit.  The
-// lengths are read on the device: neither the launch nor a captured graph
-// depends on them.
+// tokens into tiles of 128 keys.  The key tiles of all (sequence, KV head), in
+// that order, form one line that is cut into n_spans equal spans (+-1 tile; one
+// tile each where there are fewer tiles), whatever the lengths.  CTA
+// (span, group) walks over its span for the row tiles group, group + n_groups,
+// ...: the CTAs that read the same keys for other rows are neighbours and run
+// at the same time, so the keys come from HBM once.  A (sequence, KV head) that
+// does not lie in one span leaves unnormalised partial results (O, max, sum),
+// which tree_merge_kernel adds in the order of the spans -- no atomics, so
+// results repeat bit for bit.  The lengths are read on the device: neither the
+// launch nor a captured graph depends on them.
 #pragma once
 
 #include "kv_pages.cuh"
@@ -26,10 +28,14 @@ struct TreeParams {
   int group;    // query heads per KV head
   int n_rows;   // rows per row tile
   int n_row_tiles;
-  int n_ctas;
+  int n_groups, n_spans;
   float scale;
-  float* part_o;   // [n_ctas][2][n_rows][kTreePartCols]
-  float* part_ml;  // [n_ctas][2][n_rows][2]: max, sum
+  float* part_o;   // [n_spans][n_row_tiles][2][n_rows][kTreePartCols]
+  float* part_ml;  // [n_spans][n_row_tiles][2][n_rows][2]: max, sum
+
+  __host__ __device__ int64_t part_row(int span, int rt, int which, int r) const {
+    return (((int64_t)span * n_row_tiles + rt) * 2 + which) * n_rows + r;
+  }
 };
 
 struct SeqTokens {
@@ -53,12 +59,12 @@ __device__ __forceinline__ bool tree_sees(const TreeParams& p, int b, int64_t t,
 }
 
 // n spans of `total` >= n tiles, none empty.
-__device__ __forceinline__ int span_count(int64_t total, int n_ctas) { return (int)(total < n_ctas ? total : n_ctas); }
+__device__ __forceinline__ int span_count(int64_t total, int n_spans) { return (int)(total < n_spans ? total : n_spans); }
 __device__ __forceinline__ int64_t span_begin(int64_t total, int i, int n) { return total * i / n; }
 // The span that holds tile g.
 __device__ __forceinline__ int span_owner(int64_t total, int64_t g, int n) { return (int)(((g + 1) * n - 1) / total); }
 
-// Where a CTA begins: the sequence that holds tile `begin` and the number of
+// Where a span begins: the sequence that holds tile `begin` and the number of
 // its first tile.
 struct TreePlan {
   int64_t total, begin, end, seq_off;
@@ -69,24 +75,24 @@ struct TreePlanSmem {
   TreePlan plan;
 };
 // All threads of the block; ends with a __syncthreads.
-__device__ __forceinline__ void tree_plan(const TreeParams& p, int cta, TreePlanSmem& sm) {
+__device__ __forceinline__ void tree_plan(const TreeParams& p, int span, TreePlanSmem& sm) {
   const int n_thr = blockDim.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, n_warps = (n_thr + 31) >> 5;
-  const int64_t items = (int64_t)p.c.n_kv_heads * p.n_row_tiles;
+  const int64_t heads = p.c.n_kv_heads;
   int64_t sum = 0;
-  for (int b = tid; b < p.q.n_seqs; b += n_thr) sum += items * tree_key_tiles(tree_tokens(p, b));
+  for (int b = tid; b < p.q.n_seqs; b += n_thr) sum += heads * tree_key_tiles(tree_tokens(p, b));
   sum = warp_sum(sum);
   if (lane == 0) sm.warp[warp] = sum;
   __syncthreads();
   int64_t total = 0;
   for (int w = 0; w < n_warps; ++w) total += sm.warp[w];
-  const int n = span_count(total, p.n_ctas);
-  const int64_t begin = cta < n ? span_begin(total, cta, n) : 0, end = cta < n ? span_begin(total, cta + 1, n) : 0;
+  const int n = span_count(total, p.n_spans);
+  const int64_t begin = span < n ? span_begin(total, span, n) : 0, end = span < n ? span_begin(total, span + 1, n) : 0;
   if (tid == 0) sm.plan = TreePlan{total, begin, end, 0, 0};
   if (begin < end) {  // the same for every thread
     int64_t carry = 0;
     for (int b0 = 0; b0 < p.q.n_seqs && carry <= begin; b0 += n_thr) {
       const int b = b0 + tid;
-      const int64_t w = b < p.q.n_seqs ? items * tree_key_tiles(tree_tokens(p, b)) : 0;
+      const int64_t w = b < p.q.n_seqs ? heads * tree_key_tiles(tree_tokens(p, b)) : 0;
       int64_t incl = w;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -111,46 +117,45 @@ __device__ __forceinline__ void tree_plan(const TreeParams& p, int cta, TreePlan
   __syncthreads();
 }
 
-// The pieces of a CTA's span, one item (or the part of it in the span) after
-// the other.  Every role of a CTA walks the same pieces.
+// The pieces of a span, one (sequence, KV head) or the part of it in the span
+// after the other.  Every role of a CTA walks the same pieces.
 struct TreePiece {
-  int b, hk, rt;
-  int64_t k0, k1;  // key tiles
+  int b, hk;
+  int k0, k1;  // key tiles
   SeqTokens s;
-  int part;        // -1: the whole item, else the partial slot (0: begun by an earlier CTA, 1: begun here)
+  int part;    // -1: all keys, else the partial slot (0: begun by an earlier span, 1: begun here)
 };
 struct TreeWalk {
-  int64_t g, end, off, tiles;  // next tile, end of span, first tile of sequence b, key tiles of b
-  int b;
+  int64_t g, end, off;  // next tile, end of span, first tile of sequence b
+  int tiles, b;         // key tiles of b
   SeqTokens s;
   __device__ __forceinline__ void start(const TreeParams& p, const TreePlan& pl) {
     g = pl.begin;
     end = pl.end;
     off = pl.seq_off;
     b = pl.seq;
+    tiles = 0;
     if (g < end) {
       s = tree_tokens(p, b);
-      tiles = tree_key_tiles(s);
+      tiles = (int)tree_key_tiles(s);
     }
   }
   __device__ __forceinline__ bool next(const TreeParams& p, TreePiece& o) {
     if (g >= end) return false;
-    const int64_t items = (int64_t)p.c.n_kv_heads * p.n_row_tiles;
-    while (g >= off + items * tiles) {  // ends: g < end <= the tiles of all sequences
-      off += items * tiles;
+    while (g >= off + (int64_t)p.c.n_kv_heads * tiles) {  // ends: g < end <= the tiles of all sequences
+      off += (int64_t)p.c.n_kv_heads * tiles;
       s = tree_tokens(p, ++b);
-      tiles = tree_key_tiles(s);
+      tiles = (int)tree_key_tiles(s);
     }
-    const int64_t item = (g - off) / tiles, first = off + item * tiles, last = first + tiles;
-    const int64_t stop = last < end ? last : end;
+    const int64_t in_seq = g - off;
+    o.hk = (int)(in_seq / tiles);
+    o.k0 = (int)(in_seq - (int64_t)o.hk * tiles);
+    const int64_t left = end - g;
+    o.k1 = left < tiles - o.k0 ? o.k0 + (int)left : tiles;
     o.b = b;
-    o.hk = (int)(item / p.n_row_tiles);
-    o.rt = (int)(item - (int64_t)o.hk * p.n_row_tiles);
-    o.k0 = g - first;
-    o.k1 = stop - first;
     o.s = s;
     o.part = o.k0 > 0 ? 0 : (o.k1 < tiles ? 1 : -1);
-    g = stop;
+    g += o.k1 - o.k0;
     return true;
   }
 };
@@ -174,5 +179,10 @@ template <typename T>
 __device__ __forceinline__ T* tree_out_row(const TreeParams& p, int b, const TreeRow& r) {
   return static_cast<T*>(p.q.o) + b * p.q.o_seq_stride + r.h * p.q.o_head_stride + r.t * p.q.o_row_stride;
 }
+
+// Tensor-core path: bf16 queries, bf16 or 8-bit cache, head_dim a multiple of 16.
+bool tree_tc05_supported(const dcc_kv_pages& c, const dcc_tree_query& q, int dtype);
+int tree_tc05_rows(int64_t rows);
+int launch_tree_tc05(const TreeParams& p, cudaStream_t st);
 
 }  // namespace dcc

@@ -27,6 +27,12 @@ def tree_mask(parents: Sequence[int]) -> torch.Tensor:
     return sees
 
 
+def _misaligned(q: torch.Tensor) -> bool:
+    """Rows of a bfloat16 tensor that do not start on 16-byte boundaries (the tensor-core kernel needs them)."""
+    sb, sh, st, _ = q.stride()
+    return (q.data_ptr() & 15) != 0 or ((sb | sh | st) & 7) != 0
+
+
 def tree_attention(q: torch.Tensor, cache: KvCache, page_table: torch.Tensor, context_lens: torch.Tensor,
                    counts: Optional[torch.Tensor] = None, tree: Optional[torch.Tensor] = None,
                    scale: Optional[float] = None) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -60,8 +66,8 @@ def tree_attention(q: torch.Tensor, cache: KvCache, page_table: torch.Tensor, co
     L.require_cuda(q, cache.k, page_table)
     check_table(cache, b, page_table=page_table, context_lens=context_lens, counts=counts)
     L.same_device(dev, q=q, tree=tree)
-    if q.stride(3) != 1 and d > 1:
-        q = q.contiguous()
+    if (q.stride(3) != 1 and d > 1) or (q.dtype == torch.bfloat16 and _misaligned(q)):
+        q = q.clone(memory_format=torch.contiguous_format)
     code = L.dtype_code(q)
     with L.on_device(dev):
         o = torch.empty(b, hq, t, d, dtype=q.dtype, device=dev)
