@@ -57,6 +57,7 @@ int attn_error_flag_address(unsigned int** out);
 namespace tt {
 
 constexpr int kRing = 8;  // scales and masks of the last K tiles
+constexpr int kFetch = 4;   // K tiles between a page lookup and its use
 constexpr int kLead = 2;    // tiles that copies of K run ahead of V
 constexpr int kPieces = 8;  // queries of a piece are written once the scores of the one before are issued, at
                             // most kStreams tiles ahead of the softmax: 5 pieces of one tile
@@ -78,7 +79,7 @@ struct Shape {
   static constexpr uint32_t kColS = 0, kColO = kStreams * kN;
   static constexpr int kTmem = 2 * kStreams * kN;
   static constexpr int kArrays = k8 ? 3 : 1;          // bias; K and V scales
-  static constexpr size_t kFixed = (size_t)kQ + kP + (size_t)kRing * kArrays * 512 + 640 + kN * 128;
+  static constexpr size_t kFixed = (size_t)kQ + kP + (size_t)kRing * kArrays * 512 + 896 + kN * 128;
   static constexpr int kFit = (int)((kSmemLimit - kFixed) / kTile);
   static constexpr int kSlotsV = (kFit + 1) / 2 < 4 ? (kFit + 1) / 2 : 4, kSlotsK = kFit / 2 < 4 ? kFit / 2 : 4;
   static constexpr int kSlots = kSlotsK + kSlotsV;
@@ -106,6 +107,7 @@ struct Smem {
   unsigned char p[X::kP];
   __align__(16) float side[kRing][X::kArrays][128];  // bias, k_scale, v_scale
   __align__(16) uint8_t vis[kRing][16];               // bits: keys that exist
+  int32_t pages[kFetch][16];                          // of every eighth key of the next K tiles
   __align__(16) float qf[kPieces][kN];                // what undoes the scaling of a query row, by piece
   __align__(16) float m[X::kStreams][kN];
   __align__(16) float sum[X::kStreams][kN];           // while a piece runs: the last rescale
@@ -184,6 +186,9 @@ __device__ __forceinline__ bool group_any(int wg, bool x) {
       : "r"((uint32_t)x), "r"(1 + wg)
       : "memory");
   return r != 0;
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ uint4 ld_shared_v4(uint32_t a) {
   uint4 v;
@@ -269,7 +274,6 @@ template <int kMode, int kD, int kN>
 __device__ __forceinline__ void copies(const TreeParams& p, const TreeMaps& maps, SmemOf<kMode, kD, kN>& sm, int n, int lane,
                                        bool& ok) {
   using X = Shape<kMode, kD, kN>;
-  constexpr int kFetch = 3;  // tiles between a page lookup and its use
   const TreePlan& pl = sm.span;
   const uint32_t row_bytes = (uint32_t)p.c.head_dim * (X::k8 ? 1 : 2);
   const bool pow2 = (p.c.page_size & (p.c.page_size - 1)) == 0;
@@ -285,26 +289,39 @@ __device__ __forceinline__ void copies(const TreeParams& p, const TreeMaps& maps
   const uint32_t slot0 = smem_u32(sm.slot[0]) + (uint32_t)lane * 1024;
   Tiles t;
   t.start(p, pl);
-  // lane < 16: the page of rows 8 lane .. 8 lane + 7 of the next K tiles (a page
-  // holds all eight or none), the row in the page, the rows that exist
-  int page[kFetch], add[kFetch], left[kFetch];
+  // lane < 16: rows 8 lane .. 8 lane + 7 of a tile (a page holds all eight or
+  // none).  Their page numbers are on their way to shared memory kFetch tiles
+  // ahead -- a register that waits for a load would stall the warp when the
+  // queue moves on --, the row in the page and the rows that exist are known
+  int add[kFetch], left[kFetch];
   int fetched = 0;
-  auto fetch = [&](int i) {
-    page[i] = -1;
+  auto fetch = [&]() {
+    left[kFetch - 1] = 0;
     if (fetched < n) {
       t.next(p, pl);
       const int pos = t.kt * kTreeKeys + 8 * lane;
-      left[i] = (int)(t.w.s.total - pos);
-      if (lane < 16 && left[i] > 0) {
+      left[kFetch - 1] = lane < 16 ? (int)(t.w.s.total - pos) : 0;
+      if (left[kFetch - 1] > 0) {
         const int s = pow2 ? pos >> shift : pos / p.c.page_size;
-        add[i] = t.w.hk * p.c.page_size + pos - s * p.c.page_size;
-        page[i] = __ldg(p.q.page_table + (int64_t)t.w.b * p.q.table_stride + s);
+        add[kFetch - 1] = t.w.hk * p.c.page_size + pos - s * p.c.page_size;
+        cp_async4(smem_u32(&sm.pages[fetched % kFetch][lane]), p.q.page_table + (int64_t)t.w.b * p.q.table_stride + s);
       }
       ++fetched;
     }
+    asm volatile("cp.async.commit_group;\n" ::: "memory");
   };
+  auto shift_down = [&]() {
 #pragma unroll
-  for (int i = 0; i < kFetch; ++i) fetch(i);
+    for (int f = 0; f + 1 < kFetch; ++f) {
+      add[f] = add[f + 1];
+      left[f] = left[f + 1];
+    }
+  };
+#pragma unroll 1
+  for (int i = 0; i < kFetch; ++i) {
+    shift_down();
+    fetch();
+  }
   const int page_step = p.c.n_kv_heads * p.c.page_size;
   static_assert(kLead == 2, "rows of the last K tiles");
   int row0 = -1, row1 = -1, row2 = -1;  // of the latest K tile and the two before
@@ -321,7 +338,12 @@ __device__ __forceinline__ void copies(const TreeParams& p, const TreeMaps& maps
       slot = at_k.slot;
       if (kj >= X::kSlotsK) wait_or_skip(ok, &sm.bar_empty[slot], at_k.use ^ 1);
       const int ring = kj % kRing;
-      row = page[0] >= 0 && page[0] < p.c.n_pages ? page[0] * page_step + add[0] : -1;
+      asm volatile("cp.async.wait_group %0;\n" ::"n"(kFetch - 1) : "memory");  // this lane's own page number
+      row = -1;
+      if (left[0] > 0) {
+        const int page = sm.pages[kj % kFetch][lane];
+        if (page >= 0 && page < p.c.n_pages) row = page * page_step + add[0];
+      }
       if (lane < 16) {
         sm.vis[ring][lane] = row >= 0 ? (uint8_t)(left[0] >= 8 ? 0xff : (1 << left[0]) - 1) : (uint8_t)0;
       }
@@ -363,13 +385,8 @@ __device__ __forceinline__ void copies(const TreeParams& p, const TreeMaps& maps
       }
     }
     if (is_k) {
-#pragma unroll
-      for (int f = 0; f + 1 < kFetch; ++f) {
-        page[f] = page[f + 1];
-        add[f] = add[f + 1];
-        left[f] = left[f + 1];
-      }
-      fetch(kFetch - 1);
+      shift_down();
+      fetch();
       ++kj;
       at_k.next();
     } else {
@@ -377,6 +394,7 @@ __device__ __forceinline__ void copies(const TreeParams& p, const TreeMaps& maps
       at_v.next();
     }
   }
+  asm volatile("cp.async.wait_all;\n" ::: "memory");
 }
 
 // ---- 8-bit: codes to values ----------------------------------------------------------------
