@@ -228,19 +228,36 @@ __global__ void __launch_bounds__(kMergeWarps * 32) tree_merge_kernel(const __gr
         l == 0.f ? -INFINITY : m + logf(l);
 }
 
-static bool tree_params(const dcc_kv_pages& c, const dcc_tree_query& q, int dtype, TreeParams& p) {
+bool tree_tensor_supported(const dcc_kv_pages& c, const dcc_tree_query& q, int dtype) {
+  // rows of 16-byte chunks, eight rows that never leave their page
+  if (dtype != DCC_BF16 || c.format == DCC_KV_F32 || c.head_dim % 16 != 0 || c.page_size % 8 != 0) return false;
+  auto aligned = [](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15u) == 0; };
+  for (const void* x : {(const void*)c.k, (const void*)c.v, (const void*)c.k_scale, (const void*)c.v_scale,
+                        (const void*)c.bias, (const void*)q.q})
+    if (!aligned(x)) return false;
+  if (q.q_seq_stride % 8 || q.q_head_stride % 8 || q.q_row_stride % 8) return false;
+  // positions, cache rows and the tiles of a CTA are counted in 32 bits
+  const int64_t cap = (int64_t)q.max_pages * c.page_size;
+  return cap < 0x7fffff00LL && c.n_pages * c.n_kv_heads * c.page_size < 0x7fffff00LL &&
+         (double)q.n_seqs * (double)q.T * q.n_q_heads * (double)(cap + 128) < 1e15;
+}
+
+// Which kernel takes a call, with how many query rows per KV head at a time.
+enum class Path { kSimt, kMma, kTc05 };
+
+static Path tree_params(const dcc_kv_pages& c, const dcc_tree_query& q, int dtype, TreeParams& p) {
   p.c = c;
   p.q = q;
   p.group = q.n_q_heads / c.n_kv_heads;
-  const bool tc = tree_tc05_supported(c, q, dtype);
   const int64_t rows = q.T * p.group;
-  p.n_rows = tc ? tree_tc05_rows(rows) : kSimtRows;
+  const Path path = !tree_tensor_supported(c, q, dtype) ? Path::kSimt : rows <= 32 ? Path::kMma : Path::kTc05;
+  p.n_rows = path == Path::kSimt ? kSimtRows : rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
   p.n_row_tiles = (int)((rows + p.n_rows - 1) / p.n_rows);
-  const int ctas = num_sms() * (tc ? 1 : kSimtCtasPerSm);
+  const int ctas = num_sms() * (path == Path::kSimt ? kSimtCtasPerSm : 1);
   const int rounds = (p.n_row_tiles + ctas - 1) / ctas;
   p.n_groups = rounds > 0 ? (p.n_row_tiles + rounds - 1) / rounds : 1;
   p.n_spans = ctas / p.n_groups;
-  return tc;
+  return path;
 }
 
 static size_t tree_carve(TreeParams& p, Workspace& ws) {
@@ -292,7 +309,7 @@ extern "C" int dcc_tree_attention(const dcc_kv_pages* cache, const dcc_tree_quer
   if (!q.q || !q.o || !q.context || (q.max_pages > 0 && !q.page_table))
     return fail(DCC_ERR_INVALID_ARGUMENT, "tree_attention: null tensor");
   TreeParams p{};
-  const bool tc = tree_params(*cache, q, dtype, p);
+  const Path path = tree_params(*cache, q, dtype, p);
   p.scale = (float)scale;
   Workspace ws(workspace, workspace_bytes);
   tree_carve(p, ws);
@@ -300,7 +317,9 @@ extern "C" int dcc_tree_attention(const dcc_kv_pages* cache, const dcc_tree_quer
   const int64_t items = (int64_t)q.n_seqs * cache->n_kv_heads * p.n_row_tiles;
   if (items > 2147483647LL) return fail(DCC_ERR_UNSUPPORTED, "tree_attention: too many sequences");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (tc) {
+  if (path == Path::kMma) {
+    DCC_CHECK(launch_tree_mma(p, st));
+  } else if (path == Path::kTc05) {
     DCC_CHECK(launch_tree_tc05(p, st));
   } else {
     if (dtype == DCC_BF16) tree_simt_launch<__nv_bfloat16>(p, st);

@@ -180,9 +180,11 @@ __device__ __forceinline__ T* tree_out_row(const TreeParams& p, int b, const Tre
   return static_cast<T*>(p.q.o) + b * p.q.o_seq_stride + r.h * p.q.o_head_stride + r.t * p.q.o_row_stride;
 }
 
-// Tensor-core path: bf16 queries, bf16 or 8-bit cache, head_dim a multiple of 16.
-bool tree_tc05_supported(const dcc_kv_pages& c, const dcc_tree_query& q, int dtype);
-int tree_tc05_rows(int64_t rows);
+// The tensor-core kernels: bf16 queries, bf16 or 8-bit cache, head_dim a
+// multiple of 16, page_size of 8.  tree_mma.cu for up to 32 rows per KV head,
+// tree_tc05.cu for more.
+bool tree_tensor_supported(const dcc_kv_pages& c, const dcc_tree_query& q, int dtype);
+int launch_tree_mma(const TreeParams& p, cudaStream_t st);
 int launch_tree_tc05(const TreeParams& p, cudaStream_t st);
 
 }  // namespace dcc

@@ -1022,24 +1022,6 @@ static int launch_d(const TreeParams& p, const TreeMaps& maps, unsigned int* err
 
 }  // namespace tt
 
-bool tree_tc05_supported(const dcc_kv_pages& c, const dcc_tree_query& q, int dtype) {
-  // rows of 16-byte chunks, eight rows that never leave their page
-  if (dtype != DCC_BF16 || c.format == DCC_KV_F32 || c.head_dim % 16 != 0 || c.page_size % 8 != 0) return false;
-  auto aligned = [](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15u) == 0; };
-  for (const void* x : {(const void*)c.k, (const void*)c.v, (const void*)c.k_scale, (const void*)c.v_scale,
-                        (const void*)c.bias, (const void*)q.q})
-    if (!aligned(x)) return false;
-  if (q.q_seq_stride % 8 || q.q_head_stride % 8 || q.q_row_stride % 8) return false;
-  // positions, cache rows and the tiles of a CTA are counted in 32 bits
-  const int64_t cap = (int64_t)q.max_pages * c.page_size;
-  return cap < 0x7fffff00LL && c.n_pages * c.n_kv_heads * c.page_size < 0x7fffff00LL &&
-         (double)q.n_seqs * (double)q.T * q.n_q_heads * (double)(cap + 128) < 1e15;
-}
-
-// Query rows per tile = N of the MMAs: the smallest that takes all rows, since
-// a span reads its keys once for each tile.
-int tree_tc05_rows(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
-
 int launch_tree_tc05(const TreeParams& p, cudaStream_t st) {
   unsigned int* error = nullptr;
   DCC_CHECK(attn_error_flag_address(&error));
