@@ -167,10 +167,11 @@ struct TreeRow {
   bool exists;
 };
 __device__ __forceinline__ TreeRow tree_row(const TreeParams& p, int hk, int rt, int r) {
-  const int64_t row = (int64_t)rt * p.n_rows + r;
+  const int row = rt * p.n_rows + r;  // the rows of a KV head are fewer than 2^25
+  const int t = row / p.group;
   TreeRow o;
-  o.t = row / p.group;
-  o.h = hk * p.group + (int)(row - o.t * p.group);
+  o.t = t;
+  o.h = hk * p.group + row - t * p.group;
   o.exists = o.t < p.q.T;
   return o;
 }

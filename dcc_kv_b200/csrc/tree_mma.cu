@@ -7,13 +7,15 @@
 // the bytes that it will feed to its own MMA operands, so the shared memory
 // ring is private to the lane: no barriers, no swizzle, no second trip through
 // shared memory for widened codes.  The contractions are register MMAs
-// (m16n8k16, 16 query rows), which are far from their limit:
-//   S [16 rows, 8 keys]  += Q K^T    the k index runs over d in the order in
-//                                    which a lane's 16-byte chunks hold it
-//   O [16 rows, 8 cols]  += P V      column n of n-tile j stands for the
-//                                    element of V that lane group n holds as
-//                                    its j-th, so pairs of keys are joined by
-//                                    byte permutes and never transposed
+// (m16n8k16) with keys, then head columns, as the 16 rows and query rows as the
+// 8 columns -- four query heads and one token fill half of a tile:
+//   S^T [16 keys, 8 rows]  += K Q^T    the k index runs over d in the order in
+//                                      which a lane's 16-byte chunks hold it
+//   O^T [16 cols, 8 rows]  += V^T P^T  rows n and n + 8 of tile i stand for
+//                                      elements 2 i and 2 i + 1 of the chunk of V
+//                                      that lane group n holds, so pairs of keys
+//                                      are joined by byte permutes
+// (P^T is transposed between the two by movmatrix.)
 // Codes become fp16, exactly; scales act on S and P in fp32.  Beside them the
 // queries are held in fp16 too, each row scaled by a power of two that takes
 // its largest element to 2^14: bf16 digits fit, and what falls below fp16's
@@ -24,6 +26,7 @@
 // fp16 beside codes (2^-12): there P carries the V scale, so the max is taken
 // over score + log2(scale), which keeps P below 2^8 whatever the scales are.
 #include <string>
+#include <type_traits>
 
 #include "tree_attention.cuh"
 
@@ -32,48 +35,48 @@ namespace tm {
 
 constexpr size_t kSmemLimit = 232448;
 
-template <int kMode, int kD, int kMT>  // cache format, padded head_dim, 16-row tiles
+template <int kMode, int kD, int kNT>  // cache format, padded head_dim, 8-row tiles
 struct Shape {
   static constexpr bool k8 = kMode != DCC_KV_BF16;
-  // as many warps as the registers of a warp allow (and the ring has to hold
-  // 64 KB and more in flight)
-  static constexpr int kWarps = k8 && kMT == 1 ? 12 : 8;
+  // as many warps as the registers of a warp and the ring (64 KB and more in
+  // flight) allow
+  static constexpr int kWarps = k8 ? (kNT == 1 ? 16 : kNT == 2 ? 12 : 8) : (kNT == 1 ? 12 : 8);
   static constexpr int kThreads = 32 * kWarps;
   static constexpr int kE = k8 ? 16 : 8;             // elements of a 16-byte chunk
   static constexpr int kKC = kD / (4 * kE);          // K chunks of a lane and key
   static constexpr int kVC = k8 ? 1 : kD / 64;       // V chunks of a lane and key
   static constexpr int kVB = k8 ? kD / 8 : 16;       // bytes of one
   static constexpr int kSteps = kD / 16;             // k steps of S
-  static constexpr int kTiles = kD / 8;              // n-tiles of O
+  static constexpr int kTiles = kD / 16;             // 16-column tiles of O
   static constexpr int kK = 32 * 2 * kKC * 16, kV = 32 * 4 * kVC * kVB, kSide = 3 * 64;
   static constexpr int kStage = kK + kV + kSide;     // 16 keys of a warp
   // operands of the queries: in registers, or, where O takes those, in shared memory
-  static constexpr bool kQShared = k8 || kMT == 2;
-  static constexpr int kQ = kQShared ? kMT * kSteps * 512 : 16;
+  static constexpr bool kQShared = k8 ? kNT > 1 : kNT == 4;
+  static constexpr int kQ = kQShared ? kNT * kSteps * 256 : 16;
   static constexpr int kSum = kWarps * 2 * kD * 4;   // O of two rows of every warp
-  static constexpr size_t kFixed = kSum + (size_t)kWarps * 16 * kMT * 8 + kWarps * 64 + kQ + 1024;
+  static constexpr size_t kFixed = kSum + (size_t)kWarps * 8 * kNT * 8 + kWarps * 64 + kQ + 1024;
   static constexpr int kFit = (int)((kSmemLimit - kFixed) / ((size_t)kStage * kWarps));
   static constexpr int kStages = kFit < 6 ? kFit : 6;
   static_assert(kStages >= 2, "ring");
 };
 
-template <typename X, int kMT>
+template <typename X, int kNT>
 struct Smem {
   unsigned char ring[X::kWarps][X::kStages][X::kStage];
   float sum[X::kSum / 4];
   __align__(16) unsigned char q[X::kQ];
-  float m[X::kWarps][16 * kMT], l[X::kWarps][16 * kMT];
+  float m[X::kWarps][8 * kNT], l[X::kWarps][8 * kNT];
   int2 info[X::kWarps][X::kStages];  // keys that exist (16 bits), first key behind the context
   TreePlanSmem plan;
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 template <int kBytes>
-__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool real) {
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, uint32_t size) {  // size < kBytes: zeros follow
   if constexpr (kBytes == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(size) : "memory");
   else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;\n" ::"r"(dst), "l"(src), "r"(real ? 8 : 0) : "memory");
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;\n" ::"r"(dst), "l"(src), "r"(size) : "memory");
 }
 template <int kWords>
 __device__ __forceinline__ void load_words(uint32_t a, uint32_t* w) {
@@ -81,11 +84,6 @@ __device__ __forceinline__ void load_words(uint32_t a, uint32_t* w) {
     asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(a) : "memory");
   else
     asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];\n" : "=r"(w[0]), "=r"(w[1]) : "r"(a) : "memory");
-}
-__device__ __forceinline__ float2 load_pair(uint32_t a) {
-  float2 v;
-  asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];\n" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
-  return v;
 }
 template <bool kHalf>
 __device__ __forceinline__ void mma(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
@@ -99,6 +97,17 @@ __device__ __forceinline__ void mma(float* c, const uint32_t* a, uint32_t b0, ui
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};\n"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Transposes an 8 x 8 matrix of 16-bit numbers held two to a lane.
+__device__ __forceinline__ uint32_t transpose(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ float load_one(uint32_t a) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];\n" : "=f"(v) : "r"(a) : "memory");
+  return v;
 }
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
@@ -150,37 +159,44 @@ __device__ __forceinline__ uint32_t join_codes(uint32_t a, uint32_t b, int q) {
   }
 }
 
-// The tile that a chunk of 16 keys lies in, for chunks that only grow.
+// The position of a warp's next chunk of 16 keys.
 struct Cursor {
   TreeWalk walk;
   TreePiece w;
-  int rt, first;  // first tile of the piece, counted over the CTA
+  int rt, pos, end;  // end of the piece
+  __device__ __forceinline__ void open(const TreeParams& p, const TreePlan& pl) {
+    if (!walk.next(p, w)) {
+      rt += p.n_groups;
+      walk.start(p, pl);
+      walk.next(p, w);
+    }
+    pos = w.k0 * kTreeKeys;
+    end = w.k1 * kTreeKeys;
+  }
   __device__ __forceinline__ void start(const TreeParams& p, const TreePlan& pl) {
     rt = blockIdx.x % p.n_groups;
     walk.start(p, pl);
-    first = 0;
-    walk.next(p, w);
+    open(p, pl);
   }
-  __device__ __forceinline__ void seek(const TreeParams& p, const TreePlan& pl, int tile) {
-    while (tile >= first + w.k1 - w.k0) {
-      first += w.k1 - w.k0;
-      if (!walk.next(p, w)) {
-        rt += p.n_groups;
-        walk.start(p, pl);
-        walk.next(p, w);
-      }
+  // over `keys` more of the CTA's line, which does not end before them
+  __device__ __forceinline__ void move(const TreeParams& p, const TreePlan& pl, int keys) {
+    pos += keys;
+    while (pos >= end) {
+      const int over = pos - end;
+      open(p, pl);
+      pos += over;
     }
   }
 };
 
-template <int kMode, int kD, int kMT>
-__global__ void __launch_bounds__(Shape<kMode, kD, kMT>::kThreads, 1) tree_mma_kernel(const __grid_constant__ TreeParams p) {
-  using X = Shape<kMode, kD, kMT>;
+template <int kMode, int kD, int kNT>
+__global__ void __launch_bounds__(Shape<kMode, kD, kNT>::kThreads, 1) tree_mma_kernel(const __grid_constant__ TreeParams p) {
+  using X = Shape<kMode, kD, kNT>;
   constexpr bool k8 = X::k8;
-  constexpr int kRows = 16 * kMT, S = X::kStages, NW = X::kWarps;
+  constexpr int kRows = 8 * kNT, S = X::kStages, NW = X::kWarps;
   constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f, kMost = 3.402823466e38f;
   extern __shared__ __align__(16) unsigned char smem_raw[];
-  Smem<X, kMT>& sm = *reinterpret_cast<Smem<X, kMT>*>(smem_raw);
+  Smem<X, kNT>& sm = *reinterpret_cast<Smem<X, kNT>*>(smem_raw);
   const int span = blockIdx.x / p.n_groups;
   tree_plan(p, span, sm.plan);
   const TreePlan pl = sm.plan.plan;
@@ -198,78 +214,117 @@ __global__ void __launch_bounds__(Shape<kMode, kD, kMT>::kThreads, 1) tree_mma_k
   const bool guard = p.q.T > 1 || p.q.tree != nullptr;  // rows may hide newest tokens from one another
 
   // ---- copies of this warp's chunks, kStages - 1 ahead ----
-  Cursor at;
-  at.start(p, pl);
   const bool pow2 = (p.c.page_size & (p.c.page_size - 1)) == 0;
   const int shift = 31 - __clz(p.c.page_size);
+  const bool one_page = p.c.page_size % 16 == 0;  // a chunk never leaves its page
   const int page_step = p.c.n_kv_heads * p.c.page_size;
-  int next = warp, put = 0;  // chunk, stage
-  // pages of keys 0 .. 7 and 8 .. 15 of the next chunk, looked up a chunk ahead
-  int page[2] = {-1, -1}, add[2] = {0, 0}, left = 0, rel = 0;
-  auto look_up = [&]() {
-    if (next >= chunks) return;
-    at.seek(p, pl, next >> 3);
-    const int pos = (at.w.k0 + (next >> 3) - at.first) * kTreeKeys + 16 * (next & 7);
-    left = (int)min(at.w.s.total - pos, (int64_t)16);
-    const int64_t behind = pos - at.w.s.ctx;
-    rel = (int)(behind < -64 ? -64 : behind);
-    const int32_t* table = p.q.page_table + (int64_t)at.w.b * p.q.table_stride;
+  // what this lane copies of a row: chunks of K (key g of eight) and V (keys 2 t
+  // and 2 t + 1 of eight); nothing past head_dim
+  uint32_t k_off[X::kKC], k_size[X::kKC], v_off[X::kVC], v_size[X::kVC];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      page[h] = -1;
-      if (left > 8 * h) {
-        const int q = pos + 8 * h, s = pow2 ? q >> shift : q / p.c.page_size;
-        add[h] = at.w.hk * p.c.page_size + q - s * p.c.page_size;
-        page[h] = __ldg(table + s);
-      }
+  for (int c = 0; c < X::kKC; ++c) {
+    const bool real = (4 * c + t) * X::kE < d;
+    k_off[c] = (uint32_t)g * row_bytes + (real ? 64u * c + 16u * t : 0u);
+    k_size[c] = real ? 16 : 0;
+  }
+#pragma unroll
+  for (int c = 0; c < X::kVC; ++c) {
+    const bool real = X::kVB * g + 128 * c < (int)row_bytes;
+    v_off[c] = (uint32_t)(2 * t) * row_bytes + (real ? (uint32_t)(X::kVB * g + 128 * c) : 0u);
+    v_size[c] = real ? X::kVB : 0;
+  }
+  // and of the 16 keys' bias, K and V scales: four of one of them
+  const int side_kind = lane >> 2, side_key = 4 * t;
+  const float* side_src = side_kind == 0 ? p.c.bias : side_kind == 1 ? p.c.k_scale : side_kind == 2 ? p.c.v_scale : nullptr;
+  const unsigned char* const k_src = static_cast<const unsigned char*>(p.c.k);
+  const unsigned char* const v_src = static_cast<const unsigned char*>(p.c.v);
+  Cursor at;
+  at.start(p, pl);
+  at.move(p, pl, warp < chunks ? 16 * warp : 0);
+  int todo = warp < chunks ? (chunks - warp + NW - 1) / NW : 0, put = 0;  // chunks to copy, stage
+  // pages of keys 0 .. 7 and 8 .. 15 of the next chunk, looked up a chunk ahead
+  int page_a = -1, page_b = -1, add_a = 0, add_b = 0, left = 0, rel = 0;
+  auto look_up = [&]() {
+    const int32_t* table = p.q.page_table + (int64_t)at.w.b * p.q.table_stride;
+    left = (int)at.w.s.total - at.pos;
+    const int64_t behind = at.pos - at.w.s.ctx;
+    rel = behind < -64 ? -64 : (int)behind;
+    page_a = page_b = -1;
+    if (left > 0) {
+      const int q = pow2 ? at.pos >> shift : at.pos / p.c.page_size;
+      add_a = at.w.hk * p.c.page_size + at.pos - q * p.c.page_size;
+      page_a = __ldg(table + q);
+    }
+    if (!one_page && left > 8) {
+      const int pos = at.pos + 8, q = pow2 ? pos >> shift : pos / p.c.page_size;
+      add_b = at.w.hk * p.c.page_size + pos - q * p.c.page_size;
+      page_b = __ldg(table + q);
     }
   };
   auto issue = [&]() {
-    if (next < chunks) {
-      const bool okA = page[0] >= 0 && page[0] < p.c.n_pages, okB = page[1] >= 0 && page[1] < p.c.n_pages;
-      const int nA = okA ? min(max(left, 0), 8) : 0, nB = okB ? min(max(left - 8, 0), 8) : 0;
-      const int rowA = nA ? page[0] * page_step + add[0] : 0, rowB = nB ? page[1] * page_step + add[1] : 0;
+    if (todo > 0) {
       const uint32_t to = (uint32_t)put * X::kStage;
-      const unsigned char* k = static_cast<const unsigned char*>(p.c.k);
-      const unsigned char* v = static_cast<const unsigned char*>(p.c.v);
+      const bool in_a = page_a >= 0 && page_a < p.c.n_pages;
+      if (one_page && in_a && left >= 16) {
+        const int row = page_a * page_step + add_a;
+        const int64_t off = (int64_t)row * row_bytes;
+        const unsigned char* k = k_src + off;
+        const unsigned char* v = v_src + off;
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const bool key = g < (u ? nB : nA);
-        const unsigned char* src = k + (int64_t)(u ? rowB : rowA) * row_bytes + (key ? (uint32_t)g * row_bytes + 16u * t : 0u);
+        for (int u = 0; u < 2; ++u) {
 #pragma unroll
-        for (int c = 0; c < X::kKC; ++c) {
-          const bool real = key && (4 * c + t) * X::kE < d;
-          copy_async<16>(ring + to + (u * X::kKC + c) * 512, real ? src + 64 * c : k, real);
+          for (int c = 0; c < X::kKC; ++c)
+            copy_async<16>(ring + to + (u * X::kKC + c) * 512, k + (k_off[c] + 8 * u * row_bytes), k_size[c]);
         }
-      }
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {  // keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
-        const int i = 2 * t + (u & 1);
-        const bool key = i < (u >> 1 ? nB : nA);
-        const unsigned char* src = v + (int64_t)(u >> 1 ? rowB : rowA) * row_bytes + (key ? (uint32_t)i * row_bytes + (uint32_t)(X::kVB * g) : 0u);
+        for (int u = 0; u < 4; ++u) {
 #pragma unroll
-        for (int c = 0; c < X::kVC; ++c) {
-          const bool real = key && X::kVB * g + 128 * c < (int)row_bytes;
-          copy_async<X::kVB>(ring_v + to + (u * X::kVC + c) * 32 * X::kVB, real ? src + 128 * c : v, real);
+          for (int c = 0; c < X::kVC; ++c)
+            copy_async<X::kVB>(ring_v + to + (u * X::kVC + c) * 32 * X::kVB, v + (v_off[c] + (8 * (u >> 1) + (u & 1)) * row_bytes),
+                               v_size[c]);
         }
-      }
-      // bias, K and V scales of the 16 keys, four a lane
-      if (k8 || p.c.bias) {
-        const int a = lane >> 2, four = 4 * t;
-        const float* from = a == 0 ? p.c.bias : a == 1 ? p.c.k_scale : p.c.v_scale;
-        if (a < 3 && from) {
-          const bool real = (four & 7) < (four < 8 ? nA : nB);
-          copy_async<16>(ring_side + to + a * 64 + t * 16, real ? from + (four < 8 ? rowA + four : rowB + four - 8) : from, real);
+        if (side_src) copy_async<16>(ring_side + to + side_kind * 64 + t * 16, side_src + row + side_key, 16);
+        // rel >= -15: newest tokens among them
+        if (lane == 0) sm.info[warp][put] = make_int2(0xffff, rel);
+      } else {
+        // the rows that exist; the others become zeros
+        const int pb = one_page ? page_a : page_b, ab = one_page ? add_a + 8 : add_b;
+        const bool in_b = pb >= 0 && pb < p.c.n_pages;
+        const int n_a = in_a ? min(max(left, 0), 8) : 0, n_b = in_b ? min(max(left - 8, 0), 8) : 0;
+        const int rows[2] = {n_a ? page_a * page_step + add_a : 0, n_b ? pb * page_step + ab : 0};
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const bool key = g < (u ? n_b : n_a);
+          const unsigned char* k = k_src + (int64_t)rows[u] * row_bytes;
+#pragma unroll
+          for (int c = 0; c < X::kKC; ++c)
+            copy_async<16>(ring + to + (u * X::kKC + c) * 512, k + (key ? k_off[c] : 0u), key ? k_size[c] : 0);
         }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const bool key = 2 * t + (u & 1) < (u >> 1 ? n_b : n_a);
+          const unsigned char* v = v_src + (int64_t)rows[u >> 1] * row_bytes;
+#pragma unroll
+          for (int c = 0; c < X::kVC; ++c)
+            copy_async<X::kVB>(ring_v + to + (u * X::kVC + c) * 32 * X::kVB, v + (key ? v_off[c] + (u & 1) * row_bytes : 0u),
+                               key ? v_size[c] : 0);
+        }
+        if (side_src) {
+          const bool key = (side_key & 7) < (side_key < 8 ? n_a : n_b);
+          copy_async<16>(ring_side + to + side_kind * 64 + t * 16,
+                         side_src + (key ? rows[side_key >> 3] + (side_key & 7) : 0), key ? 16 : 0);
+        }
+        if (lane == 0) sm.info[warp][put] = make_int2((0xff >> (8 - n_a)) | (0xff >> (8 - n_b)) << 8, rel);
       }
-      if (lane == 0) sm.info[warp][put] = make_int2((0xff >> (8 - nA)) | (0xff >> (8 - nB)) << 8, rel);
-      next += NW;
-      look_up();
+      if (--todo > 0) {
+        at.move(p, pl, 16 * NW);
+        look_up();
+      }
     }
     if (++put == S) put = 0;
     asm volatile("cp.async.commit_group;\n" ::: "memory");
   };
-  look_up();
+  if (todo > 0) look_up();
 #pragma unroll 1
   for (int i = 0; i < S - 1; ++i) issue();
 
@@ -281,67 +336,68 @@ __global__ void __launch_bounds__(Shape<kMode, kD, kMT>::kThreads, 1) tree_mma_k
     TreePiece w;
     while (walk.next(p, w)) {
       const int stop = 8 * (base + w.k1 - w.k0);
-      // queries: rows g and g + 8 of each 16-row tile, four elements a k step
-      uint32_t q[X::kQShared ? 1 : kMT][X::kSteps][4];
-      float unit[kMT][2];  // what undoes their scaling, times the softmax scale
-      int tok[kMT][2];
+      // queries: row g of each tile, four elements a k step
+      uint2 q[X::kQShared ? 1 : kNT][X::kSteps];
+      // of rows 2 t and 2 t + 1: what undoes their scaling, times the softmax scale; the token
+      float unit[kNT][2];
+      int tok[kNT][2];
       if (X::kQShared || mine < stop) {
 #pragma unroll
-        for (int m = 0; m < kMT; ++m) {
-          uint32_t (&qm)[X::kSteps][4] = q[X::kQShared ? 0 : m];
+        for (int m = 0; m < kNT; ++m) {
+          uint2 (&qm)[X::kSteps] = q[X::kQShared ? 0 : m];
+          const TreeRow row = tree_row(p, w.hk, rt, 8 * m + g);
+          const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(p.q.q) + w.b * p.q.q_seq_stride +
+                                     row.h * p.q.q_head_stride + row.t * p.q.q_row_stride;
+          uint32_t top = 0;
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const TreeRow row = tree_row(p, w.hk, rt, 16 * m + 8 * h + g);
-            tok[m][h] = row.exists ? (int)row.t : 0x7fffffff;
-            const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(p.q.q) + w.b * p.q.q_seq_stride +
-                                       row.h * p.q.q_head_stride + row.t * p.q.q_row_stride;
-            uint32_t top = 0;
+          for (int s = 0; s < X::kSteps; ++s) {
+            // the chunk of k step s, and the four elements in it
+            const int c = s / (X::kE / 4), at4 = (4 * c + t) * X::kE + 4 * (s % (X::kE / 4));
+            uint2 v = make_uint2(0u, 0u);
+            if (row.exists && at4 < d) v = *reinterpret_cast<const uint2*>(src + at4);
+            qm[s] = v;
+            top = max(top, max(max((v.x >> 7) & 0xffu, (v.x >> 23) & 0xffu), max((v.y >> 7) & 0xffu, (v.y >> 23) & 0xffu)));
+          }
+          float undo = scale;
+          if constexpr (k8) {
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const int up = top == 0 || top == 255 ? 0 : min(14 + 127 - (int)top, 120);
+            const float f = __uint_as_float((uint32_t)(127 + up) << 23);
+            undo = scale * __uint_as_float((uint32_t)(127 - up) << 23);
 #pragma unroll
             for (int s = 0; s < X::kSteps; ++s) {
-              // the chunk of k step s, and the four elements in it
-              const int c = s / (X::kE / 4), at4 = (4 * c + t) * X::kE + 4 * (s % (X::kE / 4));
-              uint2 v = make_uint2(0u, 0u);
-              if (row.exists && at4 < d) v = *reinterpret_cast<const uint2*>(src + at4);
-              qm[s][h] = v.x;
-              qm[s][2 + h] = v.y;
-              top = max(top, max(max((v.x >> 7) & 0xffu, (v.x >> 23) & 0xffu), max((v.y >> 7) & 0xffu, (v.y >> 23) & 0xffu)));
-            }
-            unit[m][h] = scale;
-            if constexpr (k8) {
-              top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-              top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-              const int up = top == 0 || top == 255 ? 0 : min(14 + 127 - (int)top, 120);
-              const float f = __uint_as_float((uint32_t)(127 + up) << 23);
-              unit[m][h] = scale * __uint_as_float((uint32_t)(127 - up) << 23);
-#pragma unroll
-              for (int s = 0; s < X::kSteps; ++s)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                  const uint32_t x = qm[s][2 * e + h];
-                  qm[s][2 * e + h] = pack<true>(__uint_as_float(x << 16) * f, __uint_as_float(x & 0xffff0000u) * f);
-                }
+              const uint2 x = qm[s];
+              qm[s].x = pack<true>(__uint_as_float(x.x << 16) * f, __uint_as_float(x.x & 0xffff0000u) * f);
+              qm[s].y = pack<true>(__uint_as_float(x.y << 16) * f, __uint_as_float(x.y & 0xffff0000u) * f);
             }
           }
-          // every warp has the same ones; those of the last piece are no longer read
-          if (X::kQShared && warp == m % NW) {
 #pragma unroll
-            for (int s = 0; s < X::kSteps; ++s)
-              *reinterpret_cast<uint4*>(sm.q + ((m * X::kSteps + s) * 32 + lane) * 16) = make_uint4(qm[s][0], qm[s][1], qm[s][2], qm[s][3]);
+          for (int h = 0; h < 2; ++h) {
+            unit[m][h] = __shfl_sync(0xffffffffu, undo, 4 * (2 * t + h));
+            const TreeRow own = tree_row(p, w.hk, rt, 8 * m + 2 * t + h);
+            tok[m][h] = own.exists ? (int)own.t : 0x7fffffff;
+          }
+          // every warp has the same ones; those of the last piece are no longer read
+          if (X::kQShared && warp == m) {
+#pragma unroll
+            for (int s = 0; s < X::kSteps; ++s) *reinterpret_cast<uint2*>(sm.q + ((m * X::kSteps + s) * 32 + lane) * 8) = qm[s];
           }
         }
       }
       if constexpr (X::kQShared) __syncthreads();
-      auto query = [&](int m, int s, uint32_t* a) {
+      auto query = [&](int m, int s) {
         if constexpr (X::kQShared) {
-          load_words<4>(smem_addr(sm.q) + (uint32_t)((m * X::kSteps + s) * 32 + lane) * 16, a);
+          uint32_t a[2];
+          load_words<2>(smem_addr(sm.q) + (uint32_t)((m * X::kSteps + s) * 32 + lane) * 8, a);
+          return make_uint2(a[0], a[1]);
         } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) a[e] = q[m][s][e];
+          return q[m][s];
         }
       };
-      float o[kMT][X::kTiles][4], mx[kMT][2], l[kMT][2];
+      float o[kNT][X::kTiles][4], mx[kNT][2], l[kNT][2];
 #pragma unroll
-      for (int m = 0; m < kMT; ++m) {
+      for (int m = 0; m < kNT; ++m) {
         mx[m][0] = mx[m][1] = -INFINITY;
         l[m][0] = l[m][1] = 0.f;
 #pragma unroll
@@ -355,166 +411,158 @@ __global__ void __launch_bounds__(Shape<kMode, kD, kMT>::kThreads, 1) tree_mma_k
         const uint32_t from = (uint32_t)get * X::kStage;
         const int2 info = sm.info[warp][get];
         if (++get == S) get = 0;
-        // ---- scores ----
-        float s[kMT][2][4];
+        // ---- scores: keys g (e < 2) and g + 8, rows 2 t + (e & 1) ----
+        float s[kNT][4];
 #pragma unroll
-        for (int m = 0; m < kMT; ++m)
+        for (int m = 0; m < kNT; ++m) s[m][0] = s[m][1] = s[m][2] = s[m][3] = 0.f;
 #pragma unroll
-          for (int u = 0; u < 2; ++u) s[m][u][0] = s[m][u][1] = s[m][u][2] = s[m][u][3] = 0.f;
+        for (int c = 0; c < X::kKC; ++c) {
+          uint32_t kw[2][4];
+          load_words<4>(ring + from + c * 512, kw[0]);
+          load_words<4>(ring + from + (X::kKC + c) * 512, kw[1]);
+          constexpr int kPer = X::kE / 4;  // k steps of a chunk
 #pragma unroll
-        for (int c = 0; c < X::kKC; ++c)
+          for (int x = 0; x < kPer; ++x) {
+            uint32_t a[4];
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            uint32_t kw[4];
-            load_words<4>(ring + from + (u * X::kKC + c) * 512, kw);
-            if constexpr (k8) {
-#pragma unroll
-              for (int x = 0; x < 4; ++x) {
-                uint32_t b0, b1;
-                widen_word<kMode>(kw[x], b0, b1);
-#pragma unroll
-                for (int m = 0; m < kMT; ++m) {
-                  uint32_t a[4];
-                  query(m, 4 * c + x, a);
-                  mma<true>(s[m][u], a, b0, b1);
-                }
+            for (int u = 0; u < 2; ++u) {
+              if constexpr (k8) {
+                widen_word<kMode>(kw[u][x], a[u], a[2 + u]);
+              } else {
+                a[u] = kw[u][2 * x];
+                a[2 + u] = kw[u][2 * x + 1];
               }
-            } else {
+            }
 #pragma unroll
-              for (int x = 0; x < 2; ++x)
-#pragma unroll
-                for (int m = 0; m < kMT; ++m) {
-                  uint32_t a[4];
-                  query(m, 2 * c + x, a);
-                  mma<false>(s[m][u], a, kw[2 * x], kw[2 * x + 1]);
-                }
+            for (int m = 0; m < kNT; ++m) {
+              const uint2 b = query(m, kPer * c + x);
+              mma<k8>(s[m], a, b.x, b.y);
             }
           }
-        // ---- scale, bias, mask ----
-        float2 bias[2], ks[2], vs[2], lift[2];
-        uint32_t broken = 0;
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          bias[u] = make_float2(0.f, 0.f);
-          lift[u] = make_float2(0.f, 0.f);
-          if (p.c.bias) {
-            bias[u] = load_pair(ring_side + from + 32 * u + 8 * t);
-            if (bias[u].x > -INFINITY && bias[u].x < INFINITY) bias[u].x = fminf(fmaxf(bias[u].x * kLog2e, -kMost), kMost);
-            if (bias[u].y > -INFINITY && bias[u].y < INFINITY) bias[u].y = fminf(fmaxf(bias[u].y * kLog2e, -kMost), kMost);
-          }
-          if constexpr (k8) {
-            ks[u] = load_pair(ring_side + from + 64 + 32 * u + 8 * t);
-            vs[u] = load_pair(ring_side + from + 128 + 32 * u + 8 * t);
-            // from 2^-100: rows that were never written have scale 0
-            lift[u].x = __log2f(fmaxf(vs[u].x, 7.888609e-31f));
-            lift[u].y = __log2f(fmaxf(vs[u].y, 7.888609e-31f));
-          }
         }
-        const bool newest = info.y + 15 >= 0;
-        uint32_t see[kMT];  // bit 4 u + e of s[u][e]
-#pragma unroll
-        for (int m = 0; m < kMT; ++m) see[m] = 0xffu;
-        bool all = info.x == 0xffff && !newest;
+        // ---- scale, bias, mask, weights ----
+        float bias[2] = {0.f, 0.f}, ks[2], vs[2];
+        bool all = info.x == 0xffff && info.y + 15 < 0;
         if (p.c.bias) {
-          bool hidden = bias[0].x == -INFINITY || bias[0].y == -INFINITY || bias[1].x == -INFINITY || bias[1].y == -INFINITY;
-          all = all && !__any_sync(0xffffffffu, hidden);
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            bias[u] = load_one(ring_side + from + 32 * u + 4 * g);
+            if (bias[u] > -INFINITY && bias[u] < INFINITY) bias[u] = fminf(fmaxf(bias[u] * kLog2e, -kMost), kMost);
+          }
+          all = all && !__any_sync(0xffffffffu, bias[0] == -INFINITY || bias[1] == -INFINITY);
         }
-        if (!all) {
-          if (!k8 && newest && guard) {
+        if constexpr (k8) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            ks[u] = load_one(ring_side + from + 64 + 32 * u + 4 * g);
+            vs[u] = load_one(ring_side + from + 128 + 32 * u + 4 * g);
+            vs[u] = vs[u] < 7.888609e-31f ? 7.888609e-31f : vs[u];  // 2^-100: rows that were never written have scale 0
+          }
+        }
+        uint32_t pr[kNT][2];
+        // `hidden`: some row does not see some key; see[m], bit e, says which
+        uint32_t see[kNT], broken = 0;
+        auto weights = [&](auto hidden) {
+          constexpr bool kHidden = decltype(hidden)::value;
+#pragma unroll
+          for (int m = 0; m < kNT; ++m) {
+            auto seen = [&](int e) { return !kHidden || ((see[m] >> e) & 1); };
+            // weights from the scores and the running max; true when one is too large
+            float w4[4], raw[4];
+            auto weigh = [&]() {
+              bool over = false;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                float y = exp2_approx(s[m][e] - mx[m][e & 1]);
+                if (kHidden) y = seen(e) ? y : 0.f;
+                raw[e] = y;
+                if constexpr (k8) {
+                  y *= vs[e >> 1];
+                  if (kHidden) y = seen(e) ? y : 0.f;  // a hidden key's scale may be NaN
+                }
+                w4[e] = y;
+                over = over || y > 256.f;
+              }
+              return over;
+            };
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              float x = s[m][e] * unit[m][e & 1];
+              if constexpr (k8) x = fmaf(x, ks[e >> 1], bias[e >> 1]);
+              else x += bias[e >> 1];
+              if (kHidden && ((broken >> (g + 8 * (e >> 1))) & 1)) x = __uint_as_float(0x7fc00000u);
+              s[m][e] = x;
+            }
+            if (__any_sync(0xffffffffu, weigh())) {
+              // move the max of the rows to the largest score (with its V scale) so far, rescale
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                float top = mx[m][h];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                  float x = s[m][2 * u + h];
+                  if constexpr (k8) x += log2f(fminf(vs[u], kMost));
+                  if (seen(2 * u + h)) top = fmaxf(top, x);
+                }
+#pragma unroll
+                for (int off = 4; off < 32; off *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+                const float f = top == mx[m][h] ? 1.f : exp2f(mx[m][h] - top);
+                mx[m][h] = top;
+                l[m][h] *= f;
+#pragma unroll
+                for (int j = 0; j < X::kTiles; ++j) {
+                  o[m][j][h] *= f;
+                  o[m][j][2 + h] *= f;
+                }
+              }
+              weigh();
+            }
+            l[m][0] += raw[0] + raw[2];
+            l[m][1] += raw[1] + raw[3];
+            pr[m][0] = transpose(pack<k8>(w4[0], w4[1]));
+            pr[m][1] = transpose(pack<k8>(w4[2], w4[3]));
+          }
+        };
+        if (all) {
+          weights(std::false_type{});
+        } else {
+          if (!k8 && info.y + 15 >= 0 && guard) {
             // newest values that are not finite become zeros -- a row that does
             // not see them must not get 0 * inf --, and the rows that do, NaN
 #pragma unroll 1
             for (int u = 0; u < 4; ++u) {
-              if (info.y + 2 * t + (u & 1) + 8 * (u >> 1) < 0) continue;
+              const int key = 2 * t + (u & 1) + 8 * (u >> 1);
+              if (info.y + key < 0) continue;
               for (int c = 0; c < X::kVC; ++c) {
                 const uint32_t a = ring_v + from + (u * X::kVC + c) * 32 * X::kVB;
                 uint32_t x[4];
                 load_words<4>(a, x);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                  if ((x[e] & 0x7f80u) == 0x7f80u) x[e] &= 0xffff0000u, broken |= 1u << u;
-                  if ((x[e] & 0x7f800000u) == 0x7f800000u) x[e] &= 0x0000ffffu, broken |= 1u << u;
+                  if ((x[e] & 0x7f80u) == 0x7f80u) x[e] &= 0xffff0000u, broken |= 1u << key;
+                  if ((x[e] & 0x7f800000u) == 0x7f800000u) x[e] &= 0x0000ffffu, broken |= 1u << key;
                 }
                 asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(a), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3])
                              : "memory");
               }
             }
-#pragma unroll
-            for (int off = 4; off < 32; off *= 2) broken |= __shfl_xor_sync(0xffffffffu, broken, off);
+            broken = __reduce_or_sync(0xffffffffu, broken);
           }
 #pragma unroll
-          for (int u = 0; u < 2; ++u)
+          for (int m = 0; m < kNT; ++m) see[m] = 0;
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int key = 2 * t + e + 8 * u, i = info.y + key;
-              const float b = e ? bias[u].y : bias[u].x;
-              const bool exists = ((info.x >> key) & 1) && b != -INFINITY && i < w.s.cnt;
+          for (int u = 0; u < 2; ++u) {
+            const int key = g + 8 * u, i = info.y + key;
+            if (((info.x >> key) & 1) && bias[u] != -INFINITY && i < w.s.cnt) {
 #pragma unroll
-              for (int m = 0; m < kMT; ++m)
+              for (int m = 0; m < kNT; ++m)
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
-                  if (!(exists && (i < 0 || (tok[m][h] < p.q.T && tree_sees(p, w.b, tok[m][h], i)))))
-                    see[m] &= ~(1u << (4 * u + 2 * h + e));
-            }
-        }
-#pragma unroll
-        for (int m = 0; m < kMT; ++m) {
-          bool over = false;
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              float x = s[m][u][e] * unit[m][e >> 1];
-              const float b = e & 1 ? bias[u].y : bias[u].x;
-              if constexpr (k8) x = fmaf(x, e & 1 ? ks[u].y : ks[u].x, b);
-              else x += b;
-              if (!all && ((broken >> (2 * u + (e & 1))) & 1)) x = __uint_as_float(0x7fc00000u);
-              s[m][u][e] = x;
-              over = over || (x + (e & 1 ? lift[u].y : lift[u].x) > mx[m][e >> 1] + 8.f && ((see[m] >> (4 * u + e)) & 1));
-            }
-          if (__any_sync(0xffffffffu, over)) {
-            // move the max of the rows to the largest score so far, rescale
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              float top = mx[m][h];
-#pragma unroll
-              for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int e = 0; e < 2; ++e)
-                  if ((see[m] >> (4 * u + 2 * h + e)) & 1) top = fmaxf(top, s[m][u][2 * h + e] + (e ? lift[u].y : lift[u].x));
-              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-              const float f = top == mx[m][h] ? 1.f : exp2f(mx[m][h] - top);
-              mx[m][h] = top;
-              l[m][h] *= f;
-#pragma unroll
-              for (int j = 0; j < X::kTiles; ++j) {
-                o[m][j][2 * h] *= f;
-                o[m][j][2 * h + 1] *= f;
-              }
+                  if (i < 0 || (tok[m][h] < p.q.T && tree_sees(p, w.b, tok[m][h], i))) see[m] |= 1u << (2 * u + h);
             }
           }
-        }
-        // ---- weights ----
-        uint32_t pr[kMT][4];
-#pragma unroll
-        for (int m = 0; m < kMT; ++m) {
-          float e[2][4];
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              float y = exp2_approx(s[m][u][x] - mx[m][x >> 1]);
-              const bool seen = all || ((see[m] >> (4 * u + x)) & 1);
-              y = seen ? y : 0.f;
-              l[m][x >> 1] += y;
-              if constexpr (k8) y = seen ? y * (x & 1 ? vs[u].y : vs[u].x) : 0.f;  // a hidden key's scale may be NaN
-              e[u][x] = y;
-            }
-          pr[m][0] = pack<k8>(e[0][0], e[0][1]);
-          pr[m][1] = pack<k8>(e[0][2], e[0][3]);
-          pr[m][2] = pack<k8>(e[1][0], e[1][1]);
-          pr[m][3] = pack<k8>(e[1][2], e[1][3]);
+          __syncwarp();
+          weights(std::true_type{});
         }
         // ---- values ----
 #pragma unroll
@@ -526,19 +574,17 @@ __global__ void __launch_bounds__(Shape<kMode, kD, kMT>::kThreads, 1) tree_mma_k
           for (int x = 0; x < X::kVB / 4; ++x) {
             if constexpr (k8) {
 #pragma unroll
-              for (int y = 0; y < 4; ++y) {
-                const uint32_t b0 = join_codes<kMode>(vw[0][x], vw[1][x], y), b1 = join_codes<kMode>(vw[2][x], vw[3][x], y);
+              for (int y = 0; y < 4; y += 2) {
+                const uint32_t a[4] = {join_codes<kMode>(vw[0][x], vw[1][x], y), join_codes<kMode>(vw[0][x], vw[1][x], y + 1),
+                                       join_codes<kMode>(vw[2][x], vw[3][x], y), join_codes<kMode>(vw[2][x], vw[3][x], y + 1)};
 #pragma unroll
-                for (int m = 0; m < kMT; ++m) mma<true>(o[m][4 * x + y], pr[m], b0, b1);
+                for (int m = 0; m < kNT; ++m) mma<true>(o[m][2 * x + y / 2], a, pr[m][0], pr[m][1]);
               }
             } else {
+              const uint32_t a[4] = {__byte_perm(vw[0][x], vw[1][x], 0x5410), __byte_perm(vw[0][x], vw[1][x], 0x7632),
+                                     __byte_perm(vw[2][x], vw[3][x], 0x5410), __byte_perm(vw[2][x], vw[3][x], 0x7632)};
 #pragma unroll
-              for (int y = 0; y < 2; ++y) {
-                const uint32_t b0 = __byte_perm(vw[0][x], vw[1][x], y ? 0x7632 : 0x5410);
-                const uint32_t b1 = __byte_perm(vw[2][x], vw[3][x], y ? 0x7632 : 0x5410);
-#pragma unroll
-                for (int m = 0; m < kMT; ++m) mma<false>(o[m][8 * c + 2 * x + y], pr[m], b0, b1);
-              }
+              for (int m = 0; m < kNT; ++m) mma<false>(o[m][4 * c + x], a, pr[m][0], pr[m][1]);
             }
           }
         }
@@ -546,92 +592,98 @@ __global__ void __launch_bounds__(Shape<kMode, kD, kMT>::kThreads, 1) tree_mma_k
 
       // ---- the piece is done: warps together, two rows at a time ----
 #pragma unroll
-      for (int m = 0; m < kMT; ++m)
+      for (int m = 0; m < kNT; ++m)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          l[m][h] += __shfl_xor_sync(0xffffffffu, l[m][h], 1);
-          l[m][h] += __shfl_xor_sync(0xffffffffu, l[m][h], 2);
-          if (t == 0) {
-            sm.m[warp][16 * m + 8 * h + g] = mx[m][h];
-            sm.l[warp][16 * m + 8 * h + g] = l[m][h];
+#pragma unroll
+          for (int off = 4; off < 32; off *= 2) l[m][h] += __shfl_xor_sync(0xffffffffu, l[m][h], off);
+          if (g == 0) {
+            sm.m[warp][8 * m + 2 * t + h] = mx[m][h];
+            sm.l[warp][8 * m + 2 * t + h] = l[m][h];
           }
         }
       __syncthreads();
       const int64_t rows_left = p.q.T * p.group - (int64_t)rt * kRows;
       const int rows = rows_left < kRows ? (int)rows_left : kRows;
+#pragma unroll
+      for (int m = 0; m < kNT; ++m)
 #pragma unroll 1
-      for (int r0 = 0; r0 < rows; r0 += 2) {
-        // this lane's row, when it is one of the two
-        const int m_of = r0 >> 4, h_of = (r0 >> 3) & 1;
-        if ((g & ~1) == (r0 & 7)) {
-          const int r = (r0 & ~7) + g;
-          float top = -INFINITY;
-          for (int x = 0; x < NW; ++x) top = fmaxf(top, sm.m[x][r]);
-          const float own = sm.m[warp][r];
-          // a warp that saw no key of the row has nothing to add
-          const float f = sm.l[warp][r] == 0.f ? 0.f : own == top ? 1.f : exp2f(own - top);
-          float* dst = sm.sum + (warp * 2 + (g & 1)) * kD;
+        for (int r0 = 8 * m; r0 < min(rows, 8 * m + 8); r0 += 2) {
+          if (2 * t == (r0 & 7)) {  // this lane has the two rows
+            float f[2];
 #pragma unroll
-          for (int m = 0; m < kMT; ++m)
+            for (int h = 0; h < 2; ++h) {
+              float top = -INFINITY;
+              for (int x = 0; x < NW; ++x) top = fmaxf(top, sm.m[x][r0 + h]);
+              const float own = sm.m[warp][r0 + h];
+              // a warp that saw no key of the row has nothing to add
+              f[h] = sm.l[warp][r0 + h] == 0.f ? 0.f : own == top ? 1.f : exp2f(own - top);
+            }
+            float* dst = sm.sum + warp * 2 * kD;
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-              if (m == m_of && h == h_of) {
+            for (int j = 0; j < X::kTiles; ++j)
 #pragma unroll
-                for (int j = 0; j < X::kTiles; ++j) {
-                  const int d0 = k8 ? X::kVB * 2 * t + j : (j >> 3) * 64 + 16 * t + (j & 7);
-                  const int d1 = d0 + (k8 ? X::kVB : 8);
-                  dst[d0] = f == 0.f ? 0.f : f * o[m][j][2 * h];
-                  dst[d1] = f == 0.f ? 0.f : f * o[m][j][2 * h + 1];
-                }
+              for (int e = 0; e < 4; ++e) {
+                const int col = (k8 ? X::kVB * g + 2 * j : (j >> 2) * 64 + 8 * g + 2 * (j & 3)) + (e >> 1);
+                dst[(e & 1) * kD + col] = f[e & 1] == 0.f ? 0.f : f[e & 1] * o[m][j][e];
               }
-        }
-        __syncthreads();
-        for (int i = threadIdx.x; i < 2 * kD; i += X::kThreads) {
-          const int r = r0 + i / kD, col = i % kD;
-          float top = -INFINITY, sum = 0.f, acc = 0.f;
-          for (int x = 0; x < NW; ++x) top = fmaxf(top, sm.m[x][r]);
-          for (int x = 0; x < NW; ++x) {
-            const float lx = sm.l[x][r];
-            if (lx != 0.f) sum = fmaf(sm.m[x][r] == top ? 1.f : exp2f(sm.m[x][r] - top), lx, sum);
-            acc += sm.sum[x * 2 * kD + i];
           }
-          // -kMost: nothing but biases of the type's lowest value
-          const float m = top == -kMost ? -kMost : top * kLn2;
-          const TreeRow row = tree_row(p, w.hk, rt, r);
-          if (r >= rows) continue;
-          if (row.t >= w.s.cnt) sum = 0.f;  // a row that does not exist
-          if (w.part >= 0) {
-            const int64_t part = p.part_row(span, rt, w.part, r);
-            if (col < d) p.part_o[part * kTreePartCols + col] = acc;
-            if (col == 0) *reinterpret_cast<float2*>(p.part_ml + part * 2) = make_float2(m, sum);
-          } else {
-            if (col < d) tree_out_row<__nv_bfloat16>(p, w.b, row)[col] = __float2bfloat16_rn(sum != 0.f ? acc / sum : 0.f);
-            if (col == 0 && p.q.lse)
-              p.q.lse[((int64_t)w.b * p.q.n_q_heads + row.h) * p.q.T + row.t] = sum != 0.f ? m + logf(sum) : -INFINITY;
+          __syncthreads();
+          for (int i = threadIdx.x; i < 2 * kD; i += X::kThreads) {
+            const int r = r0 + i / kD, col = i % kD;
+            float top = -INFINITY, sum = 0.f, acc = 0.f;
+#pragma unroll
+            for (int x = 0; x < NW; ++x) top = fmaxf(top, sm.m[x][r]);
+#pragma unroll
+            for (int x = 0; x < NW; ++x) {
+              const float lx = sm.l[x][r];
+              if (lx != 0.f) sum = fmaf(sm.m[x][r] == top ? 1.f : exp2f(sm.m[x][r] - top), lx, sum);
+              acc += sm.sum[x * 2 * kD + i];
+            }
+            // -kMost: nothing but biases of the type's lowest value
+            const float ln = top == -kMost ? -kMost : top * kLn2;
+            const TreeRow row = tree_row(p, w.hk, rt, r);
+            if (r >= rows) continue;
+            if (row.t >= w.s.cnt) sum = 0.f;  // a row that does not exist
+            if (w.part >= 0) {
+              const int64_t part = p.part_row(span, rt, w.part, r);
+              if (col < d) p.part_o[part * kTreePartCols + col] = acc;
+              if (col == 0) *reinterpret_cast<float2*>(p.part_ml + part * 2) = make_float2(ln, sum);
+            } else {
+              if (col < d) tree_out_row<__nv_bfloat16>(p, w.b, row)[col] = __float2bfloat16_rn(sum != 0.f ? acc / sum : 0.f);
+              if (col == 0 && p.q.lse)
+                p.q.lse[((int64_t)w.b * p.q.n_q_heads + row.h) * p.q.T + row.t] = sum != 0.f ? ln + logf(sum) : -INFINITY;
+            }
           }
+          __syncthreads();
         }
-        __syncthreads();
-      }
       base += w.k1 - w.k0;
     }
   }
   asm volatile("cp.async.wait_all;\n" ::: "memory");
 }
 
-template <int kMode, int kD, int kMT>
+template <int kMode, int kD, int kNT>
 static int launch(const TreeParams& p, cudaStream_t st) {
-  using X = Shape<kMode, kD, kMT>;
-  constexpr size_t smem = sizeof(Smem<X, kMT>);
+  using X = Shape<kMode, kD, kNT>;
+  constexpr size_t smem = sizeof(Smem<X, kNT>);
   static_assert(smem <= kSmemLimit, "shared memory");
-  auto kernel = tree_mma_kernel<kMode, kD, kMT>;
+  auto kernel = tree_mma_kernel<kMode, kD, kNT>;
   DCC_CHECK(check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "tree_mma smem"));
   kernel<<<p.n_groups * p.n_spans, X::kThreads, smem, st>>>(p);
   return check_launch("tree_attention");
 }
+template <int kMode, int kD>
+static int launch_n(const TreeParams& p, cudaStream_t st) {
+  switch (p.n_rows) {
+    case 8: return launch<kMode, kD, 1>(p, st);
+    case 16: return launch<kMode, kD, 2>(p, st);
+    default: return launch<kMode, kD, 4>(p, st);
+  }
+}
 template <int kMode>
 static int launch_d(const TreeParams& p, cudaStream_t st) {
-  if (p.c.head_dim <= 64) return p.n_rows == 16 ? launch<kMode, 64, 1>(p, st) : launch<kMode, 64, 2>(p, st);
-  return p.n_rows == 16 ? launch<kMode, 128, 1>(p, st) : launch<kMode, 128, 2>(p, st);
+  return p.c.head_dim <= 64 ? launch_n<kMode, 64>(p, st) : launch_n<kMode, 128>(p, st);
 }
 
 }  // namespace tm
