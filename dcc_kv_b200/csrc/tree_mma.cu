@@ -3,10 +3,10 @@
 //
 // With few rows every key is used for so little arithmetic that HBM is the
 // bound, and what a kernel has to save is instructions per key.  Here every
-// warp works alone on 16 keys at a time, and a lane copies (cp.async) exactly
-// the bytes that it will feed to its own MMA operands, so the shared memory
-// ring is private to the lane: no barriers, no swizzle, no second trip through
-// shared memory for widened codes.  The contractions are register MMAs
+// warp works alone on 16 keys at a time: it copies them (cp.async, 512 bytes in
+// a row) into a ring of its own and widens codes in registers, on their way to
+// the MMA -- no barriers between warps, no second trip through shared memory
+// for widened codes.  The contractions are register MMAs
 // (m16n8k16) with keys, then head columns, as the 16 rows and query rows as the
 // 8 columns -- four query heads and one token fill half of a tile:
 //   S^T [16 keys, 8 rows]  += K Q^T    the k index runs over d in the order in
@@ -40,7 +40,7 @@ struct Shape {
   static constexpr bool k8 = kMode != DCC_KV_BF16;
   // as many warps as the registers of a warp and the ring (64 KB and more in
   // flight) allow
-  static constexpr int kWarps = k8 ? (kNT == 1 ? 16 : kNT == 2 ? 12 : 8) : (kNT == 1 ? 12 : 8);
+  static constexpr int kWarps = k8 ? (kNT <= 2 ? 12 : 8) : (kNT == 1 ? 12 : 8);
   static constexpr int kThreads = 32 * kWarps;
   static constexpr int kE = k8 ? 16 : 8;             // elements of a 16-byte chunk
   static constexpr int kKC = kD / (4 * kE);          // K chunks of a lane and key
@@ -48,7 +48,8 @@ struct Shape {
   static constexpr int kVB = k8 ? kD / 8 : 16;       // bytes of one
   static constexpr int kSteps = kD / 16;             // k steps of S
   static constexpr int kTiles = kD / 16;             // 16-column tiles of O
-  static constexpr int kK = 32 * 2 * kKC * 16, kV = 32 * 4 * kVC * kVB, kSide = 3 * 64;
+  static constexpr int kRowBytes = kD * (k8 ? 1 : 2), kPerRow = kRowBytes / 16;  // 16-byte chunks of a row
+  static constexpr int kK = 16 * kRowBytes, kV = kK, kSide = 3 * 64;
   static constexpr int kStage = kK + kV + kSide;     // 16 keys of a warp
   // operands of the queries: in registers, or, where O takes those, in shared memory
   static constexpr bool kQShared = k8 ? kNT > 1 : kNT == 4;
@@ -71,12 +72,11 @@ struct Smem {
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
-template <int kBytes>
-__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, uint32_t size) {  // size < kBytes: zeros follow
-  if constexpr (kBytes == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(size) : "memory");
-  else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;\n" ::"r"(dst), "l"(src), "r"(size) : "memory");
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, uint32_t size) {  // size < 16: zeros follow
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(size) : "memory");
+}
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src) : "memory");
 }
 template <int kWords>
 __device__ __forceinline__ void load_words(uint32_t a, uint32_t* w) {
@@ -207,33 +207,39 @@ __global__ void __launch_bounds__(Shape<kMode, kD, kNT>::kThreads, 1) tree_mma_k
   const int chunks = 8 * n;
   const int d = p.c.head_dim;
   const uint32_t row_bytes = (uint32_t)d * (k8 ? 1 : 2);
-  const uint32_t ring = smem_addr(sm.ring[warp][0]) + (uint32_t)lane * 16;
-  const uint32_t ring_v = smem_addr(sm.ring[warp][0]) + X::kK + (uint32_t)lane * X::kVB;
-  const uint32_t ring_side = smem_addr(sm.ring[warp][0]) + X::kK + X::kV;
+  // K: row r, chunk c of 16 bytes at (r, c ^ 4 (r & 1)): the lanes of two rows and
+  // four chunks that read together meet eight banks; here of row g, chunks t
+  // (even steps) and 4 + t (odd ones)
+  const uint32_t ring = smem_addr(sm.ring[warp][0]);
+  constexpr bool kSwap = X::kPerRow > 4;
+  const uint32_t k_at[2] = {ring + (uint32_t)(g * X::kRowBytes + 16 * t + (kSwap ? 64 * (g & 1) : 0)),
+                            ring + (uint32_t)(g * X::kRowBytes + 16 * t + (kSwap ? 64 - 64 * (g & 1) : 64))};
+  // V: chunk c at c ^ (r & 7), of four-chunk rows c ^ (r / 2 & 3); here of rows 2 t
+  // and 2 t + 1, this lane group's chunk
+  uint32_t v_at[2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int r = 2 * t + u;
+    v_at[u] = ring + X::kK + (uint32_t)(r * X::kRowBytes + (X::kPerRow > 4 ? (g ^ r) * 16 : ((g >> 1) ^ (r >> 1)) * 16 + (g & 1) * 8));
+  }
+  const uint32_t ring_side = ring + X::kK + X::kV;
   const float scale = p.scale * kLog2e;
   const bool guard = p.q.T > 1 || p.q.tree != nullptr;  // rows may hide newest tokens from one another
 
-  // ---- copies of this warp's chunks, kStages - 1 ahead ----
+  // ---- copies of this warp's chunks, kStages ahead: K and V apart, each into
+  // the place that its predecessor has just left ----
   const bool pow2 = (p.c.page_size & (p.c.page_size - 1)) == 0;
   const int shift = 31 - __clz(p.c.page_size);
   const bool one_page = p.c.page_size % 16 == 0;  // a chunk never leaves its page
   const int page_step = p.c.n_kv_heads * p.c.page_size;
-  // what this lane copies of a row: chunks of K (key g of eight) and V (keys 2 t
-  // and 2 t + 1 of eight); nothing past head_dim
-  uint32_t k_off[X::kKC], k_size[X::kKC], v_off[X::kVC], v_size[X::kVC];
-#pragma unroll
-  for (int c = 0; c < X::kKC; ++c) {
-    const bool real = (4 * c + t) * X::kE < d;
-    k_off[c] = (uint32_t)g * row_bytes + (real ? 64u * c + 16u * t : 0u);
-    k_size[c] = real ? 16 : 0;
-  }
-#pragma unroll
-  for (int c = 0; c < X::kVC; ++c) {
-    const bool real = X::kVB * g + 128 * c < (int)row_bytes;
-    v_off[c] = (uint32_t)(2 * t) * row_bytes + (real ? (uint32_t)(X::kVB * g + 128 * c) : 0u);
-    v_size[c] = real ? X::kVB : 0;
-  }
-  // and of the 16 keys' bias, K and V scales: four of one of them
+  // this lane copies the 16-byte pieces lane, lane + 32, ... of the 16 rows
+  constexpr int kCopies = 16 * X::kPerRow / 32;
+  auto place = [&](int i, bool v) {
+    const int r = (32 * i + lane) / X::kPerRow, c = (32 * i + lane) % X::kPerRow;
+    const int to = X::kPerRow > 4 ? c ^ (v ? r & 7 : 4 * (r & 1)) : v ? c ^ (r / 2 & 3) : c;
+    return ring + (uint32_t)((v ? X::kK : 0) + r * X::kRowBytes + 16 * to);
+  };
+  // and of the bias, K and V scales four keys of one of them
   const int side_kind = lane >> 2, side_key = 4 * t;
   const float* side_src = side_kind == 0 ? p.c.bias : side_kind == 1 ? p.c.k_scale : side_kind == 2 ? p.c.v_scale : nullptr;
   const unsigned char* const k_src = static_cast<const unsigned char*>(p.c.k);
@@ -261,60 +267,60 @@ __global__ void __launch_bounds__(Shape<kMode, kD, kNT>::kThreads, 1) tree_mma_k
       page_b = __ldg(table + q);
     }
   };
-  auto issue = [&]() {
-    if (todo > 0) {
-      const uint32_t to = (uint32_t)put * X::kStage;
+  // of the chunk being copied: its rows (the first of either eight) and how many exist
+  bool live = false, whole = false;
+  int rows[2] = {0, 0}, exist[2] = {0, 0};
+  auto copy_rows = [&](uint32_t stage, const unsigned char* src, bool v) {
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i) {
+      const int r = (32 * i + lane) / X::kPerRow, c = (32 * i + lane) % X::kPerRow;
+      const bool real = (r & 7) < (r < 8 ? exist[0] : exist[1]) && c * X::kE < d;
+      copy_async(place(i, v) + stage,
+                 src + (real ? (int64_t)((r < 8 ? rows[0] : rows[1]) + (r & 7)) * row_bytes + 16 * c : 0), real ? 16 : 0);
+    }
+  };
+  auto issue_k = [&]() {
+    live = todo > 0;
+    if (live) {
       const bool in_a = page_a >= 0 && page_a < p.c.n_pages;
-      if (one_page && in_a && left >= 16) {
-        const int row = page_a * page_step + add_a;
-        const int64_t off = (int64_t)row * row_bytes;
-        const unsigned char* k = k_src + off;
-        const unsigned char* v = v_src + off;
+      whole = one_page && in_a && left >= 16 && d == kD;
+      const uint32_t stage = (uint32_t)put * X::kStage;
+      if (whole) {
+        rows[0] = page_a * page_step + add_a;
+        const unsigned char* k = k_src + (int64_t)rows[0] * X::kRowBytes + 16 * lane;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-#pragma unroll
-          for (int c = 0; c < X::kKC; ++c)
-            copy_async<16>(ring + to + (u * X::kKC + c) * 512, k + (k_off[c] + 8 * u * row_bytes), k_size[c]);
-        }
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-#pragma unroll
-          for (int c = 0; c < X::kVC; ++c)
-            copy_async<X::kVB>(ring_v + to + (u * X::kVC + c) * 32 * X::kVB, v + (v_off[c] + (8 * (u >> 1) + (u & 1)) * row_bytes),
-                               v_size[c]);
-        }
-        if (side_src) copy_async<16>(ring_side + to + side_kind * 64 + t * 16, side_src + row + side_key, 16);
-        // rel >= -15: newest tokens among them
-        if (lane == 0) sm.info[warp][put] = make_int2(0xffff, rel);
+        for (int i = 0; i < kCopies; ++i) copy_async(place(i, false) + stage, k + 512 * i);
+        if (side_src)
+          copy_async(ring_side + stage + side_kind * 64 + t * 16, side_src + rows[0] + side_key);
+        if (lane == 0) sm.info[warp][put] = make_int2(0xffff, rel);  // rel >= -15: newest tokens among them
       } else {
         // the rows that exist; the others become zeros
         const int pb = one_page ? page_a : page_b, ab = one_page ? add_a + 8 : add_b;
         const bool in_b = pb >= 0 && pb < p.c.n_pages;
-        const int n_a = in_a ? min(max(left, 0), 8) : 0, n_b = in_b ? min(max(left - 8, 0), 8) : 0;
-        const int rows[2] = {n_a ? page_a * page_step + add_a : 0, n_b ? pb * page_step + ab : 0};
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const bool key = g < (u ? n_b : n_a);
-          const unsigned char* k = k_src + (int64_t)rows[u] * row_bytes;
-#pragma unroll
-          for (int c = 0; c < X::kKC; ++c)
-            copy_async<16>(ring + to + (u * X::kKC + c) * 512, k + (key ? k_off[c] : 0u), key ? k_size[c] : 0);
-        }
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const bool key = 2 * t + (u & 1) < (u >> 1 ? n_b : n_a);
-          const unsigned char* v = v_src + (int64_t)rows[u >> 1] * row_bytes;
-#pragma unroll
-          for (int c = 0; c < X::kVC; ++c)
-            copy_async<X::kVB>(ring_v + to + (u * X::kVC + c) * 32 * X::kVB, v + (key ? v_off[c] + (u & 1) * row_bytes : 0u),
-                               key ? v_size[c] : 0);
-        }
+        exist[0] = in_a ? min(max(left, 0), 8) : 0;
+        exist[1] = in_b ? min(max(left - 8, 0), 8) : 0;
+        rows[0] = exist[0] ? page_a * page_step + add_a : 0;
+        rows[1] = exist[1] ? pb * page_step + ab : 0;
+        copy_rows(stage, k_src, false);
         if (side_src) {
-          const bool key = (side_key & 7) < (side_key < 8 ? n_a : n_b);
-          copy_async<16>(ring_side + to + side_kind * 64 + t * 16,
-                         side_src + (key ? rows[side_key >> 3] + (side_key & 7) : 0), key ? 16 : 0);
+          const bool key = (side_key & 7) < (side_key < 8 ? exist[0] : exist[1]);
+          copy_async(ring_side + stage + side_kind * 64 + t * 16,
+                     side_src + (key ? (side_key < 8 ? rows[0] : rows[1]) + (side_key & 7) : 0), key ? 16 : 0);
         }
-        if (lane == 0) sm.info[warp][put] = make_int2((0xff >> (8 - n_a)) | (0xff >> (8 - n_b)) << 8, rel);
+        if (lane == 0) sm.info[warp][put] = make_int2((0xff >> (8 - exist[0])) | (0xff >> (8 - exist[1])) << 8, rel);
+      }
+    }
+    asm volatile("cp.async.commit_group;\n" ::: "memory");
+  };
+  auto issue_v = [&]() {
+    if (live) {
+      const uint32_t stage = (uint32_t)put * X::kStage;
+      if (whole) {
+        const unsigned char* v = v_src + (int64_t)rows[0] * X::kRowBytes + 16 * lane;
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) copy_async(place(i, true) + stage, v + 512 * i);
+      } else {
+        copy_rows(stage, v_src, true);
       }
       if (--todo > 0) {
         at.move(p, pl, 16 * NW);
@@ -326,7 +332,10 @@ __global__ void __launch_bounds__(Shape<kMode, kD, kNT>::kThreads, 1) tree_mma_k
   };
   if (todo > 0) look_up();
 #pragma unroll 1
-  for (int i = 0; i < S - 1; ++i) issue();
+  for (int i = 0; i < S; ++i) {
+    issue_k();
+    issue_v();
+  }
 
   // ---- pieces ----
   int base = 0, get = 0, mine = warp;  // tiles before the piece, stage, chunk
@@ -405,9 +414,8 @@ __global__ void __launch_bounds__(Shape<kMode, kD, kNT>::kThreads, 1) tree_mma_k
       }
 #pragma unroll 1
       for (; mine < stop; mine += NW) {
-        asm volatile("cp.async.wait_group %0;\n" ::"n"(S - 2) : "memory");
-        __syncwarp();  // the scales and info of the chunk; and the last chunk's have been read
-        issue();
+        asm volatile("cp.async.wait_group %0;\n" ::"n"(2 * S - 1) : "memory");  // K and scales of this chunk
+        __syncwarp();  // other lanes' scales and info
         const uint32_t from = (uint32_t)get * X::kStage;
         const int2 info = sm.info[warp][get];
         if (++get == S) get = 0;
@@ -418,8 +426,8 @@ __global__ void __launch_bounds__(Shape<kMode, kD, kNT>::kThreads, 1) tree_mma_k
 #pragma unroll
         for (int c = 0; c < X::kKC; ++c) {
           uint32_t kw[2][4];
-          load_words<4>(ring + from + c * 512, kw[0]);
-          load_words<4>(ring + from + (X::kKC + c) * 512, kw[1]);
+          load_words<4>(k_at[c & 1] + from + 128 * (c >> 1), kw[0]);
+          load_words<4>(k_at[c & 1] + from + 128 * (c >> 1) + 8 * X::kRowBytes, kw[1]);
           constexpr int kPer = X::kE / 4;  // k steps of a chunk
 #pragma unroll
           for (int x = 0; x < kPer; ++x) {
@@ -529,12 +537,14 @@ __global__ void __launch_bounds__(Shape<kMode, kD, kNT>::kThreads, 1) tree_mma_k
           if (!k8 && info.y + 15 >= 0 && guard) {
             // newest values that are not finite become zeros -- a row that does
             // not see them must not get 0 * inf --, and the rows that do, NaN
+            asm volatile("cp.async.wait_group %0;\n" ::"n"(2 * S - 2) : "memory");  // V of this chunk
+            __syncwarp();
 #pragma unroll 1
             for (int u = 0; u < 4; ++u) {
               const int key = 2 * t + (u & 1) + 8 * (u >> 1);
               if (info.y + key < 0) continue;
               for (int c = 0; c < X::kVC; ++c) {
-                const uint32_t a = ring_v + from + (u * X::kVC + c) * 32 * X::kVB;
+                const uint32_t a = v_at[u & 1] + from + (u >> 1) * 8 * X::kRowBytes + 128 * c;
                 uint32_t x[4];
                 load_words<4>(a, x);
 #pragma unroll
@@ -564,12 +574,16 @@ __global__ void __launch_bounds__(Shape<kMode, kD, kNT>::kThreads, 1) tree_mma_k
           __syncwarp();
           weights(std::true_type{});
         }
+        __syncwarp();  // the scales and info have been read
+        issue_k();
         // ---- values ----
+        asm volatile("cp.async.wait_group %0;\n" ::"n"(2 * S - 1) : "memory");
+        __syncwarp();
 #pragma unroll
         for (int c = 0; c < X::kVC; ++c) {
           uint32_t vw[4][X::kVB / 4];
 #pragma unroll
-          for (int u = 0; u < 4; ++u) load_words<X::kVB / 4>(ring_v + from + (u * X::kVC + c) * 32 * X::kVB, vw[u]);
+          for (int u = 0; u < 4; ++u) load_words<X::kVB / 4>(v_at[u & 1] + from + (u >> 1) * 8 * X::kRowBytes + 128 * c, vw[u]);
 #pragma unroll
           for (int x = 0; x < X::kVB / 4; ++x) {
             if constexpr (k8) {
@@ -588,6 +602,8 @@ __global__ void __launch_bounds__(Shape<kMode, kD, kNT>::kThreads, 1) tree_mma_k
             }
           }
         }
+        __syncwarp();
+        issue_v();
       }
 
       // ---- the piece is done: warps together, two rows at a time ----
