@@ -251,7 +251,7 @@ static Path tree_params(const dcc_kv_pages& c, const dcc_tree_query& q, int dtyp
   p.group = q.n_q_heads / c.n_kv_heads;
   const int64_t rows = q.T * p.group;
   const Path path = !tree_tensor_supported(c, q, dtype) ? Path::kSimt : rows <= 32 ? Path::kMma : Path::kTc05;
-  p.n_rows = path == Path::kSimt ? kSimtRows : rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+  p.n_rows = path == Path::kSimt ? kSimtRows : rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 128 ? 128 : 256;
   p.n_row_tiles = (int)((rows + p.n_rows - 1) / p.n_rows);
   const int ctas = num_sms() * (path == Path::kSimt ? kSimtCtasPerSm : 1);
   const int rounds = (p.n_row_tiles + ctas - 1) / ctas;

@@ -1,43 +1,40 @@
-// Tree attention over the paged cache on the 5th-gen tensor cores (tcgen05 +
-// TMEM): bf16 queries, bf16 / int8 / e4m3 cache, head_dim a multiple of 16.
+// Tree attention over the paged cache for more than 32 query rows per KV head,
+// on the 5th-gen tensor cores (tcgen05 + TMEM): bf16 queries, bf16 / int8 / e4m3
+// cache, head_dim a multiple of 16.
 //
-// The contractions are transposed, so that the 128 rows of an MMA are keys (or
-// head columns) and the few query rows are its N:
-//   S^T [128 keys, N rows]  = K [128, d]      Q^T        (both K-major)
-//   O^T [d, N rows]        += V^T [d, 128]    P^T        (both MN-major)
-// One token of 4 query heads costs an N = 16 MMA instead of 128 padded rows.
-// A CTA walks over its span of key tiles (tree_attention.cuh), one warp or
-// group of warps per role:
-//   softmax      2 or 4 warpgroups (streams); tile j belongs to stream j mod
-//                kStreams, which has its own S, P, O, running max and sums, so
-//                the chain scores -> softmax -> values of one tile (about 2500
-//                cycles, most of it waiting) runs beside those of the next;
-//                the streams are added up at the end of a piece.  Thread = key
-//                (TMEM lane), then head column
-//   1 warp       S issuer and TMEM owner
-//   1 warp       O issuer; for bf16 it clears value rows that do not exist
-//   1 warp       queries of the next piece into shared memory
-//   1 warp       page lookups and copies: the ring of K and V tiles stays full.
+//   S [128 rows, 128 keys] = Q K^T    (SS MMA, both K-major)
+//   O [128 rows, d]       += P V      (TS MMA: P over S in TMEM; V MN-major)
+// A CTA walks over its span of key tiles (tree_attention.cuh) with two streams,
+// each with its own S / P, O, running max and sums, so that the softmax of one
+// runs beside the MMAs of the other:
+//   up to 128 rows  one tile of queries; stream = key tile mod 2, added up at the
+//                   end of a piece
+//   more            two tiles of queries (256 rows), one a stream; every key tile
+//                   is loaded (and widened) once for both
+// Roles, one warp or group of warps each:
+//   8 warps      softmax, thread = query row (TMEM lane); they bring in the
+//                queries of a piece and write its results
+//   1 warp       TMEM owner and MMA issuer; clears bf16 value rows that do not exist
+//   1 warp       page lookups and copies: the rings of K and V tiles stay full.
 //                bf16 tiles come as TMA boxes of up to 128 rows of a page
 //                straight into the layout of the MMA, 8-bit codes and scales as
 //                bulk copies of rows that are neighbours in the page
-//   8 warps      (8-bit) widen codes to fp16, exactly, one group K, the
-//                other V.  A warp reads the codes of its 32 rows of the tile into
-//                registers from the place where it then writes their values;
-//                the scales are applied to S and P in fp32.  The queries are
-//                held in fp16 too, each row scaled by a power of two that takes
-//                its largest element to 2^14: bf16 digits fit, and what falls
-//                below fp16's range is under 2^-39 of that element
-// K and V tiles have rings of their own, so that every role sees every use of
-// the barriers that it waits on; copies of K run two tiles ahead of V, so that
-// a V tile does not sit in its ring while its softmax runs.
+//   8 warps      (8-bit) widen codes to fp16, exactly, one group K, the other V.
+//                A warp reads the codes of its 32 rows of the tile into registers
+//                from the place where it then writes their values.  Scales act
+//                on S and P in fp32; the queries are held in fp16 too, each row
+//                scaled by a power of two that takes its largest element to 2^14:
+//                bf16 digits fit, and what falls below fp16's range is under
+//                2^-39 of that element
+// K and V have rings of their own, so that every role sees every use of the
+// barriers that it waits on; copies of K run two tiles ahead of V.
 // The running max of a row moves (with O and the sums rescaled) only when a
 // score passes it by 2^8.  P is rounded once for its MMA, to bf16 beside bf16
 // values (a relative 2^-9 of each weight) and to fp16 beside 8-bit ones (2^-12):
 // there P carries the V scale, so the max is taken over score + log2(scale),
 // which keeps P below 2^8 whatever the scales are.
 //
-// Bound: HBM for few rows (2 d bytes a key and head against 4 N d flops).
+// Bound: tensor cores and the issue of the softmax beside them.
 //
 // Waits are bounded (2 s).  After one has run out a role sets the error word
 // and walks through the rest of its loop without waiting, so named barriers
@@ -59,69 +56,58 @@ namespace tt {
 constexpr int kRing = 8;  // scales and masks of the last K tiles
 constexpr int kFetch = 4;   // K tiles between a page lookup and its use
 constexpr int kLead = 2;    // tiles that copies of K run ahead of V
-constexpr int kPieces = 8;  // queries of a piece are written once the scores of the one before are issued, at
-                            // most kStreams tiles ahead of the softmax: 5 pieces of one tile
 constexpr size_t kSmemLimit = 232448;
 
-template <int kMode, int kD, int kN>  // cache format, padded head_dim, query rows
+template <int kMode, int kD, bool kPair>  // cache format, padded head_dim, two tiles of queries
 struct Shape {
   static constexpr bool k8 = kMode == DCC_KV_INT8 || kMode == DCC_KV_E4M3;
-  static constexpr int kStreams = kN == 16 ? 4 : 2;
-  static constexpr int kTile = 128 * kD * 2;          // K or V tile of 16-bit values
+  static constexpr int kRows = kPair ? 256 : 128;
+  static constexpr int kTile = 128 * kD * 2;          // Q, K or V tile of 16-bit values
   static constexpr int kBlocks = kD / 64;             // 64-column blocks of 128 swizzled rows
-  static constexpr int kQ = kN * kD * 2;
-  // P: 128-byte rows (keys) of 64 columns; the streams of 16 or 32 columns share them
-  static constexpr int kP = kN == 64 ? 2 * 16384 : 16384;
-  static constexpr int kPStep = kN == 64 ? 16384 : 2 * kN;  // from stream to stream
-  static constexpr int kChunk = kN < 32 ? kN : 32;    // columns held in registers at once
-  static constexpr int kChunks = kN / kChunk;
-  static constexpr int kOut = kN / kStreams;          // columns of a stream in the results
-  static constexpr uint32_t kColS = 0, kColO = kStreams * kN;
-  static constexpr int kTmem = 2 * kStreams * kN;
+  static constexpr uint32_t kColS = 0, kColO = 256;   // TMEM columns, 128 a stream
   static constexpr int kArrays = k8 ? 3 : 1;          // bias; K and V scales
-  static constexpr size_t kFixed = (size_t)kQ + kP + (size_t)kRing * kArrays * 512 + 896 + kN * 128;
+  static constexpr size_t kFixed = (size_t)kRows * kD * 2 + (size_t)kRing * kArrays * 512 + 2 * 4 * 512 + 3072 + kRows * 4;
   static constexpr int kFit = (int)((kSmemLimit - kFixed) / kTile);
   static constexpr int kSlotsV = (kFit + 1) / 2 < 4 ? (kFit + 1) / 2 : 4, kSlotsK = kFit / 2 < 4 ? kFit / 2 : 4;
   static constexpr int kSlots = kSlotsK + kSlotsV;
   static_assert(kSlotsK >= 2, "rings");
   // K tile j + kRing is copied after V tile j + kRing - kLead - 1, which waited
   // for V tile j + kRing - kLead - 1 - kSlotsV to be consumed: that has to be
-  // tile j or a later one, so that nobody reads its scales any more.  And a
-  // place of the ring of scales belongs to one stream
-  static_assert(kRing - kLead - 1 - kSlotsV >= 0 && kRing % kStreams == 0, "ring of scales");
+  // tile j or a later one, so that nobody reads its scales any more
+  static_assert(kRing - kLead - 1 - kSlotsV >= 0 && kRing % 2 == 0, "ring of scales");
   static constexpr int kWiden = k8 ? 8 : 0;
-  static constexpr int kGroups = kStreams + 1 + kWiden / 4;  // warpgroups
+  static constexpr int kGroups = 3 + kWiden / 4;      // warpgroups
   static constexpr int kThreads = kGroups * 128;
   static constexpr int kRegsLaunch = 65536 / kThreads / 8 * 8;
-  static constexpr int kRegsSoftmax = k8 ? (kN == 16 ? 80 : kN == 32 ? 128 : 152) : (kN == 16 ? 96 : 192);
-  static constexpr int kRegsWork = k8 ? 72 : (kN == 16 ? 88 : 112);  // issuers, queries, copies
-  static constexpr int kRegsWiden = kN == 16 ? 56 : kN == 32 ? 72 : 48;
-  static_assert(kStreams * kRegsSoftmax + kRegsWork + kWiden / 4 * kRegsWiden <= kGroups * kRegsLaunch, "register split");
+  static constexpr int kRegsSoftmax = k8 ? 136 : 192;
+  static constexpr int kRegsWork = k8 ? 88 : 112;     // issuer, copies
+  static constexpr int kRegsWiden = 56;
+  static_assert(2 * kRegsSoftmax + kRegsWork + kWiden / 4 * kRegsWiden <= kGroups * kRegsLaunch, "register split");
   static_assert(kRegsWork <= kRegsLaunch && kRegsWiden <= kRegsLaunch && kRegsSoftmax >= kRegsLaunch, "register split");
 };
 
-template <typename X, int kN>
+template <typename X>
 struct Smem {
   unsigned char slot[X::kSlots][X::kTile];
-  unsigned char q[X::kQ];
-  unsigned char p[X::kP];
+  unsigned char q[X::kRows / 128][X::kTile];
   __align__(16) float side[kRing][X::kArrays][128];  // bias, k_scale, v_scale
+  // of a stream's tile: bias in powers of two (-inf: hidden), K scale, V scale and its logarithm
+  __align__(16) float bias[2][128];
+  __align__(16) float ks[2][128], vs[2][128], lift[2][128];
   __align__(16) uint8_t vis[kRing][16];               // bits: keys that exist
   int32_t pages[kFetch][16];                          // of every eighth key of the next K tiles
-  __align__(16) float qf[kPieces][kN];                // what undoes the scaling of a query row, by piece
-  __align__(16) float m[X::kStreams][kN];
-  __align__(16) float sum[X::kStreams][kN];           // while a piece runs: the last rescale
+  float qf[X::kRows];                                 // what undoes the scaling of a query row
   union {
-    float red[X::kStreams][4][kN];
+    float2 ml[2][128];                                // max and sum of a row, to add the streams up
     TreePlanSmem plan;                                // only before the roles begin
   };
   TreePlan span;
-  uint64_t bar_raw[X::kSlots], bar_full[X::kSlots], bar_empty[X::kSlots], bar_side[kRing], bar_q, bar_qfree,
-      bar_s[X::kStreams], bar_p[X::kStreams], bar_o[X::kStreams], bar_end;
+  uint64_t bar_raw[X::kSlots], bar_full[X::kSlots], bar_empty[X::kSlots], bar_side[kRing], bar_q, bar_s[2], bar_p[2],
+      bar_o[2], bar_end;
   uint32_t tmem;
 };
-template <int kMode, int kD, int kN>
-using SmemOf = Smem<Shape<kMode, kD, kN>, kN>;
+template <int kMode, int kD, bool kPair>
+using SmemOf = Smem<Shape<kMode, kD, kPair>>;
 
 // Waits with a hint to sleep, so that idle roles leave the issue slots to the
 // others; gives up after 2 s.
@@ -159,34 +145,8 @@ __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
   __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&v);
 }
-template <int N>
-__device__ __forceinline__ void tmem_ld(uint32_t a, uint32_t* r) {
-  if constexpr (N == 4) tmem_ld4(a, r);
-  else if constexpr (N == 8) tmem_ld8(a, r);
-  else if constexpr (N == 16) tmem_ld16(a, r);
-  else tmem_ld32(a, r);
-}
-template <int N>
-__device__ __forceinline__ void tmem_st(uint32_t a, const uint32_t* r) {
-  if constexpr (N == 8) tmem_st8(a, r);
-  else if constexpr (N == 16) tmem_st16(a, r);
-  else tmem_st32(a, r);
-}
-template <int kStreams>
-__device__ __forceinline__ void all_streams_sync() {
-  asm volatile("bar.sync 5, %0;\n" ::"n"(128 * kStreams) : "memory");
-}
+__device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 3, 256;\n" ::: "memory"); }
 __device__ __forceinline__ void group_sync(int wg) { asm volatile("bar.sync %0, 128;\n" ::"r"(1 + wg) : "memory"); }
-// true when any thread of the warpgroup says so
-__device__ __forceinline__ bool group_any(int wg, bool x) {
-  uint32_t r;
-  asm volatile(
-      "{\n .reg .pred p, q;\n setp.ne.b32 p, %1, 0;\n bar.red.or.pred q, %2, 128, p;\n selp.u32 %0, 1, 0, q;\n}\n"
-      : "=r"(r)
-      : "r"((uint32_t)x), "r"(1 + wg)
-      : "memory");
-  return r != 0;
-}
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(dst), "l"(src) : "memory");
 }
@@ -270,10 +230,10 @@ __device__ __forceinline__ uint64_t desc_at(uint32_t saddr, uint32_t lbo) {
 }
 
 // ---- copies ----------------------------------------------------------------------------
-template <int kMode, int kD, int kN>
-__device__ __forceinline__ void copies(const TreeParams& p, const TreeMaps& maps, SmemOf<kMode, kD, kN>& sm, int n, int lane,
+template <int kMode, int kD, bool kPair>
+__device__ __forceinline__ void copies(const TreeParams& p, const TreeMaps& maps, SmemOf<kMode, kD, kPair>& sm, int n, int lane,
                                        bool& ok) {
-  using X = Shape<kMode, kD, kN>;
+  using X = Shape<kMode, kD, kPair>;
   const TreePlan& pl = sm.span;
   const uint32_t row_bytes = (uint32_t)p.c.head_dim * (X::k8 ? 1 : 2);
   const bool pow2 = (p.c.page_size & (p.c.page_size - 1)) == 0;
@@ -399,12 +359,12 @@ __device__ __forceinline__ void copies(const TreeParams& p, const TreeMaps& maps
 
 // ---- 8-bit: codes to values ----------------------------------------------------------------
 // Warps w = 0 .. 3 of the group for K or for V.
-template <int kMode, int kD, int kN, bool kIsV>
-__device__ __forceinline__ void widen_tiles(const TreeParams& p, SmemOf<kMode, kD, kN>& sm, int n, int w, int lane, bool& ok) {
-  using X = Shape<kMode, kD, kN>;
+template <int kMode, int kD, bool kPair, bool kIsV>
+__device__ __forceinline__ void widen_tiles(const TreeParams& p, SmemOf<kMode, kD, kPair>& sm, int n, int w, int lane, bool& ok) {
+  using X = Shape<kMode, kD, kPair>;
   constexpr int kPerRow = kD / 16;                  // 16-byte chunks of codes in a row
   constexpr int kRowsPer = 32 / kPerRow;            // rows of one step of the warp: 4 or 8
-  constexpr int kPair = 8 / kRowsPer;               // steps until the pattern of rows repeats, 1024 bytes on
+  constexpr int kTurn = 8 / kRowsPer;               // steps until the pattern of rows repeats, 1024 bytes on
   // lane -> (chunk, row of the step): eight lanes in a row write the eight
   // 16-byte banks of two rows, whose value chunks are two apart
   const int chunk = kPerRow == 8 ? (lane & 3) | ((lane >> 1) & 4) : lane & 3;
@@ -412,9 +372,9 @@ __device__ __forceinline__ void widen_tiles(const TreeParams& p, SmemOf<kMode, k
   const bool chunk_real = chunk * 16 < p.c.head_dim;
   // offsets in a tile: codes, value chunks 2 chunk and 2 chunk + 1 (128-byte rows
   // of a 64-column block, chunks xor-ed with the row)
-  uint32_t from[kPair], to[kPair][2];
+  uint32_t from[kTurn], to[kTurn][2];
 #pragma unroll
-  for (int i = 0; i < kPair; ++i) {
+  for (int i = 0; i < kTurn; ++i) {
     const int r = 32 * w + i * kRowsPer + sub;
     from[i] = (uint32_t)((r >> 3) * 1024 + (r & 7) * p.c.head_dim + chunk * 16);
 #pragma unroll
@@ -436,19 +396,19 @@ __device__ __forceinline__ void widen_tiles(const TreeParams& p, SmemOf<kMode, k
     if (kMode == DCC_KV_E4M3 && kIsV) real = *reinterpret_cast<const uint32_t*>(&sm.vis[j % kRing][4 * w]) >> sub;
 #pragma unroll
     for (int half = 0; half < 2; ++half) {  // 16 rows at a time
-      uint4 raw[2 * kPair];
+      uint4 raw[2 * kTurn];
 #pragma unroll
-      for (int s = 0; s < 2 * kPair; ++s)
-        raw[s] = chunk_real && (kMode != DCC_KV_E4M3 || !kIsV || ((real >> (8 * (s / kPair + 2 * half) + s % kPair * kRowsPer)) & 1))
-                     ? ld_shared_v4(tile + from[s % kPair] + (s / kPair + 2 * half) * 1024)
+      for (int s = 0; s < 2 * kTurn; ++s)
+        raw[s] = chunk_real && (kMode != DCC_KV_E4M3 || !kIsV || ((real >> (8 * (s / kTurn + 2 * half) + s % kTurn * kRowsPer)) & 1))
+                     ? ld_shared_v4(tile + from[s % kTurn] + (s / kTurn + 2 * half) * 1024)
                      : make_uint4(0u, 0u, 0u, 0u);
       __syncwarp();  // this warp alone reads and writes these rows
 #pragma unroll
-      for (int s = 0; s < 2 * kPair; ++s) {
+      for (int s = 0; s < 2 * kTurn; ++s) {
         const uint2 a = widen<kMode>(raw[s].x), b = widen<kMode>(raw[s].y), c = widen<kMode>(raw[s].z), d = widen<kMode>(raw[s].w);
-        const uint32_t on = (s / kPair + 2 * half) * 1024;
-        st_shared_v4(tile + to[s % kPair][0] + on, a.x, a.y, b.x, b.y);
-        st_shared_v4(tile + to[s % kPair][1] + on, c.x, c.y, d.x, d.y);
+        const uint32_t on = (s / kTurn + 2 * half) * 1024;
+        st_shared_v4(tile + to[s % kTurn][0] + on, a.x, a.y, b.x, b.y);
+        st_shared_v4(tile + to[s % kTurn][1] + on, c.x, c.y, d.x, d.y);
       }
     }
     fence_proxy_async_smem();
@@ -458,56 +418,13 @@ __device__ __forceinline__ void widen_tiles(const TreeParams& p, SmemOf<kMode, k
   }
 }
 
-// ---- S issuer -----------------------------------------------------------------------
-template <int kMode, int kD, int kN>
-__device__ __forceinline__ void score_issuer(const TreeParams& p, SmemOf<kMode, kD, kN>& sm, int n, uint32_t tm, int lane,
-                                             bool& ok) {
-  using X = Shape<kMode, kD, kN>;
-  const uint32_t id = X::k8 ? idesc_f16_f32(128, kN, 0, 0) : idesc_bf16_f32(128, kN, 0, 0);
-  Tiles t;
-  t.start(p, sm.span);
-  Place<X::kSlotsK> at;
-  uint32_t pieces = 0;
-  const uint64_t q = desc_at(smem_u32(sm.q), 16);
-  const uint32_t k0 = smem_u32(sm.slot[0]);
-#pragma unroll 1
-  for (int j = 0; j < n; ++j) {
-    t.next(p, sm.span);
-    const int stream = j % X::kStreams;
-    if (t.first) {
-      wait_or_skip(ok, &sm.bar_q, pieces & 1);
-      ++pieces;
-    }
-    // the softmax has read the scores of the stream's last tile
-    if (j >= X::kStreams) wait_or_skip(ok, &sm.bar_p[stream], (uint32_t)(j / X::kStreams - 1) & 1);
-    wait_or_skip(ok, &sm.bar_full[at.slot], at.use);
-    tc_fence_after();
-    if (lane == 0) {
-      const uint64_t k = desc_at(k0 + (uint32_t)at.slot * X::kTile, 16);
-#pragma unroll
-      for (int kk = 0; kk < kD / 16; ++kk)
-        umma_ss(tm + X::kColS + (uint32_t)stream * kN, k + ((kk >> 2) * 16384 + (kk & 3) * 32) / 16,
-                q + ((kk >> 2) * (kN * 128) + (kk & 3) * 32) / 16, id, kk > 0);
-      umma_commit(&sm.bar_s[stream]);
-      umma_commit(&sm.bar_empty[at.slot]);
-      if (t.last) umma_commit(&sm.bar_qfree);
-    }
-    __syncwarp();
-    at.next();
-  }
-  // every MMA has finished before TMEM is freed, also after a wait that ran out
-  if (lane == 0) umma_commit(&sm.bar_end);
-  __syncwarp();
-  if (!wait_all_lanes(&sm.bar_end, 0)) ok = false;
-}
-
-// ---- O issuer -----------------------------------------------------------------------
+// ---- MMA issuer ----------------------------------------------------------------------
 // bf16 value rows that do not exist hold whatever the page or the slot held,
 // and newest values that are not finite must not reach rows that do not see
 // them (0 * inf): both become zeros here; the softmax marks the rows that do
 // see the latter.  (8-bit codes are always finite.)
-template <int kMode, int kD, int kN>
-__device__ __forceinline__ void clear_values(SmemOf<kMode, kD, kN>& sm, uint32_t tile, int ring, bool newest, int64_t first,
+template <int kMode, int kD, bool kPair>
+__device__ __forceinline__ void clear_values(SmemOf<kMode, kD, kPair>& sm, uint32_t tile, int ring, bool newest, int64_t first,
                                              int lane) {
   constexpr int kPerRow = kD / 8, kRowsPer = 32 / kPerRow;
   const int chunk = lane % kPerRow, sub = lane / kPerRow;
@@ -532,404 +449,462 @@ __device__ __forceinline__ void clear_values(SmemOf<kMode, kD, kN>& sm, uint32_t
   __syncwarp();
 }
 
-template <int kMode, int kD, int kN>
-__device__ __forceinline__ void value_issuer(const TreeParams& p, SmemOf<kMode, kD, kN>& sm, int n, bool guard, uint32_t tm,
-                                             int lane, bool& ok) {
-  using X = Shape<kMode, kD, kN>;
-  const uint32_t id = X::k8 ? idesc_f16_f32(128, kN, 1, 1) : idesc_bf16_f32(128, kN, 1, 1);
-  // with 64 columns both halves of the 128 MMA rows read the same block
-  constexpr uint32_t kNextBlock = X::kBlocks == 2 ? 16384 : 0;
-  Tiles t;
-  t.start(p, sm.span);
-  Place<X::kSlotsV> at;
-  const uint32_t v0 = smem_u32(sm.slot[X::kSlotsK]), p0 = smem_u32(sm.p);
-#pragma unroll 1
-  for (int j = 0; j < n; ++j) {
-    t.next(p, sm.span);
-    const int stream = j % X::kStreams;
-    wait_or_skip(ok, &sm.bar_full[X::kSlotsK + at.slot], at.use);
-    const uint32_t tile = v0 + (uint32_t)at.slot * X::kTile;
+template <int kMode, int kD, bool kPair>
+__device__ __forceinline__ void issuer(const TreeParams& p, SmemOf<kMode, kD, kPair>& sm, int n, bool guard, uint32_t tm, int lane,
+                                       bool& ok) {
+  using X = Shape<kMode, kD, kPair>;
+  const uint32_t id_s = X::k8 ? idesc_f16_f32(128, 128, 0, 0) : idesc_bf16_f32(128, 128, 0, 0);
+  const uint32_t id_o = X::k8 ? idesc_f16_f32(128, kD, 0, 1) : idesc_bf16_f32(128, kD, 0, 1);
+  const uint64_t q0 = desc_at(smem_u32(sm.q[0]), 16);
+  const uint32_t k0 = smem_u32(sm.slot[0]), v0 = smem_u32(sm.slot[X::kSlotsK]);
+  Tiles ts, tv;  // of the next scores, of the next values
+  ts.start(p, sm.span);
+  tv.start(p, sm.span);
+  Place<X::kSlotsK> at_k;
+  Place<X::kSlotsV> at_v;
+  uint32_t pieces = 0;
+  auto scores = [&](int stream, uint64_t q, uint64_t k) {
+    if (lane == 0) {
+#pragma unroll
+      for (int kk = 0; kk < kD / 16; ++kk)
+        umma_ss(tm + X::kColS + (uint32_t)stream * 128, q + ((kk >> 2) * 16384 + (kk & 3) * 32) / 16,
+                k + ((kk >> 2) * 16384 + (kk & 3) * 32) / 16, id_s, kk > 0);
+      umma_commit(&sm.bar_s[stream]);
+    }
+    __syncwarp();
+  };
+  // the K tile of `ts` is there, and the queries of its piece
+  auto this_k = [&]() {
+    if (ts.first) {
+      wait_or_skip(ok, &sm.bar_q, pieces & 1);
+      ++pieces;
+    }
+    wait_or_skip(ok, &sm.bar_full[at_k.slot], at_k.use);
+    tc_fence_after();
+    return desc_at(k0 + (uint32_t)at_k.slot * X::kTile, 16);
+  };
+  auto done_k = [&]() {
+    if (lane == 0) umma_commit(&sm.bar_empty[at_k.slot]);
+    __syncwarp();
+    at_k.next();
+  };
+  auto next_v = [&](int j) {
+    tv.next(p, sm.span);
+    wait_or_skip(ok, &sm.bar_full[X::kSlotsK + at_v.slot], at_v.use);
+    const uint32_t tile = v0 + (uint32_t)at_v.slot * X::kTile;
     if constexpr (!X::k8) {
       const int ring = j % kRing;
       wait_or_skip(ok, &sm.bar_side[ring], (uint32_t)(j / kRing) & 1);
       const uint4 vis = *reinterpret_cast<const uint4*>(sm.vis[ring]);
-      const int64_t first = (int64_t)t.kt * kTreeKeys - t.w.s.ctx;  // of the tile, behind the context
+      const int64_t first = (int64_t)tv.kt * kTreeKeys - tv.w.s.ctx;  // of the tile, behind the context
       const bool newest = guard && first + kTreeKeys > 0;
       if ((vis.x & vis.y & vis.z & vis.w) != 0xffffffffu || newest)
-        clear_values<kMode, kD, kN>(sm, tile, ring, newest, first, lane);
+        clear_values<kMode, kD, kPair>(sm, tile, ring, newest, first, lane);
     }
-    wait_or_skip(ok, &sm.bar_p[stream], (uint32_t)(j / X::kStreams) & 1);
+    return desc_at(tile, 16384);
+  };
+  auto values = [&](int stream, uint64_t v, bool first) {
     tc_fence_after();
     if (lane == 0) {
-      const uint64_t v = desc_at(tile, kNextBlock), pr = desc_at(p0 + (uint32_t)stream * X::kPStep, 0);
-      const bool first = t.kt - t.w.k0 < X::kStreams;  // of the stream in this piece
 #pragma unroll
       for (int kk = 0; kk < 8; ++kk)
-        umma_ss(tm + X::kColO + (uint32_t)stream * kN, v + kk * 128, pr + kk * 128, id, (first && kk == 0) ? 0u : 1u);
-      umma_commit(&sm.bar_empty[X::kSlotsK + at.slot]);
+        umma_ts(tm + X::kColO + (uint32_t)stream * 128, tm + X::kColS + (uint32_t)stream * 128 + kk * 8, v + kk * 128, id_o,
+                (first && kk == 0) ? 0u : 1u);
       umma_commit(&sm.bar_o[stream]);
     }
     __syncwarp();
-    at.next();
+  };
+  auto done_v = [&]() {
+    if (lane == 0) umma_commit(&sm.bar_empty[X::kSlotsK + at_v.slot]);
+    __syncwarp();
+    at_v.next();
+  };
+  // A stream's next scores overwrite its last weights: they are issued behind
+  // the product that reads those, and MMAs of one thread run in order.
+  if constexpr (kPair) {
+    ts.next(p, sm.span);
+    uint64_t k = this_k();
+    scores(0, q0, k);
+    scores(1, q0 + X::kTile / 16, k);
+    done_k();
+#pragma unroll 1
+    for (int j = 0; j < n; ++j) {
+      const uint64_t v = next_v(j);
+      const bool first = tv.first, more = j + 1 < n;
+      wait_or_skip(ok, &sm.bar_p[0], (uint32_t)j & 1);
+      values(0, v, first);
+      // with a new piece the queries change: only behind both streams' products
+      if (more && !tv.last) {
+        ts.next(p, sm.span);
+        k = this_k();
+        scores(0, q0, k);
+      }
+      wait_or_skip(ok, &sm.bar_p[1], (uint32_t)j & 1);
+      values(1, v, first);
+      done_v();
+      if (more) {
+        if (tv.last) {
+          ts.next(p, sm.span);
+          k = this_k();
+          scores(0, q0, k);
+        }
+        scores(1, q0 + X::kTile / 16, k);
+        done_k();
+      }
+    }
+  } else {
+    // scores run two tiles ahead of the products, but those of a new piece only
+    // start behind all products of the one before, whose end its queries wait for
+    int js = 0;
+    ts.next(p, sm.span);
+    auto feed = [&](int done) {
+      while (js < n && js < done + 2 && (!ts.first || js == done)) {
+        scores(js & 1, q0, this_k());
+        done_k();
+        if (++js < n) ts.next(p, sm.span);
+      }
+    };
+    feed(0);
+#pragma unroll 1
+    for (int j = 0; j < n; ++j) {
+      const uint64_t v = next_v(j);
+      const bool first = tv.kt - tv.w.k0 < 2;  // of the stream in this piece
+      wait_or_skip(ok, &sm.bar_p[j & 1], (uint32_t)(j >> 1) & 1);
+      values(j & 1, v, first);
+      done_v();
+      feed(j + 1);
+    }
   }
+  // every MMA has finished before TMEM is freed, also after a wait that ran out
   if (lane == 0) umma_commit(&sm.bar_end);
   __syncwarp();
   if (!wait_all_lanes(&sm.bar_end, 0)) ok = false;
 }
 
-// ---- queries -------------------------------------------------------------------------
-template <int kMode, int kD, int kN>
-__device__ __forceinline__ void queries(const TreeParams& p, SmemOf<kMode, kD, kN>& sm, int lane, bool& ok) {
-  using X = Shape<kMode, kD, kN>;
-  constexpr int kPerRow = kD / 8, kAll = kN * kPerRow, kBatch = 4;
-  const TreePlan& pl = sm.span;
-  uint32_t piece = 0;
+// ---- softmax and results --------------------------------------------------------------
+template <int kMode, int kD, bool kPair>
+__device__ __forceinline__ void softmax(const TreeParams& p, SmemOf<kMode, kD, kPair>& sm, bool guard, int span, uint32_t tm,
+                                        int stream, int wq, int lane, bool& ok) {
+  using X = Shape<kMode, kD, kPair>;
+  constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f, kMost = 3.402823466e38f;
+  const int row = 32 * wq + lane;  // of the tile; also a key, where keys are prepared
+  const int r = kPair ? 128 * stream + row : row;
+  const uint32_t lanes = tm + ((uint32_t)(32 * wq) << 16);
+  const uint32_t s_col = lanes + X::kColS + (uint32_t)stream * 128, o_col = lanes + X::kColO + (uint32_t)stream * 128;
+  const float scale = p.scale * kLog2e;
+  uint32_t mine = 0;  // tiles of this stream so far
+  int base = 0;       // tiles of the CTA before the piece
   for (int rt = blockIdx.x % p.n_groups; rt < p.n_row_tiles; rt += p.n_groups) {
     TreeWalk walk;
-    walk.start(p, pl);
+    walk.start(p, sm.span);
     TreePiece w;
     while (walk.next(p, w)) {
-      bool free = piece == 0;
+      // ---- the queries; the scores of the last piece have all been read ----
+      constexpr int kPerRow = kD / 8, kAll = X::kRows * kPerRow, kBatch = 4;
 #pragma unroll 1
-      for (int i0 = 0; i0 < kAll; i0 += 32 * kBatch) {
+      for (int i0 = 128 * stream + row; i0 < kAll; i0 += 256 * kBatch) {
         uint4 v[kBatch];
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
-          const int i = i0 + u * 32 + lane;
-          const int r = i / kPerRow, c = i % kPerRow;
+          const int i = i0 + 256 * u, c = i % kPerRow;
           v[u] = make_uint4(0u, 0u, 0u, 0u);
           if (c * 8 < p.c.head_dim) {
-            const TreeRow row = tree_row(p, w.hk, rt, r);
-            if (row.exists)
+            const TreeRow at = tree_row(p, w.hk, rt, i / kPerRow);
+            if (at.exists)
               v[u] = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.q.q) + w.b * p.q.q_seq_stride +
-                                                     row.h * p.q.q_head_stride + row.t * p.q.q_row_stride + c * 8);
+                                                     at.h * p.q.q_head_stride + at.t * p.q.q_row_stride + c * 8);
           }
-        }
-        if (!free) {
-          wait_or_skip(ok, &sm.bar_qfree, (piece - 1) & 1);
-          free = true;
         }
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
-          const int i = i0 + u * 32 + lane;
-          const int r = i / kPerRow, c = i % kPerRow;
+          const int i = i0 + 256 * u, rr = i / kPerRow, c = i % kPerRow;
           if constexpr (X::k8) {
             uint32_t h[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
             uint32_t top = 0;  // largest exponent field of the row's kPerRow lanes
 #pragma unroll
             for (int e = 0; e < 4; ++e) top = max(top, max((h[e] >> 7) & 0xffu, (h[e] >> 23) & 0xffu));
 #pragma unroll
-            for (int o = kPerRow / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+            for (int off = kPerRow / 2; off > 0; off >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, off));
             const int up = top == 0 || top == 255 ? 0 : min(14 + 127 - (int)top, 120);
             const float f = __uint_as_float((uint32_t)(127 + up) << 23);
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              h[e] = pack_half(__uint_as_float(h[e] << 16) * f, __uint_as_float(h[e] & 0xffff0000u) * f);
+            for (int e = 0; e < 4; ++e) h[e] = pack_half(__uint_as_float(h[e] << 16) * f, __uint_as_float(h[e] & 0xffff0000u) * f);
             v[u] = make_uint4(h[0], h[1], h[2], h[3]);
-            if (c == 0) sm.qf[piece % kPieces][r] = __uint_as_float((uint32_t)(127 - up) << 23);
+            if (c == 0) sm.qf[rr] = __uint_as_float((uint32_t)(127 - up) << 23);
           }
-          st_shared_v4(smem_u32(sm.q) + (c >> 3) * (kN * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4), v[u].x, v[u].y, v[u].z,
-                       v[u].w);
+          st_shared_v4(smem_u32(sm.q[rr >> 7]) + (uint32_t)((c >> 3) * 16384 + (rr & 127) * 128 + (((c & 7) ^ (rr & 7)) << 4)),
+                       v[u].x, v[u].y, v[u].z, v[u].w);
         }
       }
       fence_proxy_async_smem();
       mbar_arrive(&sm.bar_q);
-      ++piece;
-    }
-  }
-}
-
-// ---- softmax and results --------------------------------------------------------------
-template <int kMode, int kD, int kN>
-__device__ __forceinline__ void softmax(const TreeParams& p, SmemOf<kMode, kD, kN>& sm, bool guard, int span, uint32_t tm,
-                                        int stream, int wq, int lane, bool& ok) {
-  using X = Shape<kMode, kD, kN>;
-  constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f, kMost = 3.402823466e38f;
-  const int key = 32 * wq + lane;  // of a tile; also the head column of O^T
-  const uint32_t lanes = tm + ((uint32_t)(32 * wq) << 16);
-  const uint32_t s_col = lanes + X::kColS + (uint32_t)stream * kN;
-  const uint32_t o_col = lanes + X::kColO + (uint32_t)stream * kN;
-  const float scale = p.scale * kLog2e;
-  const uint32_t p_row = smem_u32(sm.p) + (uint32_t)((key >> 3) * 1024 + (key & 7) * 128) +
-                         (uint32_t)(kN == 64 ? stream * X::kPStep : 0);
-  const int p_chunk0 = kN == 64 ? 0 : stream * kN / 8;
-  uint32_t mine = 0;   // tiles of this stream so far
-  int base = 0;        // tiles of the CTA before the piece
-  uint32_t piece = 0;
-  for (int rt = blockIdx.x % p.n_groups; rt < p.n_row_tiles; rt += p.n_groups) {
-    TreeWalk walk;
-    walk.start(p, sm.span);
-    TreePiece w;
-    while (walk.next(p, w)) {
-      float l[kN];
-#pragma unroll
-      for (int c = 0; c < kN; ++c) l[c] = 0.f;
-      if (key < kN) sm.m[stream][key] = -INFINITY;
-      group_sync(stream);
+      softmax_sync();  // qf
+      const float unit = X::k8 ? scale * sm.qf[r] : scale;
+      const TreeRow own = tree_row(p, w.hk, rt, r);
+      float m = -INFINITY, l = 0.f;
       const int count = w.k1 - w.k0;
-      const int skip = (stream - base % X::kStreams + X::kStreams) % X::kStreams;
-      const float* qf = sm.qf[piece % kPieces];
+      const int skip = kPair ? 0 : (stream - base % 2 + 2) % 2;
 #pragma unroll 1
-      for (int it = skip; it < count; it += X::kStreams, ++mine) {
+      for (int it = skip; it < count; it += kPair ? 1 : 2, ++mine) {
         const int j = base + it, ring = j % kRing;
-        const bool first = it < X::kStreams;
-        // which rows see this thread's key
-        const int64_t i = (int64_t)(w.k0 + it) * kTreeKeys + key - w.s.ctx;  // >= 0: newest token i
-        bool broken = false;
-        uint64_t see = ~0ull;
-        if (i >= 0) {
-          see = 0;
-          if (i < w.s.cnt) {
-            int64_t row = (int64_t)rt * kN;
-            int64_t tok = row / p.group;
-            int g = (int)(row - tok * p.group);
-#pragma unroll 1
-            for (int c = 0; c < kN; ++c) {
-              if (tok < p.q.T && tree_sees(p, w.b, tok, i)) see |= 1ull << c;
-              if (++g == p.group) {
-                g = 0;
-                ++tok;
-              }
-            }
-            if (!X::k8 && guard) {
-              // is the value finite?  (8-bit rows that are not have a NaN scale)
-              const PageWalk pages{p.q.page_table + w.b * p.q.table_stride, p.c.n_pages, p.c.page_size, p.q.max_pages};
-              int off = 0;
-              const int64_t page = pages.page_of(i + w.s.ctx, off);
-              if (page >= 0) {
-                const uint4* v = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.c.v) +
-                                                                page_row(p.c, page, w.hk, off) * p.c.head_dim);
-                for (int c = 0; c < p.c.head_dim / 8; ++c) {
-                  const uint4 x = __ldg(v + c);
-                  const uint32_t u[4] = {x.x, x.y, x.z, x.w};
+        const bool first = it == skip;
+        const int64_t i0 = (int64_t)(w.k0 + it) * kTreeKeys - w.s.ctx;  // of the tile's first key; >= 0: newest token
+        // ---- the keys of the tile, one a thread ----
+        wait_or_skip(ok, &sm.bar_side[ring], (uint32_t)(j / kRing) & 1);
+        const uint4 vis = *reinterpret_cast<const uint4*>(sm.vis[ring]);
+        bool hidden = (vis.x & vis.y & vis.z & vis.w) != 0xffffffffu || i0 + kTreeKeys > 0;
+        bool prepared = false;
+        if (X::k8 || p.c.bias || (hidden && guard)) {
+          prepared = true;
+          float bias = p.c.bias ? sm.side[ring][0][row] : 0.f;
+          if (bias > -INFINITY && bias < INFINITY) bias = fminf(fmaxf(bias * kLog2e, -kMost), kMost);
+          const int64_t i = i0 + row;
+          if (!X::k8 && guard && i >= 0 && i < w.s.cnt) {
+            // a newest value that is not finite: the rows that see it become NaN
+            // (8-bit rows that are not finite have a NaN scale)
+            const PageWalk pages{p.q.page_table + w.b * p.q.table_stride, p.c.n_pages, p.c.page_size, p.q.max_pages};
+            int off = 0;
+            const int64_t page = pages.page_of(i + w.s.ctx, off);
+            if (page >= 0) {
+              const uint4* v = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.c.v) +
+                                                              page_row(p.c, page, w.hk, off) * p.c.head_dim);
+              for (int c = 0; c < p.c.head_dim / 8; ++c) {
+                const uint4 x = __ldg(v + c);
+                const uint32_t u[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-                  for (int e = 0; e < 4; ++e)
-                    broken = broken || (u[e] & 0x7f80u) == 0x7f80u || (u[e] & 0x7f800000u) == 0x7f800000u;
-                }
+                for (int e = 0; e < 4; ++e)
+                  if ((u[e] & 0x7f80u) == 0x7f80u || (u[e] & 0x7f800000u) == 0x7f800000u) bias = __uint_as_float(0x7fc00000u);
               }
             }
           }
+          group_sync(stream);  // the arrays of the last tile have been read
+          sm.bias[stream][row] = bias;
+          if constexpr (X::k8) {
+            const float vs = fmaxf(sm.side[ring][2][row], 7.888609e-31f);  // 2^-100: rows that were never written have scale 0
+            sm.ks[stream][row] = sm.side[ring][1][row];
+            sm.vs[stream][row] = sm.side[ring][2][row] < 7.888609e-31f ? vs : sm.side[ring][2][row];
+            sm.lift[stream][row] = __log2f(vs);
+          }
+          group_sync(stream);
         }
-        wait_or_skip(ok, &sm.bar_side[ring], (uint32_t)(j / kRing) & 1);
-        const bool exists = (sm.vis[ring][key >> 3] >> (key & 7)) & 1;
-        float bias = 0.f, ks = scale, vs = 1.f;
-        if (p.c.bias) {
-          bias = sm.side[ring][0][key];
-          if (bias > -INFINITY && bias < INFINITY) bias = fminf(fmaxf(bias * kLog2e, -kMost), kMost);
-        }
-        // what the V scale adds to the score (from 2^-100: rows that were never
-        // written have scale 0), and the score at which the max moves
-        float lift = 0.f;
-        if constexpr (X::k8) {
-          ks *= sm.side[ring][1][key];
-          vs = sm.side[ring][2][key];
-          lift = __log2f(fmaxf(vs, 7.888609e-31f));
-        }
-        const float most = 8.f - lift;
-        if (!exists || bias == -INFINITY) see = 0;
-        if (broken) bias = __uint_as_float(0x7fc00000u);  // the rows that see it become NaN
-        const bool all = __all_sync(0xffffffffu, see == ~0ull) != 0;
-
         wait_or_skip(ok, &sm.bar_s[stream], mine & 1);
         tc_fence_after();
-        float d[X::kChunk];
-        auto raw = [&](int ch) {
-          tmem_ld<X::kChunk>(s_col + ch * X::kChunk, reinterpret_cast<uint32_t*>(d));
+
+        // keys 32 c .. 32 c + 31 that this row sees
+        auto seen = [&](int c) {
+          uint32_t see = c == 0 ? vis.x : c == 1 ? vis.y : c == 2 ? vis.z : vis.w;
+          const int64_t i = i0 + 32 * c;
+          if (i + 32 > 0) {
+            const int from = i < 0 ? (int)-i : 0;  // the first newest token of the 32
+            const int64_t some = w.s.cnt - i;
+            const int to = some < 32 ? (int)(some < 0 ? 0 : some) : 32;
+            uint32_t yes = from > 0 ? 0xffffffffu >> (32 - from) : 0u;
+            if (own.exists)
+              for (int x = from; x < to; ++x)
+                if (tree_sees(p, w.b, own.t, i + x)) yes |= 1u << x;
+            see &= yes;
+          }
+          return see;
+        };
+        float d[32];
+        auto load = [&](int c) {
+          tmem_ld32(s_col + 32 * c, reinterpret_cast<uint32_t*>(d));
           tmem_wait_ld();
-          if constexpr (X::k8) {
+        };
+        // scores in powers of two
+        auto scores = [&](int c) {
+          load(c);
+          if (X::k8 || prepared) {
 #pragma unroll
-            for (int c = 0; c < X::kChunk; c += 4) {
-              const float4 f = *reinterpret_cast<const float4*>(qf + ch * X::kChunk + c);
-              d[c] *= f.x;
-              d[c + 1] *= f.y;
-              d[c + 2] *= f.z;
-              d[c + 3] *= f.w;
+            for (int x = 0; x < 32; x += 4) {
+              const float4 b = *reinterpret_cast<const float4*>(&sm.bias[stream][32 * c + x]);
+              float4 k = make_float4(1.f, 1.f, 1.f, 1.f);
+              if constexpr (X::k8) k = *reinterpret_cast<const float4*>(&sm.ks[stream][32 * c + x]);
+              d[x] = fmaf(d[x] * unit, k.x, b.x);
+              d[x + 1] = fmaf(d[x + 1] * unit, k.y, b.y);
+              d[x + 2] = fmaf(d[x + 2] * unit, k.z, b.z);
+              d[x + 3] = fmaf(d[x + 3] * unit, k.w, b.w);
             }
-          }
-        };
-        // scores less the running max, in powers of two
-        auto load = [&](int ch) {
-          raw(ch);
-#pragma unroll
-          for (int c = 0; c < X::kChunk; c += 4) {
-            const float4 m = *reinterpret_cast<const float4*>(&sm.m[stream][ch * X::kChunk + c]);
-            d[c] = fmaf(d[c], ks, bias) - m.x;
-            d[c + 1] = fmaf(d[c + 1], ks, bias) - m.y;
-            d[c + 2] = fmaf(d[c + 2], ks, bias) - m.z;
-            d[c + 3] = fmaf(d[c + 3], ks, bias) - m.w;
-          }
-        };
-        bool over = false;
-#pragma unroll
-        for (int ch = X::kChunks - 1; ch >= 0; --ch) {
-          load(ch);
-          if (all) {
-#pragma unroll
-            for (int c = 0; c < X::kChunk; ++c) over = over || d[c] > most;
           } else {
 #pragma unroll
-            for (int c = 0; c < X::kChunk; ++c) over = over || (d[c] > most && ((see >> (ch * X::kChunk + c)) & 1));
+            for (int x = 0; x < 32; ++x) d[x] *= unit;
           }
-        }
-        // (the vote also keeps a warp from moving the max that another still reads)
-        if (group_any(stream, over)) {
-          // move the max of every row to the largest score so far, rescale
+        };
+        // ---- largest score (with its V scale) ----
+        float top = -INFINITY;
+        const bool bare = !X::k8 && !prepared && !hidden && unit > 0.f;  // the scores themselves, scaled last
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          if (bare) {
+            load(c);
 #pragma unroll
-          for (int ch = 0; ch < X::kChunks; ++ch) {
-            raw(ch);
+            for (int x = 0; x < 32; ++x) mx[x & 3] = fmaxf(mx[x & 3], d[x]);
+          } else {
+            scores(c);
+            const uint32_t see = hidden ? seen(c) : 0xffffffffu;
 #pragma unroll
-            for (int c = 0; c < X::kChunk; ++c) {
-              const float x = fmaf(d[c], ks, bias) + lift;
-              // floats as integers of the same order; NaN counts as nothing
-              const int bits = __float_as_int((((see >> (ch * X::kChunk + c)) & 1) && x == x) ? x : -INFINITY);
-              const int top = __reduce_max_sync(0xffffffffu, bits ^ ((bits >> 31) & 0x7fffffff));
-              if (lane == 0) sm.red[stream][wq][ch * X::kChunk + c] = __int_as_float(top ^ ((top >> 31) & 0x7fffffff));
+            for (int x = 0; x < 32; x += 4) {
+              float4 up = make_float4(0.f, 0.f, 0.f, 0.f);
+              if constexpr (X::k8) up = *reinterpret_cast<const float4*>(&sm.lift[stream][32 * c + x]);
+              mx[0] = fmaxf(mx[0], (see >> x) & 1 ? d[x] + up.x : -INFINITY);
+              mx[1] = fmaxf(mx[1], (see >> (x + 1)) & 1 ? d[x + 1] + up.y : -INFINITY);
+              mx[2] = fmaxf(mx[2], (see >> (x + 2)) & 1 ? d[x + 2] + up.z : -INFINITY);
+              mx[3] = fmaxf(mx[3], (see >> (x + 3)) & 1 ? d[x + 3] + up.w : -INFINITY);
             }
           }
-          group_sync(stream);
-          if (key < kN) {
-            const float m0 = sm.m[stream][key];
-            const float m1 = fmaxf(fmaxf(fmaxf(sm.red[stream][0][key], sm.red[stream][1][key]),
-                                         fmaxf(sm.red[stream][2][key], sm.red[stream][3][key])), m0);
-            sm.sum[stream][key] = m0 == m1 ? 1.f : exp2f(m0 - m1);
-            sm.m[stream][key] = m1;
-          }
-          if (!first) wait_or_skip(ok, &sm.bar_o[stream], (mine - 1) & 1);
-          tc_fence_after();
-          group_sync(stream);
-#pragma unroll
-          for (int ch = 0; ch < X::kChunks; ++ch) {
-            if (!first) {
-              tmem_ld<X::kChunk>(o_col + ch * X::kChunk, reinterpret_cast<uint32_t*>(d));
+          top = fmaxf(top, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+        }
+        if (bare) top *= unit;
+        const bool move = top > m + 8.f;
+        if (__any_sync(0xffffffffu, move)) {
+          const float f = move ? exp2f(m - top) : 1.f;  // 0 for the first score of a row
+          if (!first) {
+            wait_or_skip(ok, &sm.bar_o[stream], (mine - 1) & 1);
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < kD / 32; ++c) {
+              tmem_ld32(o_col + 32 * c, reinterpret_cast<uint32_t*>(d));
               tmem_wait_ld();
-            }
 #pragma unroll
-            for (int c = 0; c < X::kChunk; ++c) {
-              const float f = sm.sum[stream][ch * X::kChunk + c];
-              l[ch * X::kChunk + c] *= f;
-              d[c] *= f;
+              for (int x = 0; x < 32; ++x) d[x] *= f;
+              tmem_st32(o_col + 32 * c, reinterpret_cast<const uint32_t*>(d));
             }
-            if (!first) tmem_st<X::kChunk>(o_col + ch * X::kChunk, reinterpret_cast<const uint32_t*>(d));
+            tmem_wait_st();
           }
-          if (!first) tmem_wait_st();
-          load(0);
+          l *= f;
+          if (move) m = top;
         }
-        // the stream's last products have read P
-        if (mine > 0) wait_or_skip(ok, &sm.bar_o[stream], (mine - 1) & 1);
+        // ---- weights, over the scores ----
+        const float less = m == -INFINITY ? 0.f : m;
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          uint32_t see = 0xffffffffu;
+          if (bare) {
+            load(c);
 #pragma unroll
-        for (int ch = 0; ch < X::kChunks; ++ch) {
-          if (ch > 0) load(ch);
+            for (int x = 0; x < 32; ++x) d[x] = exp2_approx(fmaf(d[x], unit, -less));
+          } else {
+            scores(c);
 #pragma unroll
-          for (int c8 = 0; c8 < X::kChunk; c8 += 8) {
-            uint32_t h[4];
+            for (int x = 0; x < 32; ++x) d[x] = exp2_approx(d[x] - less);
+            if (hidden) {
+              see = seen(c);
 #pragma unroll
-            for (int c = 0; c < 8; c += 2) {
-              float e0 = exp2_approx(d[c8 + c]), e1 = exp2_approx(d[c8 + c + 1]);
-              if (!all) {
-                const uint32_t two = (uint32_t)(see >> (ch * X::kChunk + c8 + c));
-                e0 = two & 1 ? e0 : 0.f;
-                e1 = two & 2 ? e1 : 0.f;
-              }
-              l[ch * X::kChunk + c8 + c] += e0;
-              l[ch * X::kChunk + c8 + c + 1] += e1;
-              if (X::k8) {  // a hidden key's scale may be NaN
-                e0 = all || e0 != 0.f ? e0 * vs : 0.f;
-                e1 = all || e1 != 0.f ? e1 * vs : 0.f;
-              }
-              h[c / 2] = X::k8 ? pack_half(e0, e1) : pack2(e0, e1);
+              for (int x = 0; x < 32; ++x) d[x] = (see >> x) & 1 ? d[x] : 0.f;
             }
-            const int chunk = p_chunk0 + (ch * X::kChunk + c8) / 8;
-            st_shared_v4(p_row + (uint32_t)((chunk ^ (key & 7)) << 4), h[0], h[1], h[2], h[3]);
           }
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int x = 0; x < 32; ++x) sum[x & 3] += d[x];
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          uint32_t h[16];
+          if constexpr (X::k8) {
+#pragma unroll
+            for (int x = 0; x < 32; x += 4) {
+              float4 v = *reinterpret_cast<const float4*>(&sm.vs[stream][32 * c + x]);
+              if (hidden) {  // a hidden key's scale may be NaN
+                v.x = (see >> x) & 1 ? v.x : 0.f;
+                v.y = (see >> (x + 1)) & 1 ? v.y : 0.f;
+                v.z = (see >> (x + 2)) & 1 ? v.z : 0.f;
+                v.w = (see >> (x + 3)) & 1 ? v.w : 0.f;
+              }
+              h[x / 2] = pack_half(d[x] * v.x, d[x + 1] * v.y);
+              h[x / 2 + 1] = pack_half(d[x + 2] * v.z, d[x + 3] * v.w);
+            }
+          } else {
+#pragma unroll
+            for (int x = 0; x < 32; x += 2) h[x / 2] = pack2(d[x], d[x + 1]);
+          }
+          tmem_st16(s_col + 16 * c, h);  // over scores that have been read
         }
-        fence_proxy_async_smem();
+        tmem_wait_st();
         tc_fence_before();
         mbar_arrive(&sm.bar_p[stream]);
       }
 
-      // ---- the piece is done: sums over the keys, streams together ----
-#pragma unroll
-      for (int c = 0; c < kN; ++c) {
-        const float s = warp_sum(l[c]);
-        if (lane == 0) sm.red[stream][wq][c] = s;
-      }
-      group_sync(stream);
-      if (key < kN)
-        sm.sum[stream][key] = (sm.red[stream][0][key] + sm.red[stream][1][key]) + (sm.red[stream][2][key] + sm.red[stream][3][key]);
+      // ---- the piece is done ----
       if (skip < count) wait_or_skip(ok, &sm.bar_o[stream], (mine - 1) & 1);
-      all_streams_sync<X::kStreams>();
+      sm.ml[stream][row] = make_float2(m, l);
+      softmax_sync();
       tc_fence_after();
-      // O^T: thread = head column, this stream's share of the rows
-      const int64_t row0 = (int64_t)rt * kN + stream * X::kOut;
-      int64_t tok = row0 / p.group;
-      int g = (int)(row0 - tok * p.group);
-      const int64_t part0 = w.part >= 0 ? p.part_row(span, rt, w.part, stream * X::kOut) : 0;
-      constexpr int kSub = X::kOut < 8 ? X::kOut : 8;
+      const bool other = !kPair && count > 1;  // both streams had a tile
+      float f0 = 1.f, f1 = 0.f, top = m, sum = l;  // of stream 0 and 1, or of this stream
+      if constexpr (!kPair) {
+        const float2 a = sm.ml[0][row], b = sm.ml[1][row];
+        top = fmaxf(a.x, b.x);
+        f0 = a.y == 0.f ? 0.f : a.x == top ? 1.f : exp2f(a.x - top);
+        f1 = b.y == 0.f ? 0.f : b.x == top ? 1.f : exp2f(b.x - top);
+        sum = (a.y == 0.f ? 0.f : f0 * a.y) + (b.y == 0.f ? 0.f : f1 * b.y);
+      } else if (l == 0.f) {
+        f0 = 0.f;
+      }
+      // a piece of one tile lies in one stream
+      const uint32_t col_a = lanes + X::kColO + (uint32_t)(kPair ? stream : other ? 0 : base % 2) * 128;
+      const float fa = kPair || other ? f0 : base % 2 ? f1 : f0;
+      if (own.t >= w.s.cnt) sum = 0.f;  // a row that does not exist
+      // -kMost: nothing but biases of the type's lowest value
+      const float ln = top == -kMost ? -kMost : top * kLn2;
+      const int64_t part = w.part >= 0 ? p.part_row(span, rt, w.part, r) : 0;
+      const float inv = sum != 0.f ? 1.f / sum : 0.f;
+      __nv_bfloat16* out = tree_out_row<__nv_bfloat16>(p, w.b, own);
+      const bool wide = ((reinterpret_cast<uintptr_t>(out) & 15u) == 0);
+      const int c_first = kPair ? 0 : stream * (kD / 64), c_last = kPair ? kD / 32 : (stream + 1) * (kD / 64);
 #pragma unroll 1
-      for (int c0 = 0; c0 < X::kOut; c0 += kSub) {
-        float o[kSub], total[kSub], top[kSub];
+      for (int c = c_first; c < c_last; ++c) {
+        float d[32];
+        tmem_ld32(col_a + 32 * c, reinterpret_cast<uint32_t*>(d));
+        tmem_wait_ld();
 #pragma unroll
-        for (int c = 0; c < kSub; ++c) {
-          o[c] = total[c] = 0.f;
-          top[c] = -INFINITY;
-#pragma unroll
-          for (int s = 0; s < X::kStreams; ++s) top[c] = fmaxf(top[c], sm.m[s][stream * X::kOut + c0 + c]);
-        }
-#pragma unroll
-        for (int s = 0; s < X::kStreams; ++s) {
-          if ((s - base % X::kStreams + X::kStreams) % X::kStreams >= count) continue;  // no tile of the piece
-          float part[kSub];
-          tmem_ld<kSub>(lanes + X::kColO + (uint32_t)(s * kN + stream * X::kOut + c0), reinterpret_cast<uint32_t*>(part));
+        for (int x = 0; x < 32; ++x) d[x] = fa == 0.f ? 0.f : fa * d[x];
+        if (other) {
+          float e[32];
+          tmem_ld32(col_a + 128 + 32 * c, reinterpret_cast<uint32_t*>(e));
           tmem_wait_ld();
 #pragma unroll
-          for (int c = 0; c < kSub; ++c) {
-            const int col = stream * X::kOut + c0 + c;
-            const float ls = sm.sum[s][col];
-            if (ls != 0.f) {  // that stream saw a key of this row
-              const float f = sm.m[s][col] == top[c] ? 1.f : exp2f(sm.m[s][col] - top[c]);
-              o[c] = fmaf(f, part[c], o[c]);
-              total[c] = fmaf(f, ls, total[c]);
-            }
-          }
+          for (int x = 0; x < 32; ++x) d[x] = f1 == 0.f ? d[x] : fmaf(f1, e[x], d[x]);
         }
+        if (!own.exists) continue;
+        if (w.part >= 0) {
 #pragma unroll
-        for (int c = 0; c < kSub; ++c) {
-          const float sum = tok < w.s.cnt ? total[c] : 0.f;  // a row that does not exist has none
-          // -kMost: nothing but biases of the type's lowest value
-          const float m = top[c] == -kMost ? -kMost : top[c] * kLn2;
-          if (tok < p.q.T) {
-            if (w.part >= 0) {
-              if (key < p.c.head_dim) p.part_o[(part0 + c0 + c) * kTreePartCols + key] = o[c];
-              if (key == 0) *reinterpret_cast<float2*>(p.part_ml + (part0 + c0 + c) * 2) = make_float2(m, sum);
+          for (int x = 0; x < 32; x += 4)
+            if (32 * c + x < p.c.head_dim)
+              *reinterpret_cast<float4*>(p.part_o + part * kTreePartCols + 32 * c + x) = make_float4(d[x], d[x + 1], d[x + 2], d[x + 3]);
+        } else {
+#pragma unroll
+          for (int x = 0; x < 32; ++x) d[x] = sum != 0.f ? d[x] * inv : 0.f;
+#pragma unroll
+          for (int x = 0; x < 32; x += 8) {
+            if (32 * c + x >= p.c.head_dim) continue;
+            const uint4 h = make_uint4(pack2(d[x], d[x + 1]), pack2(d[x + 2], d[x + 3]), pack2(d[x + 4], d[x + 5]), pack2(d[x + 6], d[x + 7]));
+            if (wide) {
+              *reinterpret_cast<uint4*>(out + 32 * c + x) = h;
             } else {
-              const TreeRow row{tok, w.hk * p.group + g, true};
-              if (key < p.c.head_dim)
-                tree_out_row<__nv_bfloat16>(p, w.b, row)[key] = __float2bfloat16_rn(sum != 0.f ? o[c] / sum : 0.f);
-              if (key == 0 && p.q.lse)
-                p.q.lse[((int64_t)w.b * p.q.n_q_heads + row.h) * p.q.T + tok] = sum != 0.f ? m + logf(sum) : -INFINITY;
+#pragma unroll
+              for (int e = 0; e < 8; ++e) out[32 * c + x + e] = __float2bfloat16_rn(d[x + e]);
             }
-          }
-          if (++g == p.group) {
-            g = 0;
-            ++tok;
           }
         }
       }
+      if (own.exists && (kPair || stream == 0)) {
+        if (w.part >= 0) *reinterpret_cast<float2*>(p.part_ml + part * 2) = make_float2(ln, sum);
+        else if (p.q.lse)
+          p.q.lse[((int64_t)w.b * p.q.n_q_heads + own.h) * p.q.T + own.t] = sum != 0.f ? ln + logf(sum) : -INFINITY;
+      }
       tc_fence_before();
-      all_streams_sync<X::kStreams>();  // m, sums and O are free again
+      softmax_sync();  // ml, O and the queries are free again
       base += count;
-      ++piece;
     }
   }
 }
 
-template <int kMode, int kD, int kN>
-__global__ void __launch_bounds__(Shape<kMode, kD, kN>::kThreads, 1) tree_tc05_kernel(const __grid_constant__ TreeParams p,
-                                                                                      const __grid_constant__ TreeMaps maps,
-                                                                                      unsigned int* error) {
-  using X = Shape<kMode, kD, kN>;
+template <int kMode, int kD, bool kPair>
+__global__ void __launch_bounds__(Shape<kMode, kD, kPair>::kThreads, 1) tree_tc05_kernel(const __grid_constant__ TreeParams p,
+                                                                                        const __grid_constant__ TreeMaps maps,
+                                                                                        unsigned int* error) {
+  using X = Shape<kMode, kD, kPair>;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
-  SmemOf<kMode, kD, kN>& sm = *reinterpret_cast<SmemOf<kMode, kD, kN>*>(smem_raw);
+  SmemOf<kMode, kD, kPair>& sm = *reinterpret_cast<SmemOf<kMode, kD, kPair>*>(smem_raw);
   if (smem_u32(smem_raw) & 1023u) {  // the swizzled tiles need it
     if (threadIdx.x == 0) atomicOr(error, 64u);
     return;
@@ -949,19 +924,17 @@ __global__ void __launch_bounds__(Shape<kMode, kD, kN>::kThreads, 1) tree_tc05_k
       mbar_init(&sm.bar_raw[i], 1);
     }
     for (int i = 0; i < kRing; ++i) mbar_init(&sm.bar_side[i], 1);
-    mbar_init(&sm.bar_q, 32);
-    mbar_init(&sm.bar_qfree, 1);
-    for (int i = 0; i < X::kStreams; ++i) {
+    mbar_init(&sm.bar_q, 256);
+    for (int i = 0; i < 2; ++i) {
       mbar_init(&sm.bar_s[i], 1);
       mbar_init(&sm.bar_p[i], 128);
       mbar_init(&sm.bar_o[i], 1);
     }
-    mbar_init(&sm.bar_end, 2);
+    mbar_init(&sm.bar_end, 1);
     fence_mbar_init();
   }
-  constexpr int kWork = 4 * X::kStreams;  // first warp behind the softmax
-  if (warp == kWork) {
-    tmem_alloc(&sm.tmem, X::kTmem);
+  if (warp == 8) {
+    tmem_alloc(&sm.tmem, 512);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -971,32 +944,30 @@ __global__ void __launch_bounds__(Shape<kMode, kD, kN>::kThreads, 1) tree_tc05_k
   // rows may hide newest tokens from one another
   const bool guard = p.q.T > 1 || p.q.tree != nullptr;
   bool ok = true;
-  if (warp < kWork) {
+  if (warp < 8) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(X::kRegsSoftmax));
-    softmax<kMode, kD, kN>(p, sm, guard, span, tm, warp >> 2, warp & 3, lane, ok);
-  } else if (warp < kWork + 4) {
+    softmax<kMode, kD, kPair>(p, sm, guard, span, tm, warp >> 2, warp & 3, lane, ok);
+  } else if (warp < 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(X::kRegsWork));
-    if (warp == kWork) score_issuer<kMode, kD, kN>(p, sm, n, tm, lane, ok);
-    else if (warp == kWork + 1) value_issuer<kMode, kD, kN>(p, sm, n, guard, tm, lane, ok);
-    else if (warp == kWork + 2) queries<kMode, kD, kN>(p, sm, lane, ok);
-    else copies<kMode, kD, kN>(p, maps, sm, n, lane, ok);
+    if (warp == 8) issuer<kMode, kD, kPair>(p, sm, n, guard, tm, lane, ok);
+    else if (warp == 9) copies<kMode, kD, kPair>(p, maps, sm, n, lane, ok);
   } else if constexpr (X::k8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(X::kRegsWiden));
-    if (warp < kWork + 8) widen_tiles<kMode, kD, kN, false>(p, sm, n, warp & 3, lane, ok);
-    else widen_tiles<kMode, kD, kN, true>(p, sm, n, warp & 3, lane, ok);
+    if (warp < 16) widen_tiles<kMode, kD, kPair, false>(p, sm, n, warp & 3, lane, ok);
+    else widen_tiles<kMode, kD, kPair, true>(p, sm, n, warp & 3, lane, ok);
   }
   if (!ok && lane == 0) atomicOr(error, 32u);
   tc_fence_before();
   __syncthreads();
-  if (warp == kWork) tmem_dealloc(tm, X::kTmem);
+  if (warp == 8) tmem_dealloc(tm, 512);
 }
 
-template <int kMode, int kD, int kN>
+template <int kMode, int kD, bool kPair>
 static int launch(const TreeParams& p, const TreeMaps& maps, unsigned int* error, cudaStream_t st) {
-  using X = Shape<kMode, kD, kN>;
-  constexpr size_t smem = sizeof(SmemOf<kMode, kD, kN>);
+  using X = Shape<kMode, kD, kPair>;
+  constexpr size_t smem = sizeof(SmemOf<kMode, kD, kPair>);
   static_assert(smem <= kSmemLimit, "shared memory");
-  auto kernel = tree_tc05_kernel<kMode, kD, kN>;
+  auto kernel = tree_tc05_kernel<kMode, kD, kPair>;
   DCC_CHECK(check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "tree_tc05 smem"));
   // setmaxnreg draws on the launch's registers: fewer than planned would wait forever
   cudaFuncAttributes fa{};
@@ -1007,17 +978,11 @@ static int launch(const TreeParams& p, const TreeMaps& maps, unsigned int* error
   kernel<<<p.n_groups * p.n_spans, X::kThreads, smem, st>>>(p, maps, error);
   return check_launch("tree_attention");
 }
-template <int kMode, int kD>
-static int launch_n(const TreeParams& p, const TreeMaps& maps, unsigned int* error, cudaStream_t st) {
-  switch (p.n_rows) {
-    case 16: return launch<kMode, kD, 16>(p, maps, error, st);
-    case 32: return launch<kMode, kD, 32>(p, maps, error, st);
-    default: return launch<kMode, kD, 64>(p, maps, error, st);
-  }
-}
 template <int kMode>
 static int launch_d(const TreeParams& p, const TreeMaps& maps, unsigned int* error, cudaStream_t st) {
-  return p.c.head_dim <= 64 ? launch_n<kMode, 64>(p, maps, error, st) : launch_n<kMode, 128>(p, maps, error, st);
+  if (p.c.head_dim <= 64)
+    return p.n_rows == 128 ? launch<kMode, 64, false>(p, maps, error, st) : launch<kMode, 64, true>(p, maps, error, st);
+  return p.n_rows == 128 ? launch<kMode, 128, false>(p, maps, error, st) : launch<kMode, 128, true>(p, maps, error, st);
 }
 
 }  // namespace tt
