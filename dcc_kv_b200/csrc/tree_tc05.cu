@@ -15,9 +15,9 @@
 //   8 warps      softmax, thread = query row (TMEM lane); they bring in the
 //                queries of a piece and write its results
 //   1 warp       TMEM owner and MMA issuer; clears bf16 value rows that do not exist
-//   1 warp       page lookups and copies: the rings of K and V tiles stay full.
-//                bf16 tiles come as TMA boxes of up to 128 rows of a page
-//                straight into the layout of the MMA, 8-bit codes and scales as
+//   2 warps      page lookups and copies, one K (and the scales), one V: the rings
+//                of tiles stay full.  bf16 tiles come as TMA boxes of up to 128
+//                rows of a page straight into the layout of the MMA, 8-bit codes as
 //                bulk copies of rows that are neighbours in the page
 //   8 warps      (8-bit) widen codes to fp16, exactly, one group K, the other V.
 //                A warp reads the codes of its 32 rows of the tile into registers
@@ -26,8 +26,8 @@
 //                scaled by a power of two that takes its largest element to 2^14:
 //                bf16 digits fit, and what falls below fp16's range is under
 //                2^-39 of that element
-// K and V have rings of their own, so that every role sees every use of the
-// barriers that it waits on; copies of K run two tiles ahead of V.
+// K and V have rings of their own, so that neither copy waits behind the other
+// and every role sees every use of the barriers that it waits on.
 // The running max of a row moves (with O and the sums rescaled) only when a
 // score passes it by 2^8.  P is rounded once for its MMA, to bf16 beside bf16
 // values (a relative 2^-9 of each weight) and to fp16 beside 8-bit ones (2^-12):
@@ -55,7 +55,6 @@ namespace tt {
 
 constexpr int kRing = 8;  // scales and masks of the last K tiles
 constexpr int kFetch = 4;   // K tiles between a page lookup and its use
-constexpr int kLead = 2;    // tiles that copies of K run ahead of V
 constexpr size_t kSmemLimit = 232448;
 
 template <int kMode, int kD, bool kPair>  // cache format, padded head_dim, two tiles of queries
@@ -71,10 +70,10 @@ struct Shape {
   static constexpr int kSlotsV = (kFit + 1) / 2 < 4 ? (kFit + 1) / 2 : 4, kSlotsK = kFit / 2 < 4 ? kFit / 2 : 4;
   static constexpr int kSlots = kSlotsK + kSlotsV;
   static_assert(kSlotsK >= 2, "rings");
-  // K tile j + kRing is copied after V tile j + kRing - kLead - 1, which waited
-  // for V tile j + kRing - kLead - 1 - kSlotsV to be consumed: that has to be
-  // tile j or a later one, so that nobody reads its scales any more
-  static_assert(kRing - kLead - 1 - kSlotsV >= 0 && kRing % 2 == 0, "ring of scales");
+  // K tile j + kRing is copied once K tile j + kRing - kSlotsK has been consumed,
+  // and those scores were issued behind the product of the tile two before: that
+  // has to be tile j or a later one, so that nobody reads its scales any more
+  static_assert(kRing - kSlotsK - 2 >= 0, "ring of scales");
   static constexpr int kWiden = k8 ? 8 : 0;
   static constexpr int kGroups = 3 + kWiden / 4;      // warpgroups
   static constexpr int kThreads = kGroups * 128;
@@ -95,7 +94,7 @@ struct Smem {
   __align__(16) float bias[2][128];
   __align__(16) float ks[2][128], vs[2][128], lift[2][128];
   __align__(16) uint8_t vis[kRing][16];               // bits: keys that exist
-  int32_t pages[kFetch][16];                          // of every eighth key of the next K tiles
+  int32_t pages[2][kFetch][16];                       // of every eighth key of the next K and V tiles
   float qf[X::kRows];                                 // what undoes the scaling of a query row
   union {
     float2 ml[2][128];                                // max and sum of a row, to add the streams up
@@ -147,8 +146,16 @@ __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
 }
 __device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 3, 256;\n" ::: "memory"); }
 __device__ __forceinline__ void group_sync(int wg) { asm volatile("bar.sync %0, 128;\n" ::"r"(1 + wg) : "memory"); }
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(dst), "l"(src) : "memory");
+template <int kBytes>
+__device__ __forceinline__ void cp_async(uint32_t dst, const void* src, uint32_t size) {  // size < kBytes: zeros follow
+  if constexpr (kBytes == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(size) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(dst), "l"(src), "r"(size) : "memory");
+}
+// Arrives (counted beforehand) once this thread's cp.async so far have landed.
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];\n" ::"r"(smem_u32(bar)) : "memory");
 }
 __device__ __forceinline__ uint4 ld_shared_v4(uint32_t a) {
   uint4 v;
@@ -230,10 +237,11 @@ __device__ __forceinline__ uint64_t desc_at(uint32_t saddr, uint32_t lbo) {
 }
 
 // ---- copies ----------------------------------------------------------------------------
-template <int kMode, int kD, bool kPair>
+template <int kMode, int kD, bool kPair, bool kIsV>
 __device__ __forceinline__ void copies(const TreeParams& p, const TreeMaps& maps, SmemOf<kMode, kD, kPair>& sm, int n, int lane,
                                        bool& ok) {
   using X = Shape<kMode, kD, kPair>;
+  constexpr int kFirst = kIsV ? X::kSlotsK : 0, kSlots = kIsV ? X::kSlotsV : X::kSlotsK;
   const TreePlan& pl = sm.span;
   const uint32_t row_bytes = (uint32_t)p.c.head_dim * (X::k8 ? 1 : 2);
   const bool pow2 = (p.c.page_size & (p.c.page_size - 1)) == 0;
@@ -241,12 +249,10 @@ __device__ __forceinline__ void copies(const TreeParams& p, const TreeMaps& maps
   // rows of a copy: 8-bit rows shorter than their 128-byte place come in eights,
   // so that a warp's rows land within its own part of the tile
   const int rows = X::k8 && p.c.head_dim != 128 ? 8 : maps.page_rows;
-  const bool lead_side = lane < 16 && ((8 * lane) & (maps.page_rows - 1)) == 0;
-  const bool lead_tile = lane < 16 && ((8 * lane) & (rows - 1)) == 0;
-  const uint32_t side_bytes = (uint32_t)maps.page_rows * 4;
-  const uint32_t side_all = side_bytes * (uint32_t)((X::k8 ? 2 : 0) + (p.c.bias ? 1 : 0));
-  const uint32_t tile_all = (uint32_t)rows * (X::k8 ? row_bytes : X::kBlocks * 128);
-  const uint32_t slot0 = smem_u32(sm.slot[0]) + (uint32_t)lane * 1024;
+  const bool leader = lane < 16 && ((8 * lane) & (rows - 1)) == 0;
+  const uint32_t bytes = (uint32_t)rows * (X::k8 ? row_bytes : X::kBlocks * 128);
+  const uint32_t slot0 = smem_u32(sm.slot[kFirst]) + (uint32_t)lane * 1024;
+  const int page_step = p.c.n_kv_heads * p.c.page_size;
   Tiles t;
   t.start(p, pl);
   // lane < 16: rows 8 lane .. 8 lane + 7 of a tile (a page holds all eight or
@@ -264,7 +270,7 @@ __device__ __forceinline__ void copies(const TreeParams& p, const TreeMaps& maps
       if (left[kFetch - 1] > 0) {
         const int s = pow2 ? pos >> shift : pos / p.c.page_size;
         add[kFetch - 1] = t.w.hk * p.c.page_size + pos - s * p.c.page_size;
-        cp_async4(smem_u32(&sm.pages[fetched % kFetch][lane]), p.q.page_table + (int64_t)t.w.b * p.q.table_stride + s);
+        cp_async<4>(smem_u32(&sm.pages[kIsV][fetched % kFetch][lane]), p.q.page_table + (int64_t)t.w.b * p.q.table_stride + s, 4);
       }
       ++fetched;
     }
@@ -282,77 +288,53 @@ __device__ __forceinline__ void copies(const TreeParams& p, const TreeMaps& maps
     shift_down();
     fetch();
   }
-  const int page_step = p.c.n_kv_heads * p.c.page_size;
-  static_assert(kLead == 2, "rows of the last K tiles");
-  int row0 = -1, row1 = -1, row2 = -1;  // of the latest K tile and the two before
-  int kj = 0, vj = 0;      // next tiles
-  Place<X::kSlotsK> at_k;
-  Place<X::kSlotsV> at_v;
+  Place<kSlots> at;
 #pragma unroll 1
-  while (vj < n) {
-    const bool is_k = kj < n && kj <= vj + kLead;
+  for (int j = 0; j < n; ++j) {
+    const int slot = kFirst + at.slot;
+    if (j >= kSlots) wait_or_skip(ok, &sm.bar_empty[slot], at.use ^ 1);
+    asm volatile("cp.async.wait_group %0;\n" ::"n"(kFetch - 1) : "memory");  // this lane's own page number
+    int row = -1;
+    if (left[0] > 0) {
+      const int page = sm.pages[kIsV][j % kFetch][lane];
+      if (page >= 0 && page < p.c.n_pages) row = page * page_step + add[0];
+    }
+    if constexpr (!kIsV) {
+      const int ring = j % kRing;
+      if (lane < 16) sm.vis[ring][lane] = row >= 0 ? (uint8_t)(left[0] >= 8 ? 0xff : (1 << left[0]) - 1) : (uint8_t)0;
+      __syncwarp();  // vis before the arrival
+      if (lane == 0) mbar_arrive(&sm.bar_side[ring]);
+      if (X::k8 || p.c.bias) {  // of four keys a lane
+        const int eight = __shfl_sync(0xffffffffu, row, lane >> 1);
+        const uint32_t to = smem_u32(&sm.side[ring][0][4 * lane]), size = eight >= 0 ? 16 : 0;
+        const int from = eight >= 0 ? eight + 4 * (lane & 1) : 0;
+        if (p.c.bias) cp_async<16>(to, p.c.bias + from, size);
+        if constexpr (X::k8) {
+          cp_async<16>(to + 512, p.c.k_scale + from, size);
+          cp_async<16>(to + 1024, p.c.v_scale + from, size);
+        }
+        cp_async_arrive(&sm.bar_side[ring]);
+      }
+    }
     // after a wait that ran out nothing new is set in flight (what was has
     // landed by then): the barriers are only passed on
-    int row, slot;
-    if (is_k) {
-      slot = at_k.slot;
-      if (kj >= X::kSlotsK) wait_or_skip(ok, &sm.bar_empty[slot], at_k.use ^ 1);
-      const int ring = kj % kRing;
-      asm volatile("cp.async.wait_group %0;\n" ::"n"(kFetch - 1) : "memory");  // this lane's own page number
-      row = -1;
-      if (left[0] > 0) {
-        const int page = sm.pages[kj % kFetch][lane];
-        if (page >= 0 && page < p.c.n_pages) row = page * page_step + add[0];
-      }
-      if (lane < 16) {
-        sm.vis[ring][lane] = row >= 0 ? (uint8_t)(left[0] >= 8 ? 0xff : (1 << left[0]) - 1) : (uint8_t)0;
-      }
-      const bool lead = ok && row >= 0 && lead_side;
-      const uint32_t count = __popc(__ballot_sync(0xffffffffu, lead));
-      __syncwarp();  // vis before the arrival
-      if (lane == 0) mbar_expect_tx(&sm.bar_side[ring], count * side_all);
-      __syncwarp();
-      if (lead) {
-        const uint32_t dst = smem_u32(&sm.side[ring][0][8 * lane]);
-        if (p.c.bias) bulk_load(dst, p.c.bias + row, side_bytes, &sm.bar_side[ring]);
-        if constexpr (X::k8) {
-          bulk_load(dst + 512, p.c.k_scale + row, side_bytes, &sm.bar_side[ring]);
-          bulk_load(dst + 1024, p.c.v_scale + row, side_bytes, &sm.bar_side[ring]);
-        }
-      }
-      row2 = row1;
-      row1 = row0;
-      row0 = row;
-    } else {
-      slot = X::kSlotsK + at_v.slot;
-      if (vj >= X::kSlotsV) wait_or_skip(ok, &sm.bar_empty[slot], at_v.use ^ 1);
-      const int back = kj - 1 - vj;
-      row = back == 0 ? row0 : back == 1 ? row1 : row2;
-    }
     uint64_t* bar = X::k8 ? &sm.bar_raw[slot] : &sm.bar_full[slot];
-    const bool lead = ok && row >= 0 && lead_tile;
+    const bool lead = ok && row >= 0 && leader;
     const uint32_t count = __popc(__ballot_sync(0xffffffffu, lead));
-    if (lane == 0) mbar_expect_tx(bar, count * tile_all);
+    if (lane == 0) mbar_expect_tx(bar, count * bytes);
     __syncwarp();
     if (lead) {
-      const uint32_t dst = slot0 + (uint32_t)slot * X::kTile;
+      const uint32_t dst = slot0 + (uint32_t)at.slot * X::kTile;
       if constexpr (X::k8) {
-        bulk_load(dst, static_cast<const unsigned char*>(is_k ? p.c.k : p.c.v) + (int64_t)row * row_bytes, tile_all, bar);
+        bulk_load(dst, static_cast<const unsigned char*>(kIsV ? p.c.v : p.c.k) + (int64_t)row * row_bytes, bytes, bar);
       } else {
-        const CUtensorMap* map = is_k ? &maps.k : &maps.v;
 #pragma unroll
-        for (int b = 0; b < X::kBlocks; ++b) tma_load_2d(dst + b * 16384, map, bar, 64 * b, row);
+        for (int b = 0; b < X::kBlocks; ++b) tma_load_2d(dst + b * 16384, kIsV ? &maps.v : &maps.k, bar, 64 * b, row);
       }
     }
-    if (is_k) {
-      shift_down();
-      fetch();
-      ++kj;
-      at_k.next();
-    } else {
-      ++vj;
-      at_v.next();
-    }
+    shift_down();
+    fetch();
+    at.next();
   }
   asm volatile("cp.async.wait_all;\n" ::: "memory");
 }
@@ -393,7 +375,10 @@ __device__ __forceinline__ void widen_tiles(const TreeParams& p, SmemOf<kMode, k
     // whatever the slot held in rows that do not exist may be a NaN in e4m3,
     // which a zero weight would not hide
     uint32_t real = 0xffffffffu;
-    if (kMode == DCC_KV_E4M3 && kIsV) real = *reinterpret_cast<const uint32_t*>(&sm.vis[j % kRing][4 * w]) >> sub;
+    if constexpr (kMode == DCC_KV_E4M3 && kIsV) {
+      wait_or_skip(ok, &sm.bar_side[j % kRing], (uint32_t)(j / kRing) & 1);
+      real = *reinterpret_cast<const uint32_t*>(&sm.vis[j % kRing][4 * w]) >> sub;
+    }
 #pragma unroll
     for (int half = 0; half < 2; ++half) {  // 16 rows at a time
       uint4 raw[2 * kTurn];
@@ -923,7 +908,7 @@ __global__ void __launch_bounds__(Shape<kMode, kD, kPair>::kThreads, 1) tree_tc0
       mbar_init(&sm.bar_empty[i], 1);
       mbar_init(&sm.bar_raw[i], 1);
     }
-    for (int i = 0; i < kRing; ++i) mbar_init(&sm.bar_side[i], 1);
+    for (int i = 0; i < kRing; ++i) mbar_init(&sm.bar_side[i], X::k8 || p.c.bias ? 33 : 1);
     mbar_init(&sm.bar_q, 256);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sm.bar_s[i], 1);
@@ -950,7 +935,8 @@ __global__ void __launch_bounds__(Shape<kMode, kD, kPair>::kThreads, 1) tree_tc0
   } else if (warp < 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(X::kRegsWork));
     if (warp == 8) issuer<kMode, kD, kPair>(p, sm, n, guard, tm, lane, ok);
-    else if (warp == 9) copies<kMode, kD, kPair>(p, maps, sm, n, lane, ok);
+    else if (warp == 9) copies<kMode, kD, kPair, false>(p, maps, sm, n, lane, ok);
+    else if (warp == 10) copies<kMode, kD, kPair, true>(p, maps, sm, n, lane, ok);
   } else if constexpr (X::k8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(X::kRegsWiden));
     if (warp < 16) widen_tiles<kMode, kD, kPair, false>(p, sm, n, warp & 3, lane, ok);
