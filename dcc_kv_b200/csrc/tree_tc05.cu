@@ -90,7 +90,8 @@ struct Smem {
   unsigned char slot[X::kSlots][X::kTile];
   unsigned char q[X::kRows / 128][X::kTile];
   __align__(16) float side[kRing][X::kArrays][128];  // bias, k_scale, v_scale
-  // of a stream's tile: bias in powers of two (-inf: hidden), K scale, V scale and its logarithm
+  // of a stream's tile: bias in powers of two (-inf: hidden), K scale, V scale, the
+  // V scale's logarithm with the bias
   __align__(16) float bias[2][128];
   __align__(16) float ks[2][128], vs[2][128], lift[2][128];
   __align__(16) uint8_t vis[kRing][16];               // bits: keys that exist
@@ -668,7 +669,7 @@ __device__ __forceinline__ void softmax(const TreeParams& p, SmemOf<kMode, kD, k
             const float vs = fmaxf(sm.side[ring][2][row], 7.888609e-31f);  // 2^-100: rows that were never written have scale 0
             sm.ks[stream][row] = sm.side[ring][1][row];
             sm.vs[stream][row] = sm.side[ring][2][row] < 7.888609e-31f ? vs : sm.side[ring][2][row];
-            sm.lift[stream][row] = __log2f(vs);
+            sm.lift[stream][row] = __log2f(vs) + bias;
           }
           group_sync(stream);
         }
@@ -696,13 +697,14 @@ __device__ __forceinline__ void softmax(const TreeParams& p, SmemOf<kMode, kD, k
           tmem_ld32(s_col + 32 * c, reinterpret_cast<uint32_t*>(d));
           tmem_wait_ld();
         };
-        // scores in powers of two
-        auto scores = [&](int c) {
+        // scores in powers of two with `add` of their keys (8-bit: always, else when
+        // keys were prepared)
+        auto scores = [&](int c, const float (&add)[128]) {
           load(c);
           if (X::k8 || prepared) {
 #pragma unroll
             for (int x = 0; x < 32; x += 4) {
-              const float4 b = *reinterpret_cast<const float4*>(&sm.bias[stream][32 * c + x]);
+              const float4 b = *reinterpret_cast<const float4*>(&add[32 * c + x]);
               float4 k = make_float4(1.f, 1.f, 1.f, 1.f);
               if constexpr (X::k8) k = *reinterpret_cast<const float4*>(&sm.ks[stream][32 * c + x]);
               d[x] = fmaf(d[x] * unit, k.x, b.x);
@@ -726,17 +728,14 @@ __device__ __forceinline__ void softmax(const TreeParams& p, SmemOf<kMode, kD, k
 #pragma unroll
             for (int x = 0; x < 32; ++x) mx[x & 3] = fmaxf(mx[x & 3], d[x]);
           } else {
-            scores(c);
-            const uint32_t see = hidden ? seen(c) : 0xffffffffu;
+            scores(c, X::k8 ? sm.lift[stream] : sm.bias[stream]);
+            if (hidden) {
+              const uint32_t see = seen(c);
 #pragma unroll
-            for (int x = 0; x < 32; x += 4) {
-              float4 up = make_float4(0.f, 0.f, 0.f, 0.f);
-              if constexpr (X::k8) up = *reinterpret_cast<const float4*>(&sm.lift[stream][32 * c + x]);
-              mx[0] = fmaxf(mx[0], (see >> x) & 1 ? d[x] + up.x : -INFINITY);
-              mx[1] = fmaxf(mx[1], (see >> (x + 1)) & 1 ? d[x + 1] + up.y : -INFINITY);
-              mx[2] = fmaxf(mx[2], (see >> (x + 2)) & 1 ? d[x + 2] + up.z : -INFINITY);
-              mx[3] = fmaxf(mx[3], (see >> (x + 3)) & 1 ? d[x + 3] + up.w : -INFINITY);
+              for (int x = 0; x < 32; ++x) d[x] = (see >> x) & 1 ? d[x] : -INFINITY;
             }
+#pragma unroll
+            for (int x = 0; x < 32; ++x) mx[x & 3] = fmaxf(mx[x & 3], d[x]);
           }
           top = fmaxf(top, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
         }
@@ -770,9 +769,23 @@ __device__ __forceinline__ void softmax(const TreeParams& p, SmemOf<kMode, kD, k
 #pragma unroll
             for (int x = 0; x < 32; ++x) d[x] = exp2_approx(fmaf(d[x], unit, -less));
           } else {
-            scores(c);
+            if (X::k8 && !p.c.bias) {
+              load(c);
 #pragma unroll
-            for (int x = 0; x < 32; ++x) d[x] = exp2_approx(d[x] - less);
+              for (int x = 0; x < 32; x += 4) {
+                const float4 k = *reinterpret_cast<const float4*>(&sm.ks[stream][32 * c + x]);
+                d[x] = fmaf(d[x] * unit, k.x, -less);
+                d[x + 1] = fmaf(d[x + 1] * unit, k.y, -less);
+                d[x + 2] = fmaf(d[x + 2] * unit, k.z, -less);
+                d[x + 3] = fmaf(d[x + 3] * unit, k.w, -less);
+              }
+            } else {
+              scores(c, sm.bias[stream]);
+#pragma unroll
+              for (int x = 0; x < 32; ++x) d[x] -= less;
+            }
+#pragma unroll
+            for (int x = 0; x < 32; ++x) d[x] = exp2_approx(d[x]);
             if (hidden) {
               see = seen(c);
 #pragma unroll
