@@ -243,15 +243,26 @@ bool tree_tensor_supported(const dcc_kv_pages& c, const dcc_tree_query& q, int d
 }
 
 // Which kernel takes a call, with how many query rows per KV head at a time.
+// Up to 16 rows the warps of tree_mma.cu, which pay per 8 rows, are ahead of
+// the tensor core tiles of tree_tc05.cu, which pay for 128 or 256 whatever the
+// number is; above they are behind (16 sequences, 8 KV heads of 128, us):
+//   rows  tokens  int8 mma / tc05   bf16 mma / tc05
+//      8    8192       89 / 192         106 / 130
+//     16    8192      117 / 193         118 / 128
+//     32    4096      125 / 121         117 / 85
+//     32     512      175 / 128         183 / 99    (64 sequences)
+// What neither takes (other types, odd strides or sizes) goes to the plain
+// kernel of this file.
 enum class Path { kSimt, kMma, kTc05 };
+constexpr int kMmaRows = 16;
 
 static Path tree_params(const dcc_kv_pages& c, const dcc_tree_query& q, int dtype, TreeParams& p) {
   p.c = c;
   p.q = q;
   p.group = q.n_q_heads / c.n_kv_heads;
   const int64_t rows = q.T * p.group;
-  const Path path = !tree_tensor_supported(c, q, dtype) ? Path::kSimt : rows <= 32 ? Path::kMma : Path::kTc05;
-  p.n_rows = path == Path::kSimt ? kSimtRows : rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 128 ? 128 : 256;
+  const Path path = !tree_tensor_supported(c, q, dtype) ? Path::kSimt : rows <= kMmaRows ? Path::kMma : Path::kTc05;
+  p.n_rows = path == Path::kSimt ? kSimtRows : rows <= 8 ? 8 : rows <= kMmaRows ? kMmaRows : rows <= 128 ? 128 : 256;
   p.n_row_tiles = (int)((rows + p.n_rows - 1) / p.n_rows);
   const int ctas = num_sms() * (path == Path::kSimt ? kSimtCtasPerSm : 1);
   const int rounds = (p.n_row_tiles + ctas - 1) / ctas;

@@ -182,7 +182,7 @@ __device__ __forceinline__ T* tree_out_row(const TreeParams& p, int b, const Tre
 }
 
 // The tensor-core kernels: bf16 queries, bf16 or 8-bit cache, head_dim a
-// multiple of 16, page_size of 8.  tree_mma.cu for up to 32 rows per KV head,
+// multiple of 16, page_size of 8.  tree_mma.cu for up to 16 rows per KV head,
 // tree_tc05.cu for more.
 bool tree_tensor_supported(const dcc_kv_pages& c, const dcc_tree_query& q, int dtype);
 int launch_tree_mma(const TreeParams& p, cudaStream_t st);

@@ -1,4 +1,4 @@
-// Tree attention over the paged cache for few query rows (up to 32 per KV
+// Tree attention over the paged cache for few query rows (up to 16 per KV
 // head): bf16 queries, bf16 / int8 / e4m3 cache, head_dim a multiple of 16.
 //
 // With few rows every key is used for so little arithmetic that HBM is the
@@ -40,7 +40,7 @@ struct Shape {
   static constexpr bool k8 = kMode != DCC_KV_BF16;
   // as many warps as the registers of a warp and the ring (64 KB and more in
   // flight) allow
-  static constexpr int kWarps = k8 ? (kNT <= 2 ? 12 : 8) : (kNT == 1 ? 12 : 8);
+  static constexpr int kWarps = k8 || kNT == 1 ? 12 : 8;
   static constexpr int kThreads = 32 * kWarps;
   static constexpr int kE = k8 ? 16 : 8;             // elements of a 16-byte chunk
   static constexpr int kKC = kD / (4 * kE);          // K chunks of a lane and key
@@ -52,7 +52,7 @@ struct Shape {
   static constexpr int kK = 16 * kRowBytes, kV = kK, kSide = 3 * 64;
   static constexpr int kStage = kK + kV + kSide;     // 16 keys of a warp
   // operands of the queries: in registers, or, where O takes those, in shared memory
-  static constexpr bool kQShared = k8 ? kNT > 1 : kNT == 4;
+  static constexpr bool kQShared = k8 && kNT > 1;
   static constexpr int kQ = kQShared ? kNT * kSteps * 256 : 16;
   static constexpr int kSum = kWarps * 2 * kD * 4;   // O of two rows of every warp
   static constexpr size_t kFixed = kSum + (size_t)kWarps * 8 * kNT * 8 + kWarps * 64 + kQ + 1024;
@@ -691,11 +691,7 @@ static int launch(const TreeParams& p, cudaStream_t st) {
 }
 template <int kMode, int kD>
 static int launch_n(const TreeParams& p, cudaStream_t st) {
-  switch (p.n_rows) {
-    case 8: return launch<kMode, kD, 1>(p, st);
-    case 16: return launch<kMode, kD, 2>(p, st);
-    default: return launch<kMode, kD, 4>(p, st);
-  }
+  return p.n_rows == 8 ? launch<kMode, kD, 1>(p, st) : launch<kMode, kD, 2>(p, st);
 }
 template <int kMode>
 static int launch_d(const TreeParams& p, cudaStream_t st) {

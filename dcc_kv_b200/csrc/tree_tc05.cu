@@ -1,4 +1,4 @@
-// Tree attention over the paged cache for more than 32 query rows per KV head,
+// Tree attention over the paged cache for more than 16 query rows per KV head,
 // on the 5th-gen tensor cores (tcgen05 + TMEM): bf16 queries, bf16 / int8 / e4m3
 // cache, head_dim a multiple of 16.
 //
