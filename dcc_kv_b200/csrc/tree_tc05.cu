@@ -186,12 +186,12 @@ __device__ __forceinline__ uint2 widen(uint32_t w) {
 }
 
 // A place of the ring and the parity of its current use.
-template <int kSlots>
 struct Place {
-  int slot = 0;
+  int slots, slot = 0;
   uint32_t use = 0;
+  __device__ __forceinline__ explicit Place(int n) : slots(n) {}
   __device__ __forceinline__ void next() {
-    if (++slot == kSlots) {
+    if (++slot == slots) {
       slot = 0;
       use ^= 1;
     }
@@ -238,11 +238,15 @@ __device__ __forceinline__ uint64_t desc_at(uint32_t saddr, uint32_t lbo) {
 }
 
 // ---- copies ----------------------------------------------------------------------------
-template <int kMode, int kD, bool kPair, bool kIsV>
-__device__ __forceinline__ void copies(const TreeParams& p, const TreeMaps& maps, SmemOf<kMode, kD, kPair>& sm, int n, int lane,
-                                       bool& ok) {
+// One code for K and V, as in the widening: all roles together just fit into the
+// instruction cache (an instance for each: 111 instead of 102 us for 16
+// sequences of 13 tokens over 4k int8 tokens; the softmax below, unrolled over all
+// 128 keys instead of 32: 185 instead of 129 us).
+template <int kMode, int kD, bool kPair>
+__device__ __forceinline__ void copies(const TreeParams& p, const TreeMaps& maps, SmemOf<kMode, kD, kPair>& sm, bool is_v, int n,
+                                       int lane, bool& ok) {
   using X = Shape<kMode, kD, kPair>;
-  constexpr int kFirst = kIsV ? X::kSlotsK : 0, kSlots = kIsV ? X::kSlotsV : X::kSlotsK;
+  const int first_slot = is_v ? X::kSlotsK : 0;
   const TreePlan& pl = sm.span;
   const uint32_t row_bytes = (uint32_t)p.c.head_dim * (X::k8 ? 1 : 2);
   const bool pow2 = (p.c.page_size & (p.c.page_size - 1)) == 0;
@@ -252,7 +256,7 @@ __device__ __forceinline__ void copies(const TreeParams& p, const TreeMaps& maps
   const int rows = X::k8 && p.c.head_dim != 128 ? 8 : maps.page_rows;
   const bool leader = lane < 16 && ((8 * lane) & (rows - 1)) == 0;
   const uint32_t bytes = (uint32_t)rows * (X::k8 ? row_bytes : X::kBlocks * 128);
-  const uint32_t slot0 = smem_u32(sm.slot[kFirst]) + (uint32_t)lane * 1024;
+  const uint32_t slot0 = smem_u32(sm.slot[first_slot]) + (uint32_t)lane * 1024;
   const int page_step = p.c.n_kv_heads * p.c.page_size;
   Tiles t;
   t.start(p, pl);
@@ -271,7 +275,7 @@ __device__ __forceinline__ void copies(const TreeParams& p, const TreeMaps& maps
       if (left[kFetch - 1] > 0) {
         const int s = pow2 ? pos >> shift : pos / p.c.page_size;
         add[kFetch - 1] = t.w.hk * p.c.page_size + pos - s * p.c.page_size;
-        cp_async<4>(smem_u32(&sm.pages[kIsV][fetched % kFetch][lane]), p.q.page_table + (int64_t)t.w.b * p.q.table_stride + s, 4);
+        cp_async<4>(smem_u32(&sm.pages[is_v][fetched % kFetch][lane]), p.q.page_table + (int64_t)t.w.b * p.q.table_stride + s, 4);
       }
       ++fetched;
     }
@@ -289,18 +293,18 @@ __device__ __forceinline__ void copies(const TreeParams& p, const TreeMaps& maps
     shift_down();
     fetch();
   }
-  Place<kSlots> at;
+  Place at(is_v ? X::kSlotsV : X::kSlotsK);
 #pragma unroll 1
   for (int j = 0; j < n; ++j) {
-    const int slot = kFirst + at.slot;
-    if (j >= kSlots) wait_or_skip(ok, &sm.bar_empty[slot], at.use ^ 1);
+    const int slot = first_slot + at.slot;
+    if (j >= at.slots) wait_or_skip(ok, &sm.bar_empty[slot], at.use ^ 1);
     asm volatile("cp.async.wait_group %0;\n" ::"n"(kFetch - 1) : "memory");  // this lane's own page number
     int row = -1;
     if (left[0] > 0) {
-      const int page = sm.pages[kIsV][j % kFetch][lane];
+      const int page = sm.pages[is_v][j % kFetch][lane];
       if (page >= 0 && page < p.c.n_pages) row = page * page_step + add[0];
     }
-    if constexpr (!kIsV) {
+    if (!is_v) {
       const int ring = j % kRing;
       if (lane < 16) sm.vis[ring][lane] = row >= 0 ? (uint8_t)(left[0] >= 8 ? 0xff : (1 << left[0]) - 1) : (uint8_t)0;
       __syncwarp();  // vis before the arrival
@@ -327,10 +331,10 @@ __device__ __forceinline__ void copies(const TreeParams& p, const TreeMaps& maps
     if (lead) {
       const uint32_t dst = slot0 + (uint32_t)at.slot * X::kTile;
       if constexpr (X::k8) {
-        bulk_load(dst, static_cast<const unsigned char*>(kIsV ? p.c.v : p.c.k) + (int64_t)row * row_bytes, bytes, bar);
+        bulk_load(dst, static_cast<const unsigned char*>(is_v ? p.c.v : p.c.k) + (int64_t)row * row_bytes, bytes, bar);
       } else {
 #pragma unroll
-        for (int b = 0; b < X::kBlocks; ++b) tma_load_2d(dst + b * 16384, kIsV ? &maps.v : &maps.k, bar, 64 * b, row);
+        for (int b = 0; b < X::kBlocks; ++b) tma_load_2d(dst + b * 16384, is_v ? &maps.v : &maps.k, bar, 64 * b, row);
       }
     }
     shift_down();
@@ -342,8 +346,9 @@ __device__ __forceinline__ void copies(const TreeParams& p, const TreeMaps& maps
 
 // ---- 8-bit: codes to values ----------------------------------------------------------------
 // Warps w = 0 .. 3 of the group for K or for V.
-template <int kMode, int kD, bool kPair, bool kIsV>
-__device__ __forceinline__ void widen_tiles(const TreeParams& p, SmemOf<kMode, kD, kPair>& sm, int n, int w, int lane, bool& ok) {
+template <int kMode, int kD, bool kPair>
+__device__ __forceinline__ void widen_tiles(const TreeParams& p, SmemOf<kMode, kD, kPair>& sm, bool is_v, int n, int w, int lane,
+                                            bool& ok) {
   using X = Shape<kMode, kD, kPair>;
   constexpr int kPerRow = kD / 16;                  // 16-byte chunks of codes in a row
   constexpr int kRowsPer = 32 / kPerRow;            // rows of one step of the warp: 4 or 8
@@ -366,26 +371,26 @@ __device__ __forceinline__ void widen_tiles(const TreeParams& p, SmemOf<kMode, k
       to[i][h] = (uint32_t)((c >> 3) * 16384 + r * 128 + (((c & 7) ^ (r & 7)) << 4));
     }
   }
-  constexpr int kFirst = kIsV ? X::kSlotsK : 0;
-  Place<kIsV ? X::kSlotsV : X::kSlotsK> at;
+  const int first_slot = is_v ? X::kSlotsK : 0;
+  Place at(is_v ? X::kSlotsV : X::kSlotsK);
 #pragma unroll 1
   for (int j = 0; j < n; ++j) {
-    const int slot = kFirst + at.slot;
+    const int slot = first_slot + at.slot;
     wait_or_skip(ok, &sm.bar_raw[slot], at.use);
     const uint32_t tile = smem_u32(sm.slot[slot]);
     // whatever the slot held in rows that do not exist may be a NaN in e4m3,
     // which a zero weight would not hide
     uint32_t real = 0xffffffffu;
-    if constexpr (kMode == DCC_KV_E4M3 && kIsV) {
+    if (kMode == DCC_KV_E4M3 && is_v) {
       wait_or_skip(ok, &sm.bar_side[j % kRing], (uint32_t)(j / kRing) & 1);
       real = *reinterpret_cast<const uint32_t*>(&sm.vis[j % kRing][4 * w]) >> sub;
     }
-#pragma unroll
+#pragma unroll 1
     for (int half = 0; half < 2; ++half) {  // 16 rows at a time
       uint4 raw[2 * kTurn];
 #pragma unroll
       for (int s = 0; s < 2 * kTurn; ++s)
-        raw[s] = chunk_real && (kMode != DCC_KV_E4M3 || !kIsV || ((real >> (8 * (s / kTurn + 2 * half) + s % kTurn * kRowsPer)) & 1))
+        raw[s] = chunk_real && (kMode != DCC_KV_E4M3 || ((real >> (8 * (s / kTurn + 2 * half) + s % kTurn * kRowsPer)) & 1))
                      ? ld_shared_v4(tile + from[s % kTurn] + (s / kTurn + 2 * half) * 1024)
                      : make_uint4(0u, 0u, 0u, 0u);
       __syncwarp();  // this warp alone reads and writes these rows
@@ -404,6 +409,13 @@ __device__ __forceinline__ void widen_tiles(const TreeParams& p, SmemOf<kMode, k
   }
 }
 
+// One lane, the same every time; with it and a warp index that is the same in all
+// lanes the operands of MMAs stay in uniform registers.
+__device__ __forceinline__ bool elected() {
+  uint32_t e;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(e));
+  return e != 0;
+}
 // ---- MMA issuer ----------------------------------------------------------------------
 // bf16 value rows that do not exist hold whatever the page or the slot held,
 // and newest values that are not finite must not reach rows that do not see
@@ -446,11 +458,10 @@ __device__ __forceinline__ void issuer(const TreeParams& p, SmemOf<kMode, kD, kP
   Tiles ts, tv;  // of the next scores, of the next values
   ts.start(p, sm.span);
   tv.start(p, sm.span);
-  Place<X::kSlotsK> at_k;
-  Place<X::kSlotsV> at_v;
+  Place at_k(X::kSlotsK), at_v(X::kSlotsV);
   uint32_t pieces = 0;
   auto scores = [&](int stream, uint64_t q, uint64_t k) {
-    if (lane == 0) {
+    if (elected()) {
 #pragma unroll
       for (int kk = 0; kk < kD / 16; ++kk)
         umma_ss(tm + X::kColS + (uint32_t)stream * 128, q + ((kk >> 2) * 16384 + (kk & 3) * 32) / 16,
@@ -470,7 +481,7 @@ __device__ __forceinline__ void issuer(const TreeParams& p, SmemOf<kMode, kD, kP
     return desc_at(k0 + (uint32_t)at_k.slot * X::kTile, 16);
   };
   auto done_k = [&]() {
-    if (lane == 0) umma_commit(&sm.bar_empty[at_k.slot]);
+    if (elected()) umma_commit(&sm.bar_empty[at_k.slot]);
     __syncwarp();
     at_k.next();
   };
@@ -491,7 +502,7 @@ __device__ __forceinline__ void issuer(const TreeParams& p, SmemOf<kMode, kD, kP
   };
   auto values = [&](int stream, uint64_t v, bool first) {
     tc_fence_after();
-    if (lane == 0) {
+    if (elected()) {
 #pragma unroll
       for (int kk = 0; kk < 8; ++kk)
         umma_ts(tm + X::kColO + (uint32_t)stream * 128, tm + X::kColS + (uint32_t)stream * 128 + kk * 8, v + kk * 128, id_o,
@@ -501,7 +512,7 @@ __device__ __forceinline__ void issuer(const TreeParams& p, SmemOf<kMode, kD, kP
     __syncwarp();
   };
   auto done_v = [&]() {
-    if (lane == 0) umma_commit(&sm.bar_empty[X::kSlotsK + at_v.slot]);
+    if (elected()) umma_commit(&sm.bar_empty[X::kSlotsK + at_v.slot]);
     __syncwarp();
     at_v.next();
   };
@@ -562,7 +573,7 @@ __device__ __forceinline__ void issuer(const TreeParams& p, SmemOf<kMode, kD, kP
     }
   }
   // every MMA has finished before TMEM is freed, also after a wait that ran out
-  if (lane == 0) umma_commit(&sm.bar_end);
+  if (elected()) umma_commit(&sm.bar_end);
   __syncwarp();
   if (!wait_all_lanes(&sm.bar_end, 0)) ok = false;
 }
@@ -628,6 +639,7 @@ __device__ __forceinline__ void softmax(const TreeParams& p, SmemOf<kMode, kD, k
       const float unit = X::k8 ? scale * sm.qf[r] : scale;
       const TreeRow own = tree_row(p, w.hk, rt, r);
       float m = -INFINITY, l = 0.f;
+      const bool busy = __any_sync(0xffffffffu, own.exists);  // else no row of the warp is anybody's
       const int count = w.k1 - w.k0;
       const int skip = kPair ? 0 : (stream - base % 2 + 2) % 2;
 #pragma unroll 1
@@ -718,105 +730,107 @@ __device__ __forceinline__ void softmax(const TreeParams& p, SmemOf<kMode, kD, k
           }
         };
         // ---- largest score (with its V scale) ----
-        float top = -INFINITY;
-        const bool bare = !X::k8 && !prepared && !hidden && unit > 0.f;  // the scores themselves, scaled last
+        if (busy) {
+          float top = -INFINITY;
+          const bool bare = !X::k8 && !prepared && !hidden && unit > 0.f;  // the scores themselves, scaled last
 #pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-          if (bare) {
-            load(c);
-#pragma unroll
-            for (int x = 0; x < 32; ++x) mx[x & 3] = fmaxf(mx[x & 3], d[x]);
-          } else {
-            scores(c, X::k8 ? sm.lift[stream] : sm.bias[stream]);
-            if (hidden) {
-              const uint32_t see = seen(c);
-#pragma unroll
-              for (int x = 0; x < 32; ++x) d[x] = (see >> x) & 1 ? d[x] : -INFINITY;
-            }
-#pragma unroll
-            for (int x = 0; x < 32; ++x) mx[x & 3] = fmaxf(mx[x & 3], d[x]);
-          }
-          top = fmaxf(top, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
-        }
-        if (bare) top *= unit;
-        const bool move = top > m + 8.f;
-        if (__any_sync(0xffffffffu, move)) {
-          const float f = move ? exp2f(m - top) : 1.f;  // 0 for the first score of a row
-          if (!first) {
-            wait_or_skip(ok, &sm.bar_o[stream], (mine - 1) & 1);
-            tc_fence_after();
-#pragma unroll 1
-            for (int c = 0; c < kD / 32; ++c) {
-              tmem_ld32(o_col + 32 * c, reinterpret_cast<uint32_t*>(d));
-              tmem_wait_ld();
-#pragma unroll
-              for (int x = 0; x < 32; ++x) d[x] *= f;
-              tmem_st32(o_col + 32 * c, reinterpret_cast<const uint32_t*>(d));
-            }
-            tmem_wait_st();
-          }
-          l *= f;
-          if (move) m = top;
-        }
-        // ---- weights, over the scores ----
-        const float less = m == -INFINITY ? 0.f : m;
-#pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          uint32_t see = 0xffffffffu;
-          if (bare) {
-            load(c);
-#pragma unroll
-            for (int x = 0; x < 32; ++x) d[x] = exp2_approx(fmaf(d[x], unit, -less));
-          } else {
-            if (X::k8 && !p.c.bias) {
+          for (int c = 0; c < 4; ++c) {
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            if (bare) {
               load(c);
 #pragma unroll
+              for (int x = 0; x < 32; ++x) mx[x & 3] = fmaxf(mx[x & 3], d[x]);
+            } else {
+              scores(c, X::k8 ? sm.lift[stream] : sm.bias[stream]);
+              if (hidden) {
+                const uint32_t see = seen(c);
+#pragma unroll
+                for (int x = 0; x < 32; ++x) d[x] = (see >> x) & 1 ? d[x] : -INFINITY;
+              }
+#pragma unroll
+              for (int x = 0; x < 32; ++x) mx[x & 3] = fmaxf(mx[x & 3], d[x]);
+            }
+            top = fmaxf(top, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+          }
+          if (bare) top *= unit;
+          const bool move = top > m + 8.f;
+          if (__any_sync(0xffffffffu, move)) {
+            const float f = move ? exp2f(m - top) : 1.f;  // 0 for the first score of a row
+            if (!first) {
+              wait_or_skip(ok, &sm.bar_o[stream], (mine - 1) & 1);
+              tc_fence_after();
+#pragma unroll 1
+              for (int c = 0; c < kD / 32; ++c) {
+                tmem_ld32(o_col + 32 * c, reinterpret_cast<uint32_t*>(d));
+                tmem_wait_ld();
+#pragma unroll
+                for (int x = 0; x < 32; ++x) d[x] *= f;
+                tmem_st32(o_col + 32 * c, reinterpret_cast<const uint32_t*>(d));
+              }
+              tmem_wait_st();
+            }
+            l *= f;
+            if (move) m = top;
+          }
+          // ---- weights, over the scores ----
+          const float less = m == -INFINITY ? 0.f : m;
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            uint32_t see = 0xffffffffu;
+            if (bare) {
+              load(c);
+#pragma unroll
+              for (int x = 0; x < 32; ++x) d[x] = exp2_approx(fmaf(d[x], unit, -less));
+            } else {
+              if (X::k8 && !p.c.bias) {
+                load(c);
+#pragma unroll
+                for (int x = 0; x < 32; x += 4) {
+                  const float4 k = *reinterpret_cast<const float4*>(&sm.ks[stream][32 * c + x]);
+                  d[x] = fmaf(d[x] * unit, k.x, -less);
+                  d[x + 1] = fmaf(d[x + 1] * unit, k.y, -less);
+                  d[x + 2] = fmaf(d[x + 2] * unit, k.z, -less);
+                  d[x + 3] = fmaf(d[x + 3] * unit, k.w, -less);
+                }
+              } else {
+                scores(c, sm.bias[stream]);
+#pragma unroll
+                for (int x = 0; x < 32; ++x) d[x] -= less;
+              }
+#pragma unroll
+              for (int x = 0; x < 32; ++x) d[x] = exp2_approx(d[x]);
+              if (hidden) {
+                see = seen(c);
+#pragma unroll
+                for (int x = 0; x < 32; ++x) d[x] = (see >> x) & 1 ? d[x] : 0.f;
+              }
+            }
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int x = 0; x < 32; ++x) sum[x & 3] += d[x];
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            uint32_t h[16];
+            if constexpr (X::k8) {
+#pragma unroll
               for (int x = 0; x < 32; x += 4) {
-                const float4 k = *reinterpret_cast<const float4*>(&sm.ks[stream][32 * c + x]);
-                d[x] = fmaf(d[x] * unit, k.x, -less);
-                d[x + 1] = fmaf(d[x + 1] * unit, k.y, -less);
-                d[x + 2] = fmaf(d[x + 2] * unit, k.z, -less);
-                d[x + 3] = fmaf(d[x + 3] * unit, k.w, -less);
+                float4 v = *reinterpret_cast<const float4*>(&sm.vs[stream][32 * c + x]);
+                if (hidden) {  // a hidden key's scale may be NaN
+                  v.x = (see >> x) & 1 ? v.x : 0.f;
+                  v.y = (see >> (x + 1)) & 1 ? v.y : 0.f;
+                  v.z = (see >> (x + 2)) & 1 ? v.z : 0.f;
+                  v.w = (see >> (x + 3)) & 1 ? v.w : 0.f;
+                }
+                h[x / 2] = pack_half(d[x] * v.x, d[x + 1] * v.y);
+                h[x / 2 + 1] = pack_half(d[x + 2] * v.z, d[x + 3] * v.w);
               }
             } else {
-              scores(c, sm.bias[stream]);
 #pragma unroll
-              for (int x = 0; x < 32; ++x) d[x] -= less;
+              for (int x = 0; x < 32; x += 2) h[x / 2] = pack2(d[x], d[x + 1]);
             }
-#pragma unroll
-            for (int x = 0; x < 32; ++x) d[x] = exp2_approx(d[x]);
-            if (hidden) {
-              see = seen(c);
-#pragma unroll
-              for (int x = 0; x < 32; ++x) d[x] = (see >> x) & 1 ? d[x] : 0.f;
-            }
+            tmem_st16(s_col + 16 * c, h);  // over scores that have been read
           }
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int x = 0; x < 32; ++x) sum[x & 3] += d[x];
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-          uint32_t h[16];
-          if constexpr (X::k8) {
-#pragma unroll
-            for (int x = 0; x < 32; x += 4) {
-              float4 v = *reinterpret_cast<const float4*>(&sm.vs[stream][32 * c + x]);
-              if (hidden) {  // a hidden key's scale may be NaN
-                v.x = (see >> x) & 1 ? v.x : 0.f;
-                v.y = (see >> (x + 1)) & 1 ? v.y : 0.f;
-                v.z = (see >> (x + 2)) & 1 ? v.z : 0.f;
-                v.w = (see >> (x + 3)) & 1 ? v.w : 0.f;
-              }
-              h[x / 2] = pack_half(d[x] * v.x, d[x + 1] * v.y);
-              h[x / 2 + 1] = pack_half(d[x + 2] * v.z, d[x + 3] * v.w);
-            }
-          } else {
-#pragma unroll
-            for (int x = 0; x < 32; x += 2) h[x / 2] = pack2(d[x], d[x + 1]);
-          }
-          tmem_st16(s_col + 16 * c, h);  // over scores that have been read
+          tmem_wait_st();
         }
-        tmem_wait_st();
         tc_fence_before();
         mbar_arrive(&sm.bar_p[stream]);
       }
@@ -914,7 +928,8 @@ __global__ void __launch_bounds__(Shape<kMode, kD, kPair>::kThreads, 1) tree_tc0
   const int rounds = (p.n_row_tiles - (int)(blockIdx.x % p.n_groups) + p.n_groups - 1) / p.n_groups;
   const int n = (int)(sm.span.end - sm.span.begin) * rounds;
   if (n == 0) return;  // the whole CTA
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);  // uniform, also to the compiler
+  const int lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < X::kSlots; ++i) {
       mbar_init(&sm.bar_full[i], X::k8 ? 4 : 1);
@@ -948,12 +963,10 @@ __global__ void __launch_bounds__(Shape<kMode, kD, kPair>::kThreads, 1) tree_tc0
   } else if (warp < 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(X::kRegsWork));
     if (warp == 8) issuer<kMode, kD, kPair>(p, sm, n, guard, tm, lane, ok);
-    else if (warp == 9) copies<kMode, kD, kPair, false>(p, maps, sm, n, lane, ok);
-    else if (warp == 10) copies<kMode, kD, kPair, true>(p, maps, sm, n, lane, ok);
+    else if (warp <= 10) copies<kMode, kD, kPair>(p, maps, sm, warp == 10, n, lane, ok);
   } else if constexpr (X::k8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(X::kRegsWiden));
-    if (warp < 16) widen_tiles<kMode, kD, kPair, false>(p, sm, n, warp & 3, lane, ok);
-    else widen_tiles<kMode, kD, kPair, true>(p, sm, n, warp & 3, lane, ok);
+    widen_tiles<kMode, kD, kPair>(p, sm, warp >= 16, n, warp & 3, lane, ok);
   }
   if (!ok && lane == 0) atomicOr(error, 32u);
   tc_fence_before();
