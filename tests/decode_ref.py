@@ -91,6 +91,16 @@ def tree(q, cache, page_table, ctx, counts=None, mask=None, scale=None, seen_pos
             vz = torch.where(sees.any(0)[:, None], vv, torch.zeros_like(vv))
             o[b, h, :n] = p @ vz
             a[b, h, :n] = p @ vz.abs()
+            if cache.v_scale is not None and q.dtype == torch.bfloat16:
+                # p times the V scale is held in fp16, in units of at most the row's
+                # largest such product: below 2^-14 of the unit half a step is 2^-25 of
+                # it whatever p is, and a key adds that times its code.  (2^-17 here:
+                # the tolerance takes 2^-8 of a.)
+                ids = page_table[b].long()
+                pos = torch.arange(c + n, device=dev)
+                s = cache.v_scale.double()[ids[pos // cache.page_size], h // g, pos % cache.page_size]
+                code = torch.where(s > 0, vz.abs().T / torch.where(s > 0, s, torch.ones_like(s)), torch.zeros_like(s))
+                a[b, h, :n] += 2.0 ** -17 * (p * torch.nan_to_num(s)).amax(1, keepdim=True) * torch.nan_to_num(code).sum(1)
             lse[b, h, :n] = torch.where(some, top[:, 0] + torch.log(l[:, 0]), torch.full_like(l[:, 0], -math.inf))
             ex[b, h, :n] = (qq.abs() @ kk.abs().T * abs(scale)).masked_fill(~sees, 0.).amax(1)
     return o, lse, a, ex
