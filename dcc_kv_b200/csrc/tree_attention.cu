@@ -14,8 +14,10 @@ constexpr int kSimtCtasPerSm = 6;
 // Online softmax over key tiles of 128: thread = key for the scores (q rows
 // from shared memory), thread = column for the values.  fp32 throughout.
 // Bound by instruction issue (2 fused multiply-adds per row, key and column);
-// it serves fp32 queries and caches and the head_dims that the tensor-core
-// kernel does not take.
+// it serves fp32 queries and caches and the head_dims and page sizes that the
+// tensor-core kernels do not take.  16 sequences, 4 heads on each of 8 KV heads
+// of 128, 8k tokens: SIMT_BF16 us beside a bf16 cache whose pages hold 12 tokens,
+// where 16-token pages take tree_mma.cu 104 us.
 template <typename T, int kFormat>
 __global__ void __launch_bounds__(kSimtThreads) tree_simt_kernel(const __grid_constant__ TreeParams p) {
   constexpr bool kScaled = kFormat == DCC_KV_INT8 || kFormat == DCC_KV_E4M3;
@@ -230,7 +232,8 @@ __global__ void __launch_bounds__(kMergeWarps * 32) tree_merge_kernel(const __gr
 
 bool tree_tensor_supported(const dcc_kv_pages& c, const dcc_tree_query& q, int dtype) {
   // rows of 16-byte chunks, eight rows that never leave their page
-  if (dtype != DCC_BF16 || c.format == DCC_KV_F32 || c.head_dim % 16 != 0 || c.page_size % 8 != 0) return false;
+  // (a pool without pages is nothing to make a tensor map of)
+  if (dtype != DCC_BF16 || c.format == DCC_KV_F32 || c.head_dim % 16 != 0 || c.page_size % 8 != 0 || c.n_pages == 0) return false;
   auto aligned = [](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15u) == 0; };
   for (const void* x : {(const void*)c.k, (const void*)c.v, (const void*)c.k_scale, (const void*)c.v_scale,
                         (const void*)c.bias, (const void*)q.q})

@@ -88,3 +88,28 @@ def test_rows_that_were_never_written_are_zeros(fmt, t):
     cache.write(k, v, table, lens(100))
     q = randn(g, 1, 8, t, 128, dtype=torch.bfloat16)
     check(q, cache, table, lens(500), 500 + t)
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "int8", "e4m3"])
+@pytest.mark.parametrize("t", [1, 4, 9, 40])
+@pytest.mark.parametrize("d", [16, 32, 48, 80, 112])
+def test_head_dims(fmt, t, d):
+    g = gen(d)
+    cache, table = filled(g, fmt, 2, 2, d, 16, 300 + t, False)
+    q = randn(g, 2, 8, t, d, dtype=torch.bfloat16)
+    check(q, cache, table, lens(300, 65), 300 + t)
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "int8"])
+@pytest.mark.parametrize("t", [1, 40])
+def test_pool_or_table_without_pages(fmt, t):
+    for pages, width in ((0, 3), (4, 0), (0, 0)):
+        cache = dk.KvCache.empty(pages, 16, 2, 64, fmt, device="cuda")
+        table = torch.zeros(2, width, dtype=torch.int32, device="cuda")
+        o, lse = dk.tree_attention(torch.ones(2, 4, t, 64, dtype=torch.bfloat16, device="cuda"), cache, table, lens(20, 0))
+        assert (o == 0).all() and (lse == -float("inf")).all()
+        cache.write(torch.ones(2, 2, t, 64, device="cuda"), torch.ones(2, 2, t, 64, device="cuda"), table, 0)
+        k, v = cache.read(table, 0, t)
+        assert (k == 0).all() == (v == 0).all()
+        if width == 0 or pages == 0:
+            assert (k == 0).all()
