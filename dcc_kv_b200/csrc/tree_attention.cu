@@ -16,8 +16,8 @@ constexpr int kSimtCtasPerSm = 6;
 // Bound by instruction issue (2 fused multiply-adds per row, key and column);
 // it serves fp32 queries and caches and the head_dims and page sizes that the
 // tensor-core kernels do not take.  16 sequences, 4 heads on each of 8 KV heads
-// of 128, 8k tokens: SIMT_BF16 us beside a bf16 cache whose pages hold 12 tokens,
-// where 16-token pages take tree_mma.cu 104 us.
+// of 128, 8k tokens: 1161 us beside a bf16 cache whose pages hold 12 tokens,
+// where 16-token pages take tree_mma.cu 105 us.
 template <typename T, int kFormat>
 __global__ void __launch_bounds__(kSimtThreads) tree_simt_kernel(const __grid_constant__ TreeParams p) {
   constexpr bool kScaled = kFormat == DCC_KV_INT8 || kFormat == DCC_KV_E4M3;
@@ -250,10 +250,10 @@ bool tree_tensor_supported(const dcc_kv_pages& c, const dcc_tree_query& q, int d
 // the tensor core tiles of tree_tc05.cu, which pay for 128 or 256 whatever the
 // number is; above they are behind (16 sequences, 8 KV heads of 128, us):
 //   rows  tokens  int8 mma / tc05   bf16 mma / tc05
-//      8    8192       89 / 192         106 / 130
-//     16    8192      117 / 193         118 / 128
-//     32    4096      125 / 121         117 / 85
-//     32     512      175 / 128         183 / 99    (64 sequences)
+//      8    8192       87 / 159         107 / 115
+//     16    8192      117 / 160         117 / 114
+//     32    4096      125 / 98          117 / 74
+//     32     512      175 / 98          183 / 90    (64 sequences)
 // What neither takes (other types, odd strides or sizes) goes to the plain
 // kernel of this file.
 enum class Path { kSimt, kMma, kTc05 };

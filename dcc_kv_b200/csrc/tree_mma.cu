@@ -24,7 +24,13 @@
 // sums and O in registers; the warps are added up at the end of a piece.  P is
 // rounded once, to bf16 beside bf16 values (a relative 2^-9 of each weight), to
 // fp16 beside codes (2^-12): there P carries the V scale, so the max is taken
-// over score + log2(scale), which keeps P below 2^8 whatever the scales are.
+// over score + log2(scale), which keeps P below 2^8 whatever the scales are
+// (below 2^-14 of that maximum fp16 is subnormal and holds P to 2^-25 of it).
+// Measured: 16 sequences of 8192 tokens, 4 query heads on each of 8 KV heads of
+// 128: int8 81 us or 3.4 TB/s, e4m3 88 us, bf16 105 us or 5.1 TB/s; with 16 rows
+// per KV head 117 us in both.  8-bit codes are bound by the issue of their
+// widening, 560 to 600 instructions a warp and 16 keys; lines of 512 bytes a copy
+// instead of one row a lane took a quarter off.
 #include <string>
 #include <type_traits>
 

@@ -32,9 +32,14 @@
 // score passes it by 2^8.  P is rounded once for its MMA, to bf16 beside bf16
 // values (a relative 2^-9 of each weight) and to fp16 beside 8-bit ones (2^-12):
 // there P carries the V scale, so the max is taken over score + log2(scale),
-// which keeps P below 2^8 whatever the scales are.
+// which keeps P below 2^8 whatever the scales are (below 2^-14 of that maximum
+// fp16 is subnormal and holds P to 2^-25 of it).
 //
-// Bound: tensor cores and the issue of the softmax beside them.
+// Measured (8 KV heads of 128, 4 query heads each): 64 tokens over 131072, bf16,
+// 200 us or 690 TFLOP/s; int8, 292 us; 13 tokens of 16 sequences over 4001, int8,
+// 100 us; bf16 77 us.  Neither memory nor tensor cores are full: what bounds it
+// is the chain scores -> weights -> values -> next scores of a stream (its scores
+// and weights share TMEM) and the instruction cache, which all roles share.
 //
 // Waits are bounded (2 s).  After one has run out a role sets the error word
 // and walks through the rest of its loop without waiting, so named barriers
