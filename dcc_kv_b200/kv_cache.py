@@ -7,7 +7,7 @@ again for every new token by :func:`~dcc_kv_b200.tree_attention`.
 """
 from __future__ import annotations
 
-from dataclasses import dataclass, field
+from dataclasses import dataclass
 from typing import Optional, Tuple, Union
 
 import torch
@@ -35,7 +35,6 @@ class KvCache:
     k_scale: Optional[torch.Tensor] = None
     v_scale: Optional[torch.Tensor] = None
     logit_bias: Optional[torch.Tensor] = None
-    _pages: L.dcc_kv_pages = field(init=False, repr=False, compare=False)
 
     def __post_init__(self):
         k = self.k
@@ -56,9 +55,13 @@ class KvCache:
         for t in (k, self.v, self.k_scale, self.v_scale, self.logit_bias):
             if t is not None and (t.device != k.device or not t.is_contiguous()):
                 raise ValueError("the tensors of a cache must be contiguous and on one device")
-        object.__setattr__(self, "_pages", L.dcc_kv_pages(
+
+    @property
+    def _pages(self) -> L.dcc_kv_pages:
+        k = self.k
+        return L.dcc_kv_pages(
             k.data_ptr(), self.v.data_ptr(), L.ptr(self.k_scale), L.ptr(self.v_scale), L.ptr(self.logit_bias),
-            k.shape[0], k.shape[2], k.shape[1], k.shape[3], _FORMATS[k.dtype]))
+            k.shape[0], k.shape[2], k.shape[1], k.shape[3], _FORMATS[k.dtype])
 
     @classmethod
     def empty(cls, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, fmt: str = "int8",

@@ -75,8 +75,8 @@ def tree_attention(q: torch.Tensor, cache: KvCache, page_table: torch.Tensor, co
         query = L.dcc_tree_query(q.data_ptr(), o.data_ptr(), lse.data_ptr(), *q.stride()[:3], *o.stride()[:3],
                                  context_lens.data_ptr(), L.ptr(counts), tree_ptr, tree_stride,
                                  page_table.data_ptr(), page_table.stride(0), t, b, hq, page_table.shape[1], 0)
-        lib = L.lib()
-        ws = L.workspace(lib.dcc_tree_attention_workspace_bytes(cache._pages, query, code), dev)
-        L.check(lib.dcc_tree_attention(cache._pages, query, 1.0 / math.sqrt(d) if scale is None else scale, code,
+        lib, pages = L.lib(), cache._pages
+        ws = L.workspace(lib.dcc_tree_attention_workspace_bytes(pages, query, code), dev)
+        L.check(lib.dcc_tree_attention(pages, query, 1.0 / math.sqrt(d) if scale is None else scale, code,
                                        ws.data_ptr(), ws.numel(), L.stream_ptr(dev)), "tree_attention")
     return o, lse

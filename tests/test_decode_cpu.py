@@ -2,6 +2,7 @@
 refuse before anything is launched."""
 from __future__ import annotations
 
+import copy
 import ctypes as C
 import math
 
@@ -190,3 +191,10 @@ def test_c_entries_refuse_before_a_device_is_touched():
     empty.T = 0
     assert tree(q=empty, ws=None, n=0) == L.DCC_OK
     assert math.isfinite(need)
+
+
+def test_a_copied_cache_points_at_its_own_tensors():
+    cache = dk.KvCache.empty(2, 8, 1, 16, device="cpu")
+    other = copy.deepcopy(cache)
+    assert other.k.data_ptr() != cache.k.data_ptr()
+    assert other._pages.k == other.k.data_ptr() and other._pages.v_scale == other.v_scale.data_ptr()
