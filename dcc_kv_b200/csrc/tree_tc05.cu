@@ -70,7 +70,7 @@ struct Shape {
   static constexpr int kBlocks = kD / 64;             // 64-column blocks of 128 swizzled rows
   static constexpr uint32_t kColS = 0, kColO = 256;   // TMEM columns, 128 a stream
   static constexpr int kArrays = k8 ? 3 : 1;          // bias; K and V scales
-  static constexpr size_t kFixed = (size_t)kRows * kD * 2 + (size_t)kRing * kArrays * 512 + 2 * 4 * 512 + 3072 + kRows * 4;
+  static constexpr size_t kFixed = (size_t)kRows * kD * 2 + (size_t)kRing * kArrays * 512 + 2 * 4 * 512 + 3 * 1024 + kRows * 4;
   static constexpr int kFit = (int)((kSmemLimit - kFixed) / kTile);
   static constexpr int kSlotsV = (kFit + 1) / 2 < 4 ? (kFit + 1) / 2 : 4, kSlotsK = kFit / 2 < 4 ? kFit / 2 : 4;
   static constexpr int kSlots = kSlotsK + kSlotsV;
