@@ -27,8 +27,8 @@
 // over score + log2(scale), which keeps P below 2^8 whatever the scales are
 // (below 2^-14 of that maximum fp16 is subnormal and holds P to 2^-25 of it).
 // Measured: 16 sequences of 8192 tokens, 4 query heads on each of 8 KV heads of
-// 128: int8 81 us or 3.4 TB/s, e4m3 88 us, bf16 105 us or 5.1 TB/s; with 16 rows
-// per KV head 117 us in both.  8-bit codes are bound by the issue of their
+// 128: int8 75 us or 3.7 TB/s, e4m3 85 us, bf16 105 us or 5.1 TB/s; with 16 rows
+// per KV head 112 and 116 us.  8-bit codes are bound by the issue of their
 // widening, 560 to 600 instructions a warp and 16 keys; lines of 512 bytes a copy
 // instead of one row a lane took a quarter off.
 #include <string>
@@ -209,7 +209,8 @@ __global__ void __launch_bounds__(Shape<kMode, kD, kNT>::kThreads, 1) tree_mma_k
   const int rounds = (p.n_row_tiles - (int)(blockIdx.x % p.n_groups) + p.n_groups - 1) / p.n_groups;
   const int n = (int)(pl.end - pl.begin) * rounds;
   if (n == 0) return;  // the whole CTA
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);  // uniform, also to the compiler: 75 instead of 81 us
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int chunks = 8 * n;
   const int d = p.c.head_dim;
   const uint32_t row_bytes = (uint32_t)d * (k8 ? 1 : 2);
