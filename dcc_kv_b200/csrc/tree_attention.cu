@@ -250,8 +250,8 @@ bool tree_tensor_supported(const dcc_kv_pages& c, const dcc_tree_query& q, int d
 // the tensor core tiles of tree_tc05.cu, which pay for 128 or 256 whatever the
 // number is; above they are behind (16 sequences, 8 KV heads of 128, us):
 //   rows  tokens  int8 mma / tc05   bf16 mma / tc05
-//      8    8192       87 / 159         107 / 115
-//     16    8192      117 / 160         117 / 114
+//      8    8192       82 / 159         107 / 115
+//     16    8192      112 / 160         116 / 114
 //     32    4096      125 / 98          117 / 74
 //     32     512      175 / 98          183 / 90    (64 sequences)
 // What neither takes (other types, odd strides or sizes) goes to the plain

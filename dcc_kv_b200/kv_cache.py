@@ -58,10 +58,21 @@ class KvCache:
 
     @property
     def _pages(self) -> L.dcc_kv_pages:
-        k = self.k
-        return L.dcc_kv_pages(
-            k.data_ptr(), self.v.data_ptr(), L.ptr(self.k_scale), L.ptr(self.v_scale), L.ptr(self.logit_bias),
-            k.shape[0], k.shape[2], k.shape[1], k.shape[3], _FORMATS[k.dtype])
+        """The C struct: its sizes are made once, its pointers are those of now."""
+        k, p = self.k, self.__dict__.get("_struct")
+        if p is None:
+            p = L.dcc_kv_pages(None, None, None, None, None, k.shape[0], k.shape[2], k.shape[1], k.shape[3],
+                               _FORMATS[k.dtype])
+            object.__setattr__(self, "_struct", p)
+        p.k, p.v = k.data_ptr(), self.v.data_ptr()
+        if self.k_scale is not None:
+            p.k_scale, p.v_scale = self.k_scale.data_ptr(), self.v_scale.data_ptr()
+        if self.logit_bias is not None:
+            p.bias = self.logit_bias.data_ptr()
+        return p
+
+    def __getstate__(self):
+        return {name: x for name, x in self.__dict__.items() if name != "_struct"}
 
     @classmethod
     def empty(cls, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, fmt: str = "int8",
