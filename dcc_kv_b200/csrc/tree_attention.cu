@@ -256,9 +256,11 @@ bool tree_tensor_supported(const dcc_kv_pages& c, const dcc_tree_query& q, int d
 //     32     512      175 / 98          183 / 90    (64 sequences)
 // Within them 8 rows at a time where that is all (one token of 16 sequences over
 // 8192, int8: 75 us, in 16 rows 92); one tile of 128 rows up to 128 (52 rows, 16
-// sequences of 4001 int8 tokens: 104 us, as a pair 138), else pairs of them that
-// share each key tile (256 rows over 131072 tokens: int8 290 us, one by one 320;
-// bf16 200 us, one by one 192).
+// sequences of 4001 int8 tokens: 104 us, as a pair 138); beyond, beside 8-bit
+// codes, pairs of them that share each key tile and its widening (256 rows over
+// 131072 tokens, int8: 290 us, one by one 320).  bf16 tiles, with nothing to widen,
+// come to CTAs side by side from the L2 as well (256 rows over 131072 tokens 193 us,
+// as pairs 200; over 8 sequences of 8192 126, 138; over 64 of 512 208, 199).
 // What neither takes (other types, odd strides or sizes) goes to the plain
 // kernel of this file.
 enum class Path { kSimt, kMma, kTc05 };
@@ -270,7 +272,8 @@ static Path tree_params(const dcc_kv_pages& c, const dcc_tree_query& q, int dtyp
   p.group = q.n_q_heads / c.n_kv_heads;
   const int64_t rows = q.T * p.group;
   const Path path = !tree_tensor_supported(c, q, dtype) ? Path::kSimt : rows <= kMmaRows ? Path::kMma : Path::kTc05;
-  p.n_rows = path == Path::kSimt ? kSimtRows : rows <= 8 ? 8 : rows <= kMmaRows ? kMmaRows : rows <= 128 ? 128 : 256;
+  p.n_rows = path == Path::kSimt ? kSimtRows : rows <= 8 ? 8 : rows <= kMmaRows ? kMmaRows
+             : rows <= 128 || c.format == DCC_KV_BF16 ? 128 : 256;
   p.n_row_tiles = (int)((rows + p.n_rows - 1) / p.n_rows);
   const int ctas = num_sms() * (path == Path::kSimt ? kSimtCtasPerSm : 1);
   const int rounds = (p.n_row_tiles + ctas - 1) / ctas;

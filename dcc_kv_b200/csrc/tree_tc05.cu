@@ -7,10 +7,10 @@
 // A CTA walks over its span of key tiles (tree_attention.cuh) with two streams,
 // each with its own S / P, O, running max and sums, so that the softmax of one
 // runs beside the MMAs of the other:
-//   up to 128 rows  one tile of queries; stream = key tile mod 2, added up at the
-//                   end of a piece
-//   more            two tiles of queries (256 rows), one a stream; every key tile
-//                   is loaded (and widened) once for both
+//   one tile of queries (128 rows)   stream = key tile mod 2, added up at the end
+//                                    of a piece
+//   two tiles (256 rows, beside 8-bit codes only)   one a stream; every key tile is
+//                                    loaded and widened once for both
 // Roles, one warp or group of warps each:
 //   8 warps      softmax, thread = query row (TMEM lane); they bring in the
 //                queries of a piece and write its results
@@ -36,7 +36,7 @@
 // fp16 is subnormal and holds P to 2^-25 of it).
 //
 // Measured (8 KV heads of 128, 4 query heads each): 64 tokens over 131072, bf16,
-// 200 us or 690 TFLOP/s; int8, 292 us; 13 tokens of 16 sequences over 4001, int8,
+// 193 us or 710 TFLOP/s; int8, 290 us; 13 tokens of 16 sequences over 4001, int8,
 // 100 us; bf16 77 us.  Neither memory nor tensor cores are full: what bounds it
 // is the chain scores -> weights -> values -> next scores of a stream (its scores
 // and weights share TMEM) and the instruction cache, which all roles share.
@@ -995,11 +995,15 @@ static int launch(const TreeParams& p, const TreeMaps& maps, unsigned int* error
   kernel<<<p.n_groups * p.n_spans, X::kThreads, smem, st>>>(p, maps, error);
   return check_launch("tree_attention");
 }
+template <int kMode, int kD>
+static int launch_rows(const TreeParams& p, const TreeMaps& maps, unsigned int* error, cudaStream_t st) {
+  if constexpr (kMode != DCC_KV_BF16)
+    if (p.n_rows == 256) return launch<kMode, kD, true>(p, maps, error, st);
+  return launch<kMode, kD, false>(p, maps, error, st);
+}
 template <int kMode>
 static int launch_d(const TreeParams& p, const TreeMaps& maps, unsigned int* error, cudaStream_t st) {
-  if (p.c.head_dim <= 64)
-    return p.n_rows == 128 ? launch<kMode, 64, false>(p, maps, error, st) : launch<kMode, 64, true>(p, maps, error, st);
-  return p.n_rows == 128 ? launch<kMode, 128, false>(p, maps, error, st) : launch<kMode, 128, true>(p, maps, error, st);
+  return p.c.head_dim <= 64 ? launch_rows<kMode, 64>(p, maps, error, st) : launch_rows<kMode, 128>(p, maps, error, st);
 }
 
 }  // namespace tt
