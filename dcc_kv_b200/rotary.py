@@ -21,38 +21,72 @@ from . import _lib as L
 _LAYOUTS = {"half": L.DCC_ROTARY_HALF, "interleaved": L.DCC_ROTARY_INTERLEAVED}
 
 
+# what each kind of scaling reads; the first ones may stand beside any of them
+_KEYS = {"": ("rope_type", "type", "rope_theta", "partial_rotary_factor", "original_max_position_embeddings"),
+         "default": (), "linear": ("factor",), "ntk": ("factor",),
+         "yarn": ("factor", "beta_fast", "beta_slow", "truncate", "attention_factor", "mscale", "mscale_all_dim"),
+         "llama3": ("factor", "low_freq_factor", "high_freq_factor")}
+
+
 def _need(scaling: Mapping, key: str) -> float:
-    if key not in scaling:
-        raise ValueError(f"rotary scaling {scaling.get('rope_type')!r} needs {key!r}")
+    if scaling.get(key) is None:
+        raise ValueError(f"rotary scaling {_kind(scaling)!r} needs {key!r}")
     value = float(scaling[key])
     if not value > 0:
         raise ValueError(f"rotary scaling: {key} must be positive, got {scaling[key]}")
     return value
 
 
-def rotary_frequencies(rotary_dim: int, theta: float = 10000.0,
+def _kind(scaling: Mapping) -> str:
+    kind = scaling.get("rope_type", scaling.get("type")) or "default"
+    if kind not in _KEYS or kind == "":
+        raise ValueError(f"unknown rotary scaling {kind!r}; use linear, ntk, yarn or llama3")
+    return kind
+
+
+def _theta(theta: Optional[float], scaling: Optional[Mapping]) -> float:
+    """``theta``, or the one that stands in ``scaling``, or 10000."""
+    own = None if scaling is None else scaling.get("rope_theta")
+    if theta is not None and own is not None and float(own) != float(theta):
+        raise ValueError(f"rotary scaling holds rope_theta {own}, theta is {theta}")
+    theta = float(theta if theta is not None else own if own is not None else 10000.0)
+    if not theta > 1:
+        raise ValueError(f"theta must exceed 1, got {theta}")
+    return theta
+
+
+def rotary_frequencies(rotary_dim: int, theta: Optional[float] = None,
                        scaling: Optional[Mapping] = None) -> Tuple[list, float]:
     """Radians per position of each of the ``rotary_dim // 2`` pairs, and the
     magnitude that multiplies the rotated part.  f_i = theta^(-2i / rotary_dim),
     changed for long contexts by ``scaling`` (keys as in a transformers
-    ``rope_scaling``):
+    ``rope_scaling``; a key that its kind does not read is refused):
 
     * ``linear``: f / factor (positions interpolated);
     * ``ntk``: the base grows to theta * factor^(r / (r - 2)), which slows the
       slowest pair by the factor and leaves the fastest;
     * ``yarn``: pairs that turn more than ``beta_fast`` (32) times over
       ``original_max_position_embeddings`` keep f, those under ``beta_slow`` (1)
-      get f / factor, a linear ramp over the pair index between; magnitude
-      ``attention_factor`` or 0.1 ln(factor) + 1;
+      get f / factor, a linear ramp over the pair index between (from and to
+      whole indices unless ``truncate`` is false); magnitude
+      ``attention_factor``, else with a(m) = 0.1 m ln(factor) + 1 (1 for a
+      factor up to 1) a(``mscale``) / a(``mscale_all_dim``) where both are
+      given and not 0, else a(1);
     * ``llama3``: pairs with more than ``high_freq_factor`` turns keep f, those
       under ``low_freq_factor`` get f / factor, a linear ramp over the turns
-      between."""
+      between.
+
+    Without ``theta`` the ``rope_theta`` of ``scaling`` holds, else 10000."""
     r = rotary_dim
+    theta = _theta(theta, scaling)
     f = [theta ** (-2.0 * i / r) for i in range(r // 2)]
     if scaling is None:
         return f, 1.0
-    kind = scaling.get("rope_type", scaling.get("type"))
-    if kind in (None, "default"):
+    kind = _kind(scaling)
+    unknown = [k for k, x in scaling.items() if x is not None and k not in _KEYS[""] and k not in _KEYS[kind]]
+    if unknown:
+        raise ValueError(f"rotary scaling {kind!r} does not read {', '.join(map(repr, unknown))}")
+    if kind == "default":
         return f, 1.0
     if kind == "linear":
         factor = _need(scaling, "factor")
@@ -70,43 +104,56 @@ def rotary_frequencies(rotary_dim: int, theta: float = 10000.0,
         def pair_with(turns: float) -> float:
             return r * math.log(n / (2.0 * math.pi * turns)) / (2.0 * math.log(theta))
 
-        low, high = max(math.floor(pair_with(fast)), 0), min(math.ceil(pair_with(slow)), r - 1)
+        def growth(m: float) -> float:
+            return 0.1 * m * math.log(factor) + 1.0 if factor > 1 else 1.0
+
+        low, high = pair_with(fast), pair_with(slow)
+        if scaling.get("truncate") is None or scaling["truncate"]:
+            low, high = math.floor(low), math.ceil(high)
+        low, high = max(low, 0), min(high, r - 1)
         width = max(high - low, 1e-3)
         slowed = [min(max((i - low) / width, 0.0), 1.0) for i in range(r // 2)]
-        magnitude = scaling.get("attention_factor")
-        magnitude = 0.1 * math.log(factor) + 1.0 if magnitude is None and factor > 1 else float(magnitude or 1.0)
+        if scaling.get("attention_factor") is not None:
+            magnitude = _need(scaling, "attention_factor")
+        elif scaling.get("mscale") and scaling.get("mscale_all_dim"):
+            magnitude = growth(float(scaling["mscale"])) / growth(float(scaling["mscale_all_dim"]))
+        else:
+            magnitude = growth(1.0)
         return [x / factor * s + x * (1.0 - s) for x, s in zip(f, slowed)], magnitude
-    if kind == "llama3":
-        factor, n = _need(scaling, "factor"), _need(scaling, "original_max_position_embeddings")
-        low, high = _need(scaling, "low_freq_factor"), _need(scaling, "high_freq_factor")
-        if not high > low:
-            raise ValueError("rotary scaling 'llama3': high_freq_factor must exceed low_freq_factor")
-        out = []
-        for x in f:
-            kept = min(max((n * x / (2.0 * math.pi) - low) / (high - low), 0.0), 1.0)
-            out.append(x / factor * (1.0 - kept) + x * kept)
-        return out, 1.0
-    raise ValueError(f"unknown rotary scaling {kind!r}; use linear, ntk, yarn or llama3")
+    factor, n = _need(scaling, "factor"), _need(scaling, "original_max_position_embeddings")
+    low, high = _need(scaling, "low_freq_factor"), _need(scaling, "high_freq_factor")
+    if not high > low:
+        raise ValueError("rotary scaling 'llama3': high_freq_factor must exceed low_freq_factor")
+    out = []
+    for x in f:
+        kept = min(max((n * x / (2.0 * math.pi) - low) / (high - low), 0.0), 1.0)
+        out.append(x / factor * (1.0 - kept) + x * kept)
+    return out, 1.0
 
 
 class Rotary:
     """Rotary positions of one kind of head: pairs (i, i + r/2) of the first
     r = ``rotary_dim`` elements (``layout="half"``) or (2i, 2i + 1)
     (``"interleaved"``); the rest of the head is passed through.  See
-    :func:`rotary_frequencies` for ``theta`` and ``scaling``."""
+    :func:`rotary_frequencies` for ``theta`` and ``scaling``; a
+    ``partial_rotary_factor`` of the latter is r / ``head_dim``."""
 
-    def __init__(self, head_dim: int, rotary_dim: Optional[int] = None, theta: float = 10000.0,
+    def __init__(self, head_dim: int, rotary_dim: Optional[int] = None, theta: Optional[float] = None,
                  layout: str = "half", scaling: Optional[Mapping] = None):
-        r = head_dim if rotary_dim is None else rotary_dim
+        part = None if scaling is None else scaling.get("partial_rotary_factor")
+        if part is not None:
+            part = int(head_dim * part)
+            if rotary_dim not in (None, part):
+                raise ValueError(f"rotary scaling holds partial_rotary_factor {scaling['partial_rotary_factor']}, "
+                                 f"rotary_dim is {rotary_dim} of {head_dim}")
+        r = rotary_dim if rotary_dim is not None else part if part is not None else head_dim
         if r < 2 or r % 2 or r > head_dim:
             raise ValueError(f"rotary_dim must be even and within the head of {head_dim}, got {r}")
         if r > 256:
             raise ValueError(f"rotary_dim up to 256 is supported, got {r}")
         if layout not in _LAYOUTS:
             raise ValueError(f"layout must be 'half' or 'interleaved', got {layout!r}")
-        if not theta > 1:
-            raise ValueError(f"theta must exceed 1, got {theta}")
-        self.head_dim, self.rotary_dim, self.theta, self.layout = head_dim, r, float(theta), layout
+        self.head_dim, self.rotary_dim, self.theta, self.layout = head_dim, r, _theta(theta, scaling), layout
         self.frequencies, self.magnitude = rotary_frequencies(r, self.theta, scaling)
         self._turns = (C.c_double * (r // 2))(*[f / (2.0 * math.pi) for f in self.frequencies])
 

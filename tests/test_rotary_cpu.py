@@ -1,0 +1,52 @@
+"""Rotary positions without a GPU: the scalings' keys, and what autograd sees."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import dcc_kv_b200 as dk
+
+
+@pytest.mark.parametrize("theta,n,extra", [
+    (150000.0, 4096, {"factor": 32.0, "truncate": False}), (150000.0, 4096, {"factor": 32.0, "truncate": True}),
+    (10000.0, 4096, {"factor": 40.0, "mscale": 1.0, "mscale_all_dim": 1.0}),
+    (10000.0, 4096, {"factor": 40.0, "mscale": 0.707, "mscale_all_dim": 1.2}),
+    (10000.0, 4096, {"factor": 40.0, "mscale": 0.707}), (10000.0, 4096, {"factor": 40.0, "mscale_all_dim": 1.0}),
+    (10000.0, 4096, {"factor": 40.0, "mscale": 1.0, "mscale_all_dim": 1.0, "attention_factor": 1.25}),
+    (10000.0, 4096, {"factor": 40.0, "mscale": 0.0, "mscale_all_dim": 1.0}),
+    (1000000.0, 32768, {"factor": 4.0, "beta_fast": 32.0, "beta_slow": 1.0, "truncate": False})])
+def test_every_yarn_key_agrees_with_transformers(theta, n, extra):
+    pytest.importorskip("transformers")
+    from transformers import LlamaConfig
+    from transformers.modeling_rope_utils import ROPE_INIT_FUNCTIONS
+    scaling = {"rope_type": "yarn", "original_max_position_embeddings": n, "rope_theta": theta, **extra}
+    cfg = LlamaConfig(hidden_size=64 * 32, num_attention_heads=32, max_position_embeddings=int(n * extra["factor"]),
+                      rope_theta=theta, rope_scaling=dict(scaling), rope_parameters=dict(scaling))
+    want, magnitude = ROPE_INIT_FUNCTIONS["yarn"](cfg, "cpu")
+    for given in (theta, None):
+        f, m = dk.rotary_frequencies(64, given, scaling)
+        assert m == pytest.approx(magnitude, rel=1e-7)
+        assert torch.tensor(f, dtype=torch.float64) == pytest.approx(want.double(), rel=1e-5)   # theirs are 32-bit
+    rot = dk.Rotary(64, scaling=scaling)
+    assert rot.theta == theta and rot.magnitude == m and rot.frequencies == f
+
+
+def test_scaling_keys_that_would_be_dropped_are_refused():
+    base = {"factor": 4.0, "original_max_position_embeddings": 4096}
+    llama = {"low_freq_factor": 1.0, "high_freq_factor": 4.0}
+    for bad in ({"rope_type": "linear", "factor": 4.0, "mscale": 1.0}, {"rope_type": "yarn", "beta": 3.0, **base},
+                {"rope_type": "ntk", "factor": 4.0, "alpha": 1000}, {"rope_type": "llama3", "truncate": False, **llama, **base},
+                {"rope_type": "default", "factor": 4.0}, {"factor": 4.0}, {"rope_type": "linear", "factor": None},
+                {"rope_type": "yarn", "attention_factor": 0.0, **base}, {"rope_type": "default", "mrope_section": [16, 24, 24]}):
+        with pytest.raises(ValueError, match="rotary scaling"):
+            dk.Rotary(128, scaling=bad)
+    with pytest.raises(ValueError, match="rope_theta"):
+        dk.Rotary(128, theta=500000.0, scaling={"rope_type": "linear", "factor": 4.0, "rope_theta": 10000.0})
+    with pytest.raises(ValueError, match="exceed 1"):
+        dk.Rotary(128, scaling={"rope_type": "default", "rope_theta": 0.5})
+    with pytest.raises(ValueError, match="partial_rotary_factor"):
+        dk.Rotary(128, rotary_dim=32, scaling={"rope_type": "default", "partial_rotary_factor": 0.5})
+    rot = dk.Rotary(128, scaling={"rope_type": "default", "partial_rotary_factor": 0.5, "rope_theta": 50000, "factor": None})
+    assert rot.rotary_dim == 64 and rot.theta == 50000.0 and len(rot.frequencies) == 32
+    assert dk.Rotary(128).theta == 10000.0
+    assert dk.Rotary(128, scaling={"type": "linear", **base}).frequencies[0] == 0.25
