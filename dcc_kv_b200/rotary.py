@@ -15,6 +15,7 @@ import math
 from typing import Mapping, Optional, Tuple, Union
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib as L
 
@@ -202,41 +203,52 @@ class Rotary:
         L.require_cuda(q, positions, k)
         L.same_device(q.device, positions=positions, k=k)
         xs = (q,) if k is None else (q, k)
-        grad = torch.is_grad_enabled() and any(x.requires_grad for x in xs)
         if inplace:
-            if grad:
+            if _differentiated(xs):
                 raise ValueError("inplace rotary positions have no gradient; run without inplace")
             for x in xs:
                 if any(n > 1 and s == 0 for n, s in zip(x.shape, x.stride())) or (x.stride(3) != 1 and x.shape[3] > 1):
                     raise ValueError("inplace needs tensors with unit last stride that are not expanded")
             ys = self._run(xs, positions, False, outs=xs)
-        elif grad:
-            ys = _RotaryFunction.apply(self, positions, False, *xs)
         else:
-            ys = self._run(xs, positions, False)
+            ys = self._map(xs, positions, False)
         return ys[0] if k is None else (ys[0], ys[1])
+
+    def _map(self, xs, positions: torch.Tensor, inverse: bool):
+        if _differentiated(xs):
+            return _RotaryFunction.apply(self, positions, inverse, *xs)
+        return self._run(xs, positions, inverse)
+
+
+def _differentiated(xs) -> bool:
+    """Autograd follows what happens to one of them, in reverse or forward mode."""
+    return (torch.is_grad_enabled() and any(x.requires_grad for x in xs)) or \
+        any(forward_ad.unpack_dual(x).tangent is not None for x in xs)
 
 
 class _RotaryFunction(torch.autograd.Function):
-    """The map is linear: its gradient is the map with the angles negated."""
+    """The map is linear: it is its own derivative, and its gradient is the map
+    with the angles negated."""
 
     @staticmethod
     def forward(ctx, rotary: Rotary, positions: torch.Tensor, inverse: bool, *xs):
         ctx.rotary, ctx.inverse = rotary, inverse
         ctx.save_for_backward(positions)
+        ctx.save_for_forward(positions)
         return tuple(rotary._run(xs, positions, inverse))
+
+    @staticmethod
+    def jvp(ctx, _rotary, _positions, _inverse, *tangents):
+        (positions,) = ctx.saved_tensors
+        ys = iter(ctx.rotary._map([t for t in tangents if t is not None], positions, ctx.inverse))
+        return tuple(None if t is None else next(ys) for t in tangents)
 
     @staticmethod
     def backward(ctx, *grads):
         (positions,) = ctx.saved_tensors
         wanted = [i for i in range(len(grads)) if ctx.needs_input_grad[3 + i]]
         out = [None] * len(grads)
-        gs = [grads[i] for i in wanted]
-        if gs:
-            if torch.is_grad_enabled() and any(g.requires_grad for g in gs):
-                ys = _RotaryFunction.apply(ctx.rotary, positions, not ctx.inverse, *gs)
-            else:
-                ys = ctx.rotary._run(gs, positions, not ctx.inverse)
-            for i, y in zip(wanted, ys):
+        if wanted:
+            for i, y in zip(wanted, ctx.rotary._map([grads[i] for i in wanted], positions, not ctx.inverse)):
                 out[i] = y
         return (None, None, None, *out)

@@ -3,8 +3,11 @@ from __future__ import annotations
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import dcc_kv_b200 as dk
+import decode_ref as ref
+from dcc_kv_b200 import _lib as L
 
 
 @pytest.mark.parametrize("theta,n,extra", [
@@ -50,3 +53,34 @@ def test_scaling_keys_that_would_be_dropped_are_refused():
     assert rot.rotary_dim == 64 and rot.theta == 50000.0 and len(rot.frequencies) == 32
     assert dk.Rotary(128).theta == 10000.0
     assert dk.Rotary(128, scaling={"type": "linear", **base}).frequencies[0] == 0.25
+
+
+@pytest.fixture
+def on_the_cpu(monkeypatch):
+    """The launch replaced by its definition, so that what stands around it runs without a GPU."""
+    def run(self, xs, positions, inverse, outs=None):
+        p = positions.expand(xs[0].shape[0], -1) if positions.dim() == 1 else positions
+        ys = [ref.rotate(x.detach().double(), p, self.frequencies, self.magnitude, self.layout, inverse).to(x.dtype) for x in xs]
+        return ys if outs is None else [o.detach().copy_(y) for o, y in zip(outs, ys)] and list(outs)
+    monkeypatch.setattr(dk.Rotary, "_run", run)
+    monkeypatch.setattr(L, "require_cuda", lambda *tensors: None)
+
+
+def test_forward_mode_tangents(on_the_cpu):
+    rot, pos = dk.Rotary(16, rotary_dim=8), torch.arange(3) + 1000
+    q, tq = torch.randn(2, 2, 4, 3, 16, dtype=torch.float64)
+    k, tk = torch.randn(2, 2, 1, 3, 16, dtype=torch.float64)
+    with forward_ad.dual_level():
+        a, b = rot(forward_ad.make_dual(q, tq), pos, forward_ad.make_dual(k, tk))
+        for y, x, t in ((a, q, tq), (b, k, tk)):
+            got = forward_ad.unpack_dual(y)
+            assert torch.equal(got.primal, rot(x, pos)) and torch.equal(got.tangent, rot(t, pos))
+        a, b = rot(q, pos, forward_ad.make_dual(k, tk))          # one of two
+        assert forward_ad.unpack_dual(a).tangent is None or not forward_ad.unpack_dual(a).tangent.any()
+        assert torch.equal(forward_ad.unpack_dual(b).tangent, rot(tk, pos))
+        assert torch.equal(forward_ad.unpack_dual(rot(forward_ad.make_dual(q, tq), pos)).tangent, rot(tq, pos))
+        with torch.no_grad(), pytest.raises(ValueError, match="gradient"):
+            rot(forward_ad.make_dual(q, tq), pos, inplace=True)
+    assert torch.autograd.gradcheck(lambda x, y: rot(x, pos, y), (q.requires_grad_(), k.requires_grad_()),
+                                    check_forward_ad=True, check_backward_ad=True)
+    assert torch.autograd.gradgradcheck(lambda x, y: rot(x, pos, y), (q, k), check_fwd_over_rev=True)
