@@ -223,6 +223,13 @@ def same_device(device: torch.device, **tensors: Optional[torch.Tensor]) -> None
             raise ValueError(f"{name} is on {t.device}, expected {device}")
 
 
+def written(*tensors: Optional[torch.Tensor]) -> None:
+    """Tells autograd that a kernel has written over these tensors of the
+    caller: a backward pass that saved one of them refuses instead of using
+    the new values."""
+    torch.autograd.graph.increment_version([t for t in tensors if t is not None])
+
+
 def ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 

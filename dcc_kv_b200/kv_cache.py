@@ -145,6 +145,7 @@ class KvCache:
             tok = self._tokens(k, v, logit_bias, page_table, start, counts, b, t)
             L.check(L.lib().dcc_kv_cache_write(self._pages, tok, L.dtype_code(k), L.stream_ptr(self.device)),
                     "kv_cache_write")
+        L.written(self.k, self.v, self.k_scale, self.v_scale, self.logit_bias)
 
     def read(self, page_table: torch.Tensor, start: Union[int, torch.Tensor], length: int,
              counts: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.bfloat16,

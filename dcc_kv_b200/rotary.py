@@ -210,6 +210,7 @@ class Rotary:
                 if any(n > 1 and s == 0 for n, s in zip(x.shape, x.stride())) or (x.stride(3) != 1 and x.shape[3] > 1):
                     raise ValueError("inplace needs tensors with unit last stride that are not expanded")
             ys = self._run(xs, positions, False, outs=xs)
+            L.written(*xs)
         else:
             ys = self._map(xs, positions, False)
         return ys[0] if k is None else (ys[0], ys[1])

@@ -61,7 +61,10 @@ def on_the_cpu(monkeypatch):
     def run(self, xs, positions, inverse, outs=None):
         p = positions.expand(xs[0].shape[0], -1) if positions.dim() == 1 else positions
         ys = [ref.rotate(x.detach().double(), p, self.frequencies, self.magnitude, self.layout, inverse).to(x.dtype) for x in xs]
-        return ys if outs is None else [o.detach().copy_(y) for o, y in zip(outs, ys)] and list(outs)
+        if outs is not None:
+            for o, y in zip(outs, ys):
+                o.detach().numpy()[...] = y.numpy()   # past autograd, as a launch
+        return ys if outs is None else list(outs)
     monkeypatch.setattr(dk.Rotary, "_run", run)
     monkeypatch.setattr(L, "require_cuda", lambda *tensors: None)
 
@@ -84,3 +87,19 @@ def test_forward_mode_tangents(on_the_cpu):
     assert torch.autograd.gradcheck(lambda x, y: rot(x, pos, y), (q.requires_grad_(), k.requires_grad_()),
                                     check_forward_ad=True, check_backward_ad=True)
     assert torch.autograd.gradgradcheck(lambda x, y: rot(x, pos, y), (q, k), check_fwd_over_rev=True)
+
+
+def test_inplace_is_seen_by_a_backward_that_saved_the_tensor(on_the_cpu):
+    rot, pos = dk.Rotary(16), torch.arange(3)
+    w = torch.randn(2, 2, 3, 16, requires_grad=True)
+    q, k = torch.randn(2, 2, 2, 3, 16)
+    for saved in (q, k):
+        y = (w * saved).sum()
+        rot(q, pos, k, inplace=True)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    y = (w * q).sum()
+    rot(q, pos)
+    y.backward()
+    with torch.inference_mode():
+        rot(torch.randn(1, 1, 3, 16), pos, inplace=True)
