@@ -174,7 +174,12 @@ class Rotary:
         for i, x in enumerate(xs):
             if x.stride(3) != 1 and d > 1:
                 x = x.contiguous()
-            y = torch.empty_like(x) if outs is None else outs[i]
+            if outs is not None:
+                y = outs[i]
+            else:
+                y = torch.empty_like(x)  # keeps the order of the axes, but not always a unit last stride of rows that overlap
+                if y.stride(3) != 1:
+                    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
             arr[i] = (x.data_ptr(), y.data_ptr(), *x.stride()[:3], *y.stride()[:3], x.shape[1])
             ys.append(y)
         code = L.dtype_code(xs[0])

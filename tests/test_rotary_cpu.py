@@ -103,3 +103,28 @@ def test_inplace_is_seen_by_a_backward_that_saved_the_tensor(on_the_cpu):
     y.backward()
     with torch.inference_mode():
         rot(torch.randn(1, 1, 3, 16), pos, inplace=True)
+
+
+def test_rows_that_overlap(monkeypatch):
+    """Views whose rows lie one element apart: the result has rows of its own."""
+    called = []
+
+    class Library:
+        def dcc_rotary(self, arr, n, *rest):
+            called.extend((t.y_seq_stride, t.y_head_stride, t.y_row_stride) for t in arr)
+            return L.DCC_OK
+
+    monkeypatch.setattr(L, "lib", Library)
+    monkeypatch.setattr(L, "require_cuda", lambda *tensors: None)
+    monkeypatch.setattr(L, "stream_ptr", lambda device: 0)
+    monkeypatch.setattr(L, "on_device", lambda device: torch.no_grad())
+    base = torch.zeros(4096)
+    rot = dk.Rotary(64)
+    for shape, strides in (((1, 3, 5, 64), (0, 70, 1, 1)), ((2, 3, 4, 64), (1000, 100, 1, 1)), ((2, 3, 5, 64), (1, 64, 2, 1)),
+                           ((2, 3, 5, 64), (0, 0, 0, 1))):
+        y = rot(torch.as_strided(base, shape, strides), torch.arange(shape[2]))
+        assert y.shape == shape and y.stride(3) == 1 and called[-1] == y.stride()[:3]
+        steps = sorted((s, n) for s, n in zip(y.stride(), shape) if n > 1)
+        assert all(s >= n0 * s0 for (s0, n0), (s, _) in zip(steps, steps[1:]))
+    x = torch.zeros(2, 5, 3, 64).transpose(1, 2)       # ordinary views keep the order of their axes
+    assert rot(x, torch.arange(5)).stride() == x.stride()
