@@ -212,8 +212,8 @@ class Rotary:
             if _differentiated(xs):
                 raise ValueError("inplace rotary positions have no gradient; run without inplace")
             for x in xs:
-                if any(n > 1 and s == 0 for n, s in zip(x.shape, x.stride())) or (x.stride(3) != 1 and x.shape[3] > 1):
-                    raise ValueError("inplace needs tensors with unit last stride that are not expanded")
+                if x.stride(3) != 1 or _overlaps(x):
+                    raise ValueError("inplace needs tensors with unit last stride that are not expanded and do not overlap themselves")
             ys = self._run(xs, positions, False, outs=xs)
             L.written(*xs)
         else:
@@ -224,6 +224,16 @@ class Rotary:
         if _differentiated(xs):
             return _RotaryFunction.apply(self, positions, inverse, *xs)
         return self._run(xs, positions, inverse)
+
+
+def _overlaps(x: torch.Tensor) -> bool:
+    """Two indices of x may be one element: an axis steps by no more than what the axes below it span."""
+    span = 0
+    for stride, n in sorted((s, n) for s, n in zip(x.stride(), x.shape) if n > 1):
+        if stride <= span:
+            return x.numel() > 0
+        span += stride * (n - 1)
+    return False
 
 
 def _differentiated(xs) -> bool:

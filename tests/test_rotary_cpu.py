@@ -128,3 +128,15 @@ def test_rows_that_overlap(monkeypatch):
         assert all(s >= n0 * s0 for (s0, n0), (s, _) in zip(steps, steps[1:]))
     x = torch.zeros(2, 5, 3, 64).transpose(1, 2)       # ordinary views keep the order of their axes
     assert rot(x, torch.arange(5)).stride() == x.stride()
+
+
+def test_inplace_refuses_what_overlaps_itself(on_the_cpu):
+    base, rot = torch.zeros(4096), dk.Rotary(64)
+    for shape, strides in (((1, 3, 5, 64), (0, 70, 1, 1)), ((2, 3, 4, 64), (1000, 100, 32, 1)), ((2, 3, 5, 64), (320, 320, 64, 1)),
+                           ((2, 3, 5, 64), (0, 320, 64, 1)), ((1, 1, 2, 64), (0, 0, 63, 1))):
+        with pytest.raises(ValueError, match="overlap"):
+            rot(torch.as_strided(base, shape, strides), torch.arange(shape[2]), inplace=True)
+    for shape, strides in (((1, 3, 5, 64), (0, 400, 64, 1)), ((2, 3, 5, 64), (64, 640, 128, 1)), ((2, 1, 0, 64), (0, 0, 0, 1)),
+                           ((2, 3, 4, 64), (768, 64, 192, 1))):
+        x = torch.as_strided(base, shape, strides)
+        assert rot(x, torch.arange(shape[2]), inplace=True) is x
