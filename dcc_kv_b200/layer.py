@@ -422,6 +422,9 @@ class DccKvSyncLayer:
         if not 0 <= r < self.nb:
             raise ValueError(f"block {r} of {self.nb}")
         self.check_inputs(self.out, k, v)
+        if self._host_stream is not None and self._last_call_host:
+            # the compact keys come from the host-buffer path's stream, which the stream of now may not have waited for
+            torch.cuda.current_stream(self.device).wait_stream(self._host_stream)
         n = self.total[r] + self.L
         if page_table.shape[-1] * cache.page_size < n:
             raise ValueError(f"the page table holds {page_table.shape[-1] * cache.page_size} tokens, need {n}")
