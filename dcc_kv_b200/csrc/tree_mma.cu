@@ -516,7 +516,8 @@ __global__ void __launch_bounds__(Shape<kMode, kD, kNT>::kThreads, 1) tree_mma_k
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                   float x = s[m][2 * u + h];
-                  if constexpr (k8) x += log2f(fminf(vs[u], kMost));
+                  // (a NaN scale is not to move the max: it makes the row NaN by its product)
+                  if constexpr (k8) x += log2f(fminf(fmaxf(vs[u], 7.888609e-31f), kMost));
                   if (seen(2 * u + h)) top = fmaxf(top, x);
                 }
 #pragma unroll

@@ -3,14 +3,31 @@ values that are not finite or of extreme size, masks, pools that a caller
 filled, and waits that ran out."""
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
 import dcc_kv_b200 as dk
+import decode_ref as ref
 
-from gpu_util import dev
+from gpu_util import assert_no_device_timeouts, dev
+from test_gpu_decode import filled, gen, lens, randn, within
 
 pytestmark = pytest.mark.gpu
+
+# newest tokens, query heads of a KV head: both sides of every rule on rows
+ROWS = [(1, 4), (6, 2), (20, 4), (70, 2), (70, 4)]
+
+
+def packed(g, fmt, b, d, n, k, v, bias=None, page=16):
+    """b sequences that read the same n cached tokens (one KV head): one sequence
+    is whole in a CTA when b is large."""
+    per = -(-n // page)
+    cache = dk.KvCache.empty(per, page, 1, d, fmt, logit_bias=bias is not None, device=dev())
+    table = torch.arange(per, dtype=torch.int32, device=dev())[None]
+    cache.write(k, v, table, 0, logit_bias=bias)
+    return cache, table.expand(b, per)
 
 
 def test_hand_over_on_another_stream_behind_a_host_forward():
@@ -32,3 +49,29 @@ def test_hand_over_on_another_stream_behind_a_host_forward():
         rk, rv, rb = cache.read(table, 0, layer.total[nb - 1], logit_bias=True)
         for got, want in ((rk, layer.ck), (rv, layer.cv), (rb, layer.cb)):
             assert torch.equal(got[0], want[nb - 1])
+
+
+# ---- attention: values that are not finite -----------------------------------------------------------
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "int8", "e4m3", "f32"])
+@pytest.mark.parametrize("t,group", ROWS)
+@pytest.mark.parametrize("at", [0, 300, 777])
+def test_a_nan_value_makes_the_rows_that_see_it_nan(fmt, t, group, at):
+    """One column of it in the types without a scale; the log-sum-exp is that of the keys."""
+    g = gen(31)
+    cache, table = filled(g, fmt, 1, 2, 64, 16, 900 + t, outliers=False)
+    q = randn(g, 1, 2 * group, t, 64, dtype=torch.bfloat16)
+    want = dk.tree_attention(q, cache, table, lens(900))
+    k, v = cache.read(table, lens(at), 1, dtype=torch.float32)
+    v[..., 5] = math.nan
+    cache.write(k, v, table, at)
+    o, lse = dk.tree_attention(q, cache, table, lens(900))
+    hit = torch.ones(64, dtype=torch.bool, device=dev())
+    if fmt in ("bf16", "f32"):
+        hit[:] = False
+        hit[5] = True
+    assert torch.isnan(o[..., hit]).all()
+    assert torch.equal(o[..., ~hit], want[0][..., ~hit])
+    # the row's max may be up to 2^-100 lower and is then a number below 128: half a step of it and one of the difference
+    within(lse, want[1].double(), 2.0 ** -17 * (1 + want[1].double().abs()))
