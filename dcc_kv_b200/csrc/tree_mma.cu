@@ -635,13 +635,14 @@ __global__ void __launch_bounds__(Shape<kMode, kD, kNT>::kThreads, 1) tree_mma_k
         for (int r0 = 8 * m; r0 < min(rows, 8 * m + 8); r0 += 2) {
           if (2 * t == (r0 & 7)) {  // this lane has the two rows
             float f[2];
+            bool none[2];  // a warp that saw no key of the row has nothing to add
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               float top = -INFINITY;
               for (int x = 0; x < NW; ++x) top = fmaxf(top, sm.m[x][r0 + h]);
               const float own = sm.m[warp][r0 + h];
-              // a warp that saw no key of the row has nothing to add
-              f[h] = sm.l[warp][r0 + h] == 0.f ? 0.f : own == top ? 1.f : exp2f(own - top);
+              none[h] = sm.l[warp][r0 + h] == 0.f;
+              f[h] = own == top ? 1.f : exp2f(own - top);  // 0 is a factor too: O may hold a NaN
             }
             float* dst = sm.sum + warp * 2 * kD;
 #pragma unroll
@@ -649,7 +650,7 @@ __global__ void __launch_bounds__(Shape<kMode, kD, kNT>::kThreads, 1) tree_mma_k
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 const int col = (k8 ? X::kVB * g + 2 * j : (j >> 2) * 64 + 8 * g + 2 * (j & 3)) + (e >> 1);
-                dst[(e & 1) * kD + col] = f[e & 1] == 0.f ? 0.f : f[e & 1] * o[m][j][e];
+                dst[(e & 1) * kD + col] = none[e & 1] ? 0.f : f[e & 1] * o[m][j][e];
               }
           }
           __syncthreads();

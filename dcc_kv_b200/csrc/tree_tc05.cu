@@ -846,19 +846,24 @@ __device__ __forceinline__ void softmax(const TreeParams& p, SmemOf<kMode, kD, k
       softmax_sync();
       tc_fence_after();
       const bool other = !kPair && count > 1;  // both streams had a tile
-      float f0 = 1.f, f1 = 0.f, top = m, sum = l;  // of stream 0 and 1, or of this stream
+      // of stream 0 and 1, or of this stream; `none`: the row saw no key there
+      // (a factor of 0 is one: O may hold a NaN)
+      float f0 = 1.f, f1 = 0.f, top = m, sum = l;
+      bool none0 = l == 0.f, none1 = true;
       if constexpr (!kPair) {
         const float2 a = sm.ml[0][row], b = sm.ml[1][row];
         top = fmaxf(a.x, b.x);
-        f0 = a.y == 0.f ? 0.f : a.x == top ? 1.f : exp2f(a.x - top);
-        f1 = b.y == 0.f ? 0.f : b.x == top ? 1.f : exp2f(b.x - top);
-        sum = (a.y == 0.f ? 0.f : f0 * a.y) + (b.y == 0.f ? 0.f : f1 * b.y);
-      } else if (l == 0.f) {
-        f0 = 0.f;
+        none0 = a.y == 0.f;
+        none1 = b.y == 0.f;
+        f0 = a.x == top ? 1.f : exp2f(a.x - top);
+        f1 = b.x == top ? 1.f : exp2f(b.x - top);
+        sum = (none0 ? 0.f : f0 * a.y) + (none1 ? 0.f : f1 * b.y);
       }
       // a piece of one tile lies in one stream
       const uint32_t col_a = lanes + X::kColO + (uint32_t)(kPair ? stream : other ? 0 : base % 2) * 128;
-      const float fa = kPair || other ? f0 : base % 2 ? f1 : f0;
+      const bool second = !kPair && !other && base % 2;
+      const float fa = second ? f1 : f0;
+      const bool none_a = second ? none1 : none0;
       if (own.t >= w.s.cnt) sum = 0.f;  // a row that does not exist
       // -kMost: nothing but biases of the type's lowest value
       const float ln = top == -kMost ? -kMost : top * kLn2;
@@ -873,13 +878,13 @@ __device__ __forceinline__ void softmax(const TreeParams& p, SmemOf<kMode, kD, k
         tmem_ld32(col_a + 32 * c, reinterpret_cast<uint32_t*>(d));
         tmem_wait_ld();
 #pragma unroll
-        for (int x = 0; x < 32; ++x) d[x] = fa == 0.f ? 0.f : fa * d[x];
+        for (int x = 0; x < 32; ++x) d[x] = none_a ? 0.f : fa * d[x];
         if (other) {
           float e[32];
           tmem_ld32(col_a + 128 + 32 * c, reinterpret_cast<uint32_t*>(e));
           tmem_wait_ld();
 #pragma unroll
-          for (int x = 0; x < 32; ++x) d[x] = f1 == 0.f ? d[x] : fmaf(f1, e[x], d[x]);
+          for (int x = 0; x < 32; ++x) d[x] = none1 ? d[x] : fmaf(f1, e[x], d[x]);
         }
         if (!own.exists) continue;
         if (w.part >= 0) {

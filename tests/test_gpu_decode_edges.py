@@ -75,3 +75,24 @@ def test_a_nan_value_makes_the_rows_that_see_it_nan(fmt, t, group, at):
     assert torch.equal(o[..., ~hit], want[0][..., ~hit])
     # the row's max may be up to 2^-100 lower and is then a number below 128: half a step of it and one of the difference
     within(lse, want[1].double(), 2.0 ** -17 * (1 + want[1].double().abs()))
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "int8", "e4m3", "f32"])
+@pytest.mark.parametrize("t,group", ROWS)
+@pytest.mark.parametrize("at", [40, 130, 300, 777])
+@pytest.mark.parametrize("b", [1, 160])
+def test_a_nan_value_counts_however_small_its_weight(fmt, t, group, at, b):
+    """Its weight underflows beside keys e^1600 ahead, in the same tile or in another one, of the same CTA or not."""
+    g = gen(32)
+    n = 900
+    k, v = torch.zeros(1, 1, n, 64, device=dev()), randn(g, 1, 1, n, 64)
+    k[..., 0] = -800.0
+    top = 512 if at != 777 else 16
+    k[:, :, top: top + 16, 0] = 800.0
+    v[:, :, at] = math.nan
+    cache, table = packed(g, fmt, b, 64, n, k, v)
+    q = torch.zeros(b, group, t, 64, dtype=torch.bfloat16, device=dev())
+    q[..., 0] = 1
+    o, lse = dk.tree_attention(q, cache, table, lens(*[n - t] * b), scale=1.0)
+    assert torch.isnan(o).all()
+    assert torch.isfinite(lse).all()
