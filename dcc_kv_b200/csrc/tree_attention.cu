@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(kSimtThreads) tree_simt_kernel(const __grid_co
       for (int r = 0; r < kSimtRows; ++r) {
         if (w.part >= 0) {
           const int64_t slot = p.part_row(span, rt, w.part, r);
-          if (tid < d) p.part_o[slot * kTreePartCols + tid] = o[r];
+          if (tid < d) p.part_o[slot * kTreePartCols + tid] = l_s[r] == 0.f ? 0.f : o[r] / l_s[r];
           if (tid == 0) {
             p.part_ml[slot * 2] = m_s[r];
             p.part_ml[slot * 2 + 1] = l_s[r];
@@ -162,7 +162,9 @@ __global__ void __launch_bounds__(kSimtThreads) tree_simt_kernel(const __grid_co
 constexpr int kMergeWarps = 4;
 
 // One warp per row of an item that several CTAs worked on (or that no key
-// tile belongs to): o = sum_i e^(m_i - m) O_i / sum_i e^(m_i - m) l_i.
+// tile belongs to): with w_i = e^(m_i - m) l_i, o = sum_i w_i O_i / sum_i w_i
+// (O_i is an output already, so whatever the sizes of the values are, only
+// weights are compared here).
 template <typename T>
 __global__ void __launch_bounds__(kMergeWarps * 32) tree_merge_kernel(const __grid_constant__ TreeParams p) {
   __shared__ int64_t sums[2][kMergeWarps];
@@ -213,8 +215,8 @@ __global__ void __launch_bounds__(kMergeWarps * 32) tree_merge_kernel(const __gr
     const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + slot(i) * 2);
     const float4 v = *reinterpret_cast<const float4*>(p.part_o + slot(i) * kTreePartCols + lane * 4);
     if (ml.y == 0.f) continue;  // no key of that part was seen; its O holds nothing
-    const float w = expf(ml.x - msub);
-    l = fmaf(w, ml.y, l);
+    const float w = expf(ml.x - msub) * ml.y;
+    l += w;
     o[0] = fmaf(w, v.x, o[0]);
     o[1] = fmaf(w, v.y, o[1]);
     o[2] = fmaf(w, v.z, o[2]);

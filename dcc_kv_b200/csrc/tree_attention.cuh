@@ -8,7 +8,7 @@
 // (span, group) walks over its span for the row tiles group, group + n_groups,
 // ...: the CTAs that read the same keys for other rows are neighbours and run
 // at the same time, so the keys come from HBM once.  A (sequence, KV head) that
-// does not lie in one span leaves unnormalised partial results (O, max, sum),
+// does not lie in one span leaves partial results (output, max, sum),
 // which tree_merge_kernel adds in the order of the spans -- no atomics, so
 // results repeat bit for bit.  The lengths are read on the device: neither the
 // launch nor a captured graph depends on them.
@@ -57,6 +57,23 @@ __device__ __forceinline__ int64_t tree_key_tiles(const SeqTokens& s) { return (
 __device__ __forceinline__ bool tree_sees(const TreeParams& p, int b, int64_t t, int64_t i) {
   return p.q.tree ? p.q.tree[b * p.q.tree_seq_stride + t * p.q.T + i] != 0 : i <= t;
 }
+
+// Where weights are held in fp16 (beside 8-bit codes) they carry the V scale, in
+// units of 2^(e - 6) with e the exponent of the largest V scale of the first
+// keys of a part (0 where those have none): the first weights are below 2^7
+// whatever the values' size, also where the scores are so large (biases of the
+// type's lowest value) that a logarithm added to them is lost, and six bits
+// more of small weights are kept.  2^8 on, where the running max has to move,
+// fp16 still reaches.  (Scales of one sequence that differ by more than 2^90 are
+// beyond this.)
+constexpr int kWeightUp = 6;
+constexpr float kLeastScale = 5.048709793e-29f;  // 2^-94, in those units: rows that were never written have scale 0
+constexpr float kMostScale = 3.402823466e38f;
+__device__ __forceinline__ int scale_exponent(float largest) {
+  const int e = (int)(__float_as_uint(largest) >> 23) - 127;
+  return e < -64 || e > 126 ? 0 : e;  // rows of zeros or never written, or not a number
+}
+__device__ __forceinline__ float two_to(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 
 // n spans of `total` >= n tiles, none empty.
 __device__ __forceinline__ int span_count(int64_t total, int n_spans) { return (int)(total < n_spans ? total : n_spans); }

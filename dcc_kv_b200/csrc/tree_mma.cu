@@ -24,8 +24,9 @@
 // sums and O in registers; the warps are added up at the end of a piece.  P is
 // rounded once, to bf16 beside bf16 values (a relative 2^-9 of each weight), to
 // fp16 beside codes (2^-12): there P carries the V scale, so the max is taken
-// over score + log2(scale), which keeps P below 2^8 whatever the scales are
-// (below 2^-14 of that maximum fp16 is subnormal and holds P to 2^-25 of it).
+// over score + log2(scale), in units that keep it below 2^14 (kWeightUp in
+// tree_attention.cuh; below 2^-20 of the largest fp16 is subnormal and holds P
+// to 2^-31 of that).
 // Measured: 16 sequences of 8192 tokens, 4 query heads on each of 8 KV heads of
 // 128: int8 75 us or 3.7 TB/s, e4m3 85 us, bf16 105 us or 5.1 TB/s; with 16 rows
 // per KV head 112 and 116 us.  8-bit codes are bound by the issue of their
@@ -61,7 +62,7 @@ struct Shape {
   static constexpr bool kQShared = k8 && kNT > 1;
   static constexpr int kQ = kQShared ? kNT * kSteps * 256 : 16;
   static constexpr int kSum = kWarps * 2 * kD * 4;   // O of two rows of every warp
-  static constexpr size_t kFixed = kSum + (size_t)kWarps * 8 * kNT * 8 + kWarps * 64 + kQ + 1024;
+  static constexpr size_t kFixed = kSum + (size_t)kWarps * 8 * kNT * 8 + kWarps * 68 + kQ + 1024;
   static constexpr int kFit = (int)((kSmemLimit - kFixed) / ((size_t)kStage * kWarps));
   static constexpr int kStages = kFit < 6 ? kFit : 6;
   static_assert(kStages >= 2, "ring");
@@ -73,6 +74,7 @@ struct Smem {
   float sum[X::kSum / 4];
   __align__(16) unsigned char q[X::kQ];
   float m[X::kWarps][8 * kNT], l[X::kWarps][8 * kNT];
+  int up[X::kWarps];  // exponent of the warp's V scales (see kWeightUp)
   int2 info[X::kWarps][X::kStages];  // keys that exist (16 bits), first key behind the context
   TreePlanSmem plan;
 };
@@ -419,6 +421,19 @@ __global__ void __launch_bounds__(Shape<kMode, kD, kNT>::kThreads, 1) tree_mma_k
 #pragma unroll
         for (int j = 0; j < X::kTiles; ++j) o[m][j][0] = o[m][j][1] = o[m][j][2] = o[m][j][3] = 0.f;
       }
+      int v_exp = -128;   // exponent of the V scales of this warp's first keys; -128: no keys
+      float v_unit = 1.f;
+      if constexpr (k8) {
+        if (mine < stop) {
+          asm volatile("cp.async.wait_group %0;\n" ::"n"(2 * S - 1) : "memory");
+          __syncwarp();
+          float most = load_one(ring_side + (uint32_t)get * X::kStage + 128 + 4 * (lane & 15));
+#pragma unroll
+          for (int off = 8; off > 0; off /= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
+          v_exp = scale_exponent(most);
+          v_unit = two_to(kWeightUp - v_exp);
+        }
+      }
 #pragma unroll 1
       for (; mine < stop; mine += NW) {
         asm volatile("cp.async.wait_group %0;\n" ::"n"(2 * S - 1) : "memory");  // K and scales of this chunk
@@ -470,8 +485,8 @@ __global__ void __launch_bounds__(Shape<kMode, kD, kNT>::kThreads, 1) tree_mma_k
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             ks[u] = load_one(ring_side + from + 64 + 32 * u + 4 * g);
-            vs[u] = load_one(ring_side + from + 128 + 32 * u + 4 * g);
-            vs[u] = vs[u] < 7.888609e-31f ? 7.888609e-31f : vs[u];  // 2^-100: rows that were never written have scale 0
+            vs[u] = load_one(ring_side + from + 128 + 32 * u + 4 * g) * v_unit;
+            vs[u] = vs[u] < kLeastScale ? kLeastScale : vs[u];
           }
         }
         uint32_t pr[kNT][2];
@@ -496,7 +511,7 @@ __global__ void __launch_bounds__(Shape<kMode, kD, kNT>::kThreads, 1) tree_mma_k
                   if (kHidden) y = seen(e) ? y : 0.f;  // a hidden key's scale may be NaN
                 }
                 w4[e] = y;
-                over = over || y > 256.f;
+                over = over || y > (k8 ? 256.f * (1 << kWeightUp) : 256.f);
               }
               return over;
             };
@@ -517,7 +532,7 @@ __global__ void __launch_bounds__(Shape<kMode, kD, kNT>::kThreads, 1) tree_mma_k
                 for (int u = 0; u < 2; ++u) {
                   float x = s[m][2 * u + h];
                   // (a NaN scale is not to move the max: it makes the row NaN by its product)
-                  if constexpr (k8) x += log2f(fminf(fmaxf(vs[u], 7.888609e-31f), kMost));
+                  if constexpr (k8) x += log2f(fminf(fmaxf(vs[u], kLeastScale), kMostScale)) - kWeightUp;
                   if (seen(2 * u + h)) top = fmaxf(top, x);
                 }
 #pragma unroll
@@ -626,7 +641,17 @@ __global__ void __launch_bounds__(Shape<kMode, kD, kNT>::kThreads, 1) tree_mma_k
             sm.l[warp][8 * m + 2 * t + h] = l[m][h];
           }
         }
+      if (lane == 0) sm.up[warp] = v_exp;
       __syncthreads();
+      int most_up = 0;
+      float to_most = 1.f, from_most = 1.f;  // from this warp's units to those of the largest, from those to none
+      if constexpr (k8) {
+        most_up = sm.up[0];
+#pragma unroll
+        for (int x = 1; x < NW; ++x) most_up = max(most_up, sm.up[x]);
+        to_most = two_to(max(v_exp - most_up - kWeightUp, -126));
+        from_most = two_to(most_up);
+      }
       const int64_t rows_left = p.q.T * p.group - (int64_t)rt * kRows;
       const int rows = rows_left < kRows ? (int)rows_left : kRows;
 #pragma unroll
@@ -642,7 +667,7 @@ __global__ void __launch_bounds__(Shape<kMode, kD, kNT>::kThreads, 1) tree_mma_k
               for (int x = 0; x < NW; ++x) top = fmaxf(top, sm.m[x][r0 + h]);
               const float own = sm.m[warp][r0 + h];
               none[h] = sm.l[warp][r0 + h] == 0.f;
-              f[h] = own == top ? 1.f : exp2f(own - top);  // 0 is a factor too: O may hold a NaN
+              f[h] = (own == top ? 1.f : exp2f(own - top)) * to_most;  // 0 is a factor too: O may hold a NaN
             }
             float* dst = sm.sum + warp * 2 * kD;
 #pragma unroll
@@ -670,12 +695,13 @@ __global__ void __launch_bounds__(Shape<kMode, kD, kNT>::kThreads, 1) tree_mma_k
             const TreeRow row = tree_row(p, w.hk, rt, r);
             if (r >= rows) continue;
             if (row.t >= w.s.cnt) sum = 0.f;  // a row that does not exist
+            const float out = sum != 0.f ? acc / sum * from_most : 0.f;
             if (w.part >= 0) {
               const int64_t part = p.part_row(span, rt, w.part, r);
-              if (col < d) p.part_o[part * kTreePartCols + col] = acc;
+              if (col < d) p.part_o[part * kTreePartCols + col] = out;
               if (col == 0) *reinterpret_cast<float2*>(p.part_ml + part * 2) = make_float2(ln, sum);
             } else {
-              if (col < d) tree_out_row<__nv_bfloat16>(p, w.b, row)[col] = __float2bfloat16_rn(sum != 0.f ? acc / sum : 0.f);
+              if (col < d) tree_out_row<__nv_bfloat16>(p, w.b, row)[col] = __float2bfloat16_rn(out);
               if (col == 0 && p.q.lse)
                 p.q.lse[((int64_t)w.b * p.q.n_q_heads + row.h) * p.q.T + row.t] = sum != 0.f ? ln + logf(sum) : -INFINITY;
             }

@@ -31,9 +31,9 @@
 // The running max of a row moves (with O and the sums rescaled) only when a
 // score passes it by 2^8.  P is rounded once for its MMA, to bf16 beside bf16
 // values (a relative 2^-9 of each weight) and to fp16 beside 8-bit ones (2^-12):
-// there P carries the V scale, so the max is taken over score + log2(scale),
-// which keeps P below 2^8 whatever the scales are (below 2^-14 of that maximum
-// fp16 is subnormal and holds P to 2^-25 of it).
+// there P carries the V scale, so the max is taken over score + log2(scale), in
+// units that keep P below 2^14 (kWeightUp in tree_attention.cuh; below 2^-20 of
+// the largest fp16 is subnormal and holds P to 2^-31 of that).
 //
 // Measured (8 KV heads of 128, 4 query heads each): 64 tokens over 131072, bf16,
 // 193 us or 710 TFLOP/s; int8, 290 us; 13 tokens of 16 sequences over 4001, int8,
@@ -70,7 +70,7 @@ struct Shape {
   static constexpr int kBlocks = kD / 64;             // 64-column blocks of 128 swizzled rows
   static constexpr uint32_t kColS = 0, kColO = 256;   // TMEM columns, 128 a stream
   static constexpr int kArrays = k8 ? 3 : 1;          // bias; K and V scales
-  static constexpr size_t kFixed = (size_t)kRows * kD * 2 + (size_t)kRing * kArrays * 512 + 2 * 4 * 512 + 3 * 1024 + kRows * 4;
+  static constexpr size_t kFixed = (size_t)kRows * kD * 2 + (size_t)kRing * kArrays * 512 + 2 * 4 * 512 + 3 * 1024 + kRows * 4 + 40;
   static constexpr int kFit = (int)((kSmemLimit - kFixed) / kTile);
   static constexpr int kSlotsV = (kFit + 1) / 2 < 4 ? (kFit + 1) / 2 : 4, kSlotsK = kFit / 2 < 4 ? kFit / 2 : 4;
   static constexpr int kSlots = kSlotsK + kSlotsV;
@@ -99,6 +99,8 @@ struct Smem {
   // V scale's logarithm with the bias
   __align__(16) float bias[2][128];
   __align__(16) float ks[2][128], vs[2][128], lift[2][128];
+  float most[2][4];                                   // largest V scale of a stream's first tile, by warp
+  int up[2];                                          // its exponent (see kWeightUp)
   __align__(16) uint8_t vis[kRing][16];               // bits: keys that exist
   int32_t pages[2][kFetch][16];                       // of every eighth key of the next K and V tiles
   float qf[X::kRows];                                 // what undoes the scaling of a query row
@@ -644,6 +646,7 @@ __device__ __forceinline__ void softmax(const TreeParams& p, SmemOf<kMode, kD, k
       const float unit = X::k8 ? scale * sm.qf[r] : scale;
       const TreeRow own = tree_row(p, w.hk, rt, r);
       float m = -INFINITY, l = 0.f;
+      int v_exp = 0;  // exponent of the stream's V scales
       const bool busy = __any_sync(0xffffffffu, own.exists);  // else no row of the warp is anybody's
       const int count = w.k1 - w.k0;
       const int skip = kPair ? 0 : (stream - base % 2 + 2) % 2;
@@ -680,13 +683,25 @@ __device__ __forceinline__ void softmax(const TreeParams& p, SmemOf<kMode, kD, k
               }
             }
           }
+          if constexpr (X::k8) {
+            if (first) {
+              float most = fmaxf(sm.side[ring][2][row], 0.f);
+#pragma unroll
+              for (int off = 16; off > 0; off /= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
+              if (lane == 0) sm.most[stream][wq] = most;
+            }
+          }
           group_sync(stream);  // the arrays of the last tile have been read
           sm.bias[stream][row] = bias;
           if constexpr (X::k8) {
-            const float vs = fmaxf(sm.side[ring][2][row], 7.888609e-31f);  // 2^-100: rows that were never written have scale 0
+            if (first) {
+              v_exp = scale_exponent(fmaxf(fmaxf(sm.most[stream][0], sm.most[stream][1]), fmaxf(sm.most[stream][2], sm.most[stream][3])));
+              if (row == 0) sm.up[stream] = v_exp;
+            }
+            const float own_vs = sm.side[ring][2][row] * two_to(kWeightUp - v_exp), vs = fmaxf(own_vs, kLeastScale);
             sm.ks[stream][row] = sm.side[ring][1][row];
-            sm.vs[stream][row] = sm.side[ring][2][row] < 7.888609e-31f ? vs : sm.side[ring][2][row];
-            sm.lift[stream][row] = __log2f(vs) + bias;
+            sm.vs[stream][row] = own_vs < kLeastScale ? vs : own_vs;
+            sm.lift[stream][row] = __log2f(vs) - kWeightUp + bias;
           }
           group_sync(stream);
         }
@@ -859,6 +874,18 @@ __device__ __forceinline__ void softmax(const TreeParams& p, SmemOf<kMode, kD, k
         f1 = b.x == top ? 1.f : exp2f(b.x - top);
         sum = (none0 ? 0.f : f0 * a.y) + (none1 ? 0.f : f1 * b.y);
       }
+      float unit_o = 1.f;  // of O
+      if constexpr (X::k8) {
+        if (other) v_exp = max(sm.up[0], sm.up[1]);
+        else if (!kPair) v_exp = sm.up[base % 2];
+        unit_o = two_to(v_exp);
+        if constexpr (kPair) {
+          f0 *= two_to(-kWeightUp);
+        } else {
+          f0 *= two_to(max(sm.up[0] - v_exp - kWeightUp, -126));
+          f1 *= two_to(max(sm.up[1] - v_exp - kWeightUp, -126));
+        }
+      }
       // a piece of one tile lies in one stream
       const uint32_t col_a = lanes + X::kColO + (uint32_t)(kPair ? stream : other ? 0 : base % 2) * 128;
       const bool second = !kPair && !other && base % 2;
@@ -887,6 +914,8 @@ __device__ __forceinline__ void softmax(const TreeParams& p, SmemOf<kMode, kD, k
           for (int x = 0; x < 32; ++x) d[x] = none1 ? d[x] : fmaf(f1, e[x], d[x]);
         }
         if (!own.exists) continue;
+#pragma unroll
+        for (int x = 0; x < 32; ++x) d[x] = d[x] * inv * unit_o;
         if (w.part >= 0) {
 #pragma unroll
           for (int x = 0; x < 32; x += 4)
@@ -894,7 +923,7 @@ __device__ __forceinline__ void softmax(const TreeParams& p, SmemOf<kMode, kD, k
               *reinterpret_cast<float4*>(p.part_o + part * kTreePartCols + 32 * c + x) = make_float4(d[x], d[x + 1], d[x + 2], d[x + 3]);
         } else {
 #pragma unroll
-          for (int x = 0; x < 32; ++x) d[x] = sum != 0.f ? d[x] * inv : 0.f;
+          for (int x = 0; x < 32; ++x) d[x] = sum != 0.f ? d[x] : 0.f;
 #pragma unroll
           for (int x = 0; x < 32; x += 8) {
             if (32 * c + x >= p.c.head_dim) continue;

@@ -96,3 +96,67 @@ def test_a_nan_value_counts_however_small_its_weight(fmt, t, group, at, b):
     o, lse = dk.tree_attention(q, cache, table, lens(*[n - t] * b), scale=1.0)
     assert torch.isnan(o).all()
     assert torch.isfinite(lse).all()
+
+
+# ---- attention: values of extreme size beside 8-bit codes, whose weights carry the V scale in fp16 ------
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "int8", "e4m3"])
+@pytest.mark.parametrize("group", [2, 40, 140])
+@pytest.mark.parametrize("b", [1, 160])
+@pytest.mark.parametrize("size", [1e-6, 1.0, 1e8])
+@pytest.mark.parametrize("low", [torch.finfo(torch.float32).min, -1e30])
+def test_biases_at_the_lowest_value_beside_values_of_any_size(fmt, group, b, size, low):
+    """All keys alike: the mean of the values, although a logarithm of the V scale is lost beside such scores."""
+    g = gen(33)
+    n = 400
+    k, v = (randn(g, 1, 1, n, 64) for _ in range(2))
+    cache, table = packed(g, fmt, b, 64, n, k, v * size, bias=torch.full((1, 1, n), low, device=dev()))
+    q = randn(g, b, group, 1, 64, dtype=torch.bfloat16)
+    o, lse = dk.tree_attention(q, cache, table, lens(*[n - 1] * b))
+    vv = ref.cached(cache, table, 0, n)[1]
+    want, a = vv.mean(1), vv.abs().mean(1)
+    # the sum and the quotient in 32 bits; the weight's rounding and the result's
+    bound = ((n + 20) * ref.F32 + 2.0 ** -20) * a + 2 * ref.BF16 * a
+    within(o[:, :, 0], want.expand(b, group, 64), bound.expand(b, group, 64))
+    assert torch.isfinite(lse).all()
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("t,group", ROWS)
+@pytest.mark.parametrize("b", [1, 160])
+@pytest.mark.parametrize("size", [2.0 ** 122, 2.0 ** -90])
+def test_values_at_the_ends_of_their_type(fmt, t, group, b, size):
+    g = gen(34)
+    n = 700
+    k, v = randn(g, 1, 1, n, 64) * 4, randn(g, 1, 1, n, 64)
+    v[:, :, ::7] *= 2.0 ** -20
+    cache, table = packed(g, fmt, b, 64, n, k, v * size)
+    q = randn(g, 1, group, t, 64, dtype=torch.bfloat16)
+    o, lse = dk.tree_attention(q.expand(b, group, t, 64), cache, table, lens(*[n - t] * b))
+    want = ref.tree(q, cache, table, lens(n - t))
+    for i in (0, b // 2, b - 1):
+        ref.tree_close((o[i: i + 1], lse[i: i + 1]), want, 64, n)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("group", [1, 40, 140])
+def test_many_small_weights_add_up(fmt, group):
+    """One key ahead of 262143 others that weigh 2^-26.3 of it each: 0.3 % in all, in columns of their own.
+    fp16 holds each to 2^-25 / 64 of the largest weight at worst."""
+    b, n = 200, 262144
+    k, v = torch.zeros(1, 1, n, 64, device=dev()), torch.zeros(1, 1, n, 64, device=dev())
+    k[..., 0], k[:, :, 0, 0] = 1, -1
+    v[..., 1], v[:, :, 0, 1], v[:, :, 0, 0] = 1, 0, 1
+    cache, table = packed(gen(35), fmt, b, 64, n, k, v, page=64)
+    q = torch.zeros(1, group, 1, 64, dtype=torch.bfloat16, device=dev())
+    q[..., 0] = -1
+    scale = 13.15 * math.log(2)
+    o, _ = dk.tree_attention(q.expand(b, group, 1, 64), cache, table, lens(*[n - 1] * b), scale=scale)
+    kk, vv, _ = ref.cached(cache, table, 0, n)
+    p = torch.softmax(q[0, :, 0].double() @ kk[0].T * scale, -1)
+    want, a = p @ vv[0], p @ vv[0].abs()
+    # logits below 2^5 in 32 bits, twice; exponential and sum in 32 bits; the result's rounding
+    bound = (2 * 32 * 4 * ref.F32 + 2.0 ** -20) * a + ref.BF16 * want.abs() + n * 2.0 ** -31
+    assert (want[:, 1] > 20 * n * 2.0 ** -31).all()
+    within(o[:, :, 0], want.expand(b, group, 64), bound.expand(b, group, 64))
