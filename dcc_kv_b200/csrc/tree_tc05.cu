@@ -42,8 +42,11 @@
 // and weights share TMEM) and the instruction cache, which all roles share.
 //
 // Waits are bounded (2 s).  After one has run out a role sets the error word
-// and walks through the rest of its loop without waiting, so named barriers
-// still match and TMEM is freed; the outputs are then invalid.
+// and walks through the rest of its loop without waiting; the outputs are then
+// invalid.  Named barriers still match -- whether a warp comes to one depends on
+// lengths and arguments alone, never on what another role left in shared
+// memory --, the copy warps begin no copy into a place whose last one has not
+// landed and wait for all of theirs, and TMEM is freed.
 #include <string>
 #include <type_traits>
 
@@ -301,10 +304,16 @@ __device__ __forceinline__ void copies(const TreeParams& p, const TreeMaps& maps
     fetch();
   }
   Place at(is_v ? X::kSlotsV : X::kSlotsK);
+  int j = 0;
 #pragma unroll 1
-  for (int j = 0; j < n; ++j) {
+  for (; j < n; ++j) {
     const int slot = first_slot + at.slot;
-    if (j >= at.slots) wait_or_skip(ok, &sm.bar_empty[slot], at.use ^ 1);
+    uint64_t* bar = X::k8 ? &sm.bar_raw[slot] : &sm.bar_full[slot];
+    if (j >= at.slots) {
+      wait_or_skip(ok, &sm.bar_empty[slot], at.use ^ 1);
+      wait_or_skip(ok, bar, at.use ^ 1);  // the copies of before have landed, also if others gave up and passed the tile on
+      if (!ok) break;
+    }
     asm volatile("cp.async.wait_group %0;\n" ::"n"(kFetch - 1) : "memory");  // this lane's own page number
     int row = -1;
     if (left[0] > 0) {
@@ -328,10 +337,7 @@ __device__ __forceinline__ void copies(const TreeParams& p, const TreeMaps& maps
         cp_async_arrive(&sm.bar_side[ring]);
       }
     }
-    // after a wait that ran out nothing new is set in flight (what was has
-    // landed by then): the barriers are only passed on
-    uint64_t* bar = X::k8 ? &sm.bar_raw[slot] : &sm.bar_full[slot];
-    const bool lead = ok && row >= 0 && leader;
+    const bool lead = row >= 0 && leader;
     const uint32_t count = __popc(__ballot_sync(0xffffffffu, lead));
     if (lane == 0) mbar_expect_tx(bar, count * bytes);
     __syncwarp();
@@ -349,6 +355,11 @@ __device__ __forceinline__ void copies(const TreeParams& p, const TreeMaps& maps
     at.next();
   }
   asm volatile("cp.async.wait_all;\n" ::: "memory");
+  // nothing may still be on its way into shared memory when the CTA ends
+  for (int i = 0; i < min(j, at.slots); ++i) {
+    const uint32_t last = (uint32_t)((j - 1 - i) / at.slots);  // use of slot i
+    if (!wait_all_lanes(X::k8 ? &sm.bar_raw[first_slot + i] : &sm.bar_full[first_slot + i], last & 1)) ok = false;
+  }
 }
 
 // ---- 8-bit: codes to values ----------------------------------------------------------------
@@ -658,9 +669,9 @@ __device__ __forceinline__ void softmax(const TreeParams& p, SmemOf<kMode, kD, k
         // ---- the keys of the tile, one a thread ----
         wait_or_skip(ok, &sm.bar_side[ring], (uint32_t)(j / kRing) & 1);
         const uint4 vis = *reinterpret_cast<const uint4*>(sm.vis[ring]);
-        bool hidden = (vis.x & vis.y & vis.z & vis.w) != 0xffffffffu || i0 + kTreeKeys > 0;
+        const bool hidden = __any_sync(0xffffffffu, (vis.x & vis.y & vis.z & vis.w) != 0xffffffffu) || i0 + kTreeKeys > 0;
         bool prepared = false;
-        if (X::k8 || p.c.bias || (hidden && guard)) {
+        if (X::k8 || p.c.bias || (guard && i0 + kTreeKeys > 0)) {  // the same in all warps of the stream: they meet at barriers
           prepared = true;
           float bias = p.c.bias ? sm.side[ring][0][row] : 0.f;
           if (bias > -INFINITY && bias < INFINITY) bias = fminf(fmaxf(bias * kLog2e, -kMost), kMost);
