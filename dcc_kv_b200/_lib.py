@@ -10,7 +10,8 @@ from __future__ import annotations
 import contextlib
 import ctypes as C
 import os
-from typing import Optional
+import threading
+from typing import Dict, Optional
 
 import torch
 
@@ -149,6 +150,7 @@ SIGNATURES = {
     "dcc_device_error_status": (_I, [_I]),
     "dcc_build_error_status": (_I, [_I]),
     "dcc_device_error_flags_async": (_I, [_P, _P]),
+    "dcc_device_error_report": (_I, [_P]),
     "dcc_debug_expire_wait": (_I, [C.c_uint64, _P]),
     "dcc_online_softmax_from_attention": (_I, [_P, _P, _P, _I64, _I64, _I64, _I64, _I, _P, _P, _P, _P]),
     "dcc_merge_softmax_states": (_I, [_P, _P, _P, _P, _P, _P, _I64, _I64, _I, _P, _P, _P, _P]),
@@ -278,3 +280,36 @@ class DeviceErrorWatch:
         self.poll()
         check(lib().dcc_device_error_status(1), "attention")
         check(lib().dcc_build_error_status(1), "compact-KV build")
+
+
+_reports: Dict[int, tuple] = {}
+_reports_lock = threading.Lock()
+
+
+def poll_give_ups(device: torch.device) -> None:
+    """Raises ``DccError(DCC_ERR_TIMEOUT)`` when a bounded device-side wait of
+    an earlier decoding call on ``device`` (the current one) has given up, as
+    far as the host can know without a synchronisation: such kernels write a
+    pinned word, one a device, which is read here.  (While a graph is captured
+    nothing is set up and nothing cleared, as both would end the capture.)"""
+    report = _reports.get(device.index)
+    if report is None:
+        if torch.cuda.is_current_stream_capturing():
+            return
+        with _reports_lock:
+            if device.index not in _reports:
+                host = torch.zeros(1, dtype=torch.int32).pin_memory()
+                check(lib().dcc_device_error_report(host.data_ptr()), "device_error_report")
+                _reports[device.index] = (host, C.c_uint32.from_address(host.data_ptr()))
+    elif report[1].value:
+        flags = report[1].value
+        if not torch.cuda.is_current_stream_capturing():
+            lib().dcc_device_error_status(1)  # clears both words (this synchronises; only on the error path)
+        raise DccError(DCC_ERR_TIMEOUT, f"a bounded device wait expired in an earlier call (attention flags {flags}); "
+                                        "its output is not valid")
+
+
+def check_give_ups(device: torch.device, what: str) -> None:
+    """The same after a synchronisation of ``device``."""
+    with on_device(device):
+        check(lib().dcc_device_error_status(1), what)

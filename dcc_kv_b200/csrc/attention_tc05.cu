@@ -23,6 +23,7 @@
 //
 // Every mbarrier wait is bounded (2 s); a timeout sets g_attn_error, the
 // roles unwind, in-flight copies and MMAs are waited for, TMEM is freed.
+#include <atomic>
 #include <memory>
 #include <mutex>
 #include <string>
@@ -614,6 +615,22 @@ int attn_error_flag_address(unsigned int** out) {
   return check_cuda(cudaGetSymbolAddress(reinterpret_cast<void**>(out), g_attn_error), "attention flag address");
 }
 
+// Caller-owned pinned words, one a device, that kernels which give up write to
+// as well: what a call without a flag report of its own (the tree attention)
+// reads before its next launch.
+constexpr int kReportDevices = 64;
+static std::atomic<unsigned int*> g_report[kReportDevices];
+
+static std::atomic<unsigned int*>* report_of_this_device() {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kReportDevices) return nullptr;
+  return &g_report[dev];
+}
+unsigned int* attn_error_report() {
+  std::atomic<unsigned int*>* r = report_of_this_device();
+  return r ? r->load() : nullptr;
+}
+
 // Both error words to host memory by a posted write from the device (pinned
 // host memory is device-accessible under unified addressing), so reading
 // them needs neither a copy engine nor a synchronisation.
@@ -627,14 +644,14 @@ __global__ void flags_to_host_kernel(const unsigned int* score_flag, unsigned in
 // mbarrier that nothing arrives at; when the limit passes it records the
 // timeout in the attention error word (bit 16).  It has no asynchronous
 // copy or MMA in flight, so it simply returns.
-__global__ void expire_wait_kernel(uint64_t limit_ns) {
+__global__ void expire_wait_kernel(uint64_t limit_ns, unsigned int* report) {
   __shared__ uint64_t bar;
   if (threadIdx.x == 0) {
     mbar_init(&bar, 1);
     fence_mbar_init();
   }
   __syncwarp();
-  if (!warp_wait_limited(&bar, 0, limit_ns) && threadIdx.x == 0) atomicOr(&g_attn_error, 16u);
+  if (!warp_wait_limited(&bar, 0, limit_ns) && threadIdx.x == 0) record_give_up(&g_attn_error, report, 16u);
 }
 
 }  // namespace dcc
@@ -661,9 +678,22 @@ extern "C" int dcc_device_error_flags_async(unsigned int* host_flags, void* stre
   return check_cuda(cudaGetLastError(), "device_error_flags_async launch");
 }
 
+extern "C" int dcc_device_error_report(unsigned int* host_word) {
+  std::atomic<unsigned int*>* report = report_of_this_device();
+  if (!report) return fail(DCC_ERR_UNSUPPORTED, "device_error_report: no device, or its ordinal is above 63");
+  if (host_word) {
+    cudaPointerAttributes pa{};
+    DCC_CHECK(check_cuda(cudaPointerGetAttributes(&pa, host_word), "device_error_report: pointer attributes"));
+    if (pa.type != cudaMemoryTypeHost || pa.devicePointer != host_word)
+      return fail(DCC_ERR_INVALID_ARGUMENT, "device_error_report: destination must be pinned host memory");
+  }
+  report->store(host_word);
+  return DCC_OK;
+}
+
 extern "C" int dcc_debug_expire_wait(uint64_t limit_ns, void* stream) {
   if (limit_ns > 100000000ull) return fail(DCC_ERR_INVALID_ARGUMENT, "debug_expire_wait: limit above 100 ms");
-  expire_wait_kernel<<<1, 32, 0, static_cast<cudaStream_t>(stream)>>>(limit_ns);
+  expire_wait_kernel<<<1, 32, 0, static_cast<cudaStream_t>(stream)>>>(limit_ns, attn_error_report());
   return check_cuda(cudaGetLastError(), "debug_expire_wait launch");
 }
 
@@ -675,6 +705,8 @@ extern "C" int dcc_device_error_status(int clear) {
     unsigned int z = 0;
     DCC_CHECK(check_cuda(cudaMemcpyToSymbol(g_attn_error, &z, sizeof(z)), "device_error_status: clear"));
   }
+  if (clear)
+    if (unsigned int* host = attn_error_report()) *static_cast<volatile unsigned int*>(host) = 0;
   if (v) return fail(DCC_ERR_TIMEOUT, "attention: a bounded device wait expired (flags " + std::to_string(v) + ")");
   return DCC_OK;
 }

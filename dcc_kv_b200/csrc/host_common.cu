@@ -50,7 +50,7 @@ const char* dcc_status_string(int status) {
 
 const char* dcc_last_error(void) { return dcc::g_last_error.c_str(); }
 
-int dcc_version(void) { return 3; }
+int dcc_version(void) { return 4; }
 
 size_t dcc_struct_size(const char* name) {
   if (!name) return 0;

@@ -57,6 +57,16 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, uint64
   }
 }
 
+// A wait has run out: sets `flags` in the error word on the device and, where
+// the host gave one, in its own (written whole, so that it is not 0).
+__device__ __forceinline__ void record_give_up(unsigned int* error, unsigned int* report, unsigned int flags) {
+  atomicOr(error, flags);
+  if (report) {
+    *static_cast<volatile unsigned int*>(report) = flags;
+    __threadfence_system();
+  }
+}
+
 // ---- TMA -----------------------------------------------------------------------
 __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1,
                                             int c2) {

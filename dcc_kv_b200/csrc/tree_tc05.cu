@@ -58,6 +58,7 @@ namespace dcc {
 using namespace tc05;
 
 int attn_error_flag_address(unsigned int** out);
+unsigned int* attn_error_report();
 
 namespace tt {
 
@@ -963,12 +964,13 @@ __device__ __forceinline__ void softmax(const TreeParams& p, SmemOf<kMode, kD, k
 template <int kMode, int kD, bool kPair>
 __global__ void __launch_bounds__(Shape<kMode, kD, kPair>::kThreads, 1) tree_tc05_kernel(const __grid_constant__ TreeParams p,
                                                                                         const __grid_constant__ TreeMaps maps,
-                                                                                        unsigned int* error) {
+                                                                                        unsigned int* error,
+                                                                                        unsigned int* report) {
   using X = Shape<kMode, kD, kPair>;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   SmemOf<kMode, kD, kPair>& sm = *reinterpret_cast<SmemOf<kMode, kD, kPair>*>(smem_raw);
   if (smem_u32(smem_raw) & 1023u) {  // the swizzled tiles need it
-    if (threadIdx.x == 0) atomicOr(error, 64u);
+    if (threadIdx.x == 0) record_give_up(error, report, 64u);
     return;
   }
   const int span = blockIdx.x / p.n_groups;
@@ -1018,7 +1020,7 @@ __global__ void __launch_bounds__(Shape<kMode, kD, kPair>::kThreads, 1) tree_tc0
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(X::kRegsWiden));
     widen_tiles<kMode, kD, kPair>(p, sm, warp >= 16, n, warp & 3, lane, ok);
   }
-  if (!ok && lane == 0) atomicOr(error, 32u);
+  if (!ok && lane == 0) record_give_up(error, report, 32u);
   tc_fence_before();
   __syncthreads();
   if (warp == 8) tmem_dealloc(tm, 512);
@@ -1037,7 +1039,7 @@ static int launch(const TreeParams& p, const TreeMaps& maps, unsigned int* error
   if (fa.numRegs < X::kRegsLaunch)
     return fail(DCC_ERR_UNSUPPORTED, "tree_tc05: compiled with " + std::to_string(fa.numRegs) +
                                          " registers per thread, the register split needs " + std::to_string(X::kRegsLaunch));
-  kernel<<<p.n_groups * p.n_spans, X::kThreads, smem, st>>>(p, maps, error);
+  kernel<<<p.n_groups * p.n_spans, X::kThreads, smem, st>>>(p, maps, error, attn_error_report());
   return check_launch("tree_attention");
 }
 template <int kMode, int kD>

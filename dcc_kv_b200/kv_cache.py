@@ -170,6 +170,13 @@ class KvCache:
                     "kv_cache_read")
         return (k, v, bias) if logit_bias else (k, v)
 
+    def check(self) -> None:
+        """Synchronises the device and raises ``DccError(DCC_ERR_TIMEOUT)`` if a
+        bounded device wait of any :func:`~dcc_kv_b200.tree_attention` on it so
+        far gave up (each call also reports the ones before it)."""
+        L.require_cuda(self.k)
+        L.check_give_ups(self.device, "tree_attention")
+
     def _check_rows(self, k: torch.Tensor, v: torch.Tensor) -> Tuple[int, int]:
         if k.dim() != 4 or k.shape[1] != self.n_kv_heads or k.shape[3] != self.head_dim or v.shape != k.shape:
             raise ValueError(f"k and v must be [B, {self.n_kv_heads}, T, {self.head_dim}]; got {tuple(k.shape)}, "

@@ -48,7 +48,11 @@ def tree_attention(q: torch.Tensor, cache: KvCache, page_table: torch.Tensor, co
     Returns (O [B, H_q, T, d] in q's dtype, LSE [B, H_q, T] float32), as
     :func:`~dcc_kv_b200.attention` does: :func:`~dcc_kv_b200.merge_lse` joins
     it with attention over other keys.  A row that sees nothing, and the rows
-    behind counts[s], give O = 0 and LSE = -inf."""
+    behind counts[s], give O = 0 and LSE = -inf.
+
+    Waits inside the kernels are bounded: one that gave up leaves the call's
+    output invalid and is reported by the next call on the device, or by
+    ``cache.check()``, as ``DccError(DCC_ERR_TIMEOUT)``."""
     if q.dim() != 4 or q.shape[3] != cache.head_dim:
         raise ValueError(f"q must be [B, H_q, T, {cache.head_dim}], got {tuple(q.shape)}")
     b, hq, t, d = q.shape
@@ -70,6 +74,7 @@ def tree_attention(q: torch.Tensor, cache: KvCache, page_table: torch.Tensor, co
         q = q.clone(memory_format=torch.contiguous_format)
     code = L.dtype_code(q)
     with L.on_device(dev):
+        L.poll_give_ups(dev)
         o = torch.empty(b, hq, t, d, dtype=q.dtype, device=dev)
         lse = torch.empty(b, hq, t, dtype=torch.float32, device=dev)
         query = L.dcc_tree_query(q.data_ptr(), o.data_ptr(), lse.data_ptr(), *q.stride()[:3], *o.stride()[:3],

@@ -44,7 +44,7 @@ enum { DCC_F32 = 0, DCC_BF16 = 1, DCC_F64 = 2 };
 const char* dcc_status_string(int status);
 const char* dcc_last_error(void);
 /* ABI version: 2 added the initial state of dcc_attn_problem, 3 the decoding
- * entry points at the end of this file. */
+ * entry points at the end of this file, 4 dcc_device_error_report. */
 int dcc_version(void);
 /* sizeof of an ABI struct by its name ("dcc_query_set", "dcc_build_problem",
  * "dcc_kv_segment", "dcc_attn_problem", "dcc_rotary_tensor", "dcc_kv_pages",
@@ -257,9 +257,17 @@ int dcc_build_error_status(int clear);
  * counterpart in the reference, whose CPU path has no device waits; the
  * timeout maps to the RuntimeError style of comm.py:97-99. */
 int dcc_device_error_flags_async(unsigned int* host_flags, void* stream);
+/* Names a caller-owned pinned host word (NULL: none) to which calls of
+ * dcc_tree_attention on the current device, made from now on, write a non-zero
+ * value when a bounded wait of theirs gives up, beside the attention error word
+ * of dcc_device_error_status: a caller reads it before its next call without
+ * synchronising.  dcc_device_error_status clears it with its own.  The word has
+ * to outlive those calls, and the replays of graphs that captured them. */
+int dcc_device_error_report(unsigned int* host_word);
 /* Test hook for the error path: one warp waits `limit_ns` (at most 100 ms)
  * on an mbarrier that nothing arrives at, then records a timeout in the
- * attention error word -- a wait that runs out without any fault. */
+ * attention error word (and the word of dcc_device_error_report) -- a wait that
+ * runs out without any fault. */
 int dcc_debug_expire_wait(uint64_t limit_ns, void* stream);
 
 /* ---- online softmax ------------------------------------------------------

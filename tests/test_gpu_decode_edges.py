@@ -160,3 +160,60 @@ def test_many_small_weights_add_up(fmt, group):
     bound = (2 * 32 * 4 * ref.F32 + 2.0 ** -20) * a + ref.BF16 * want.abs() + n * 2.0 ** -31
     assert (want[:, 1] > 20 * n * 2.0 ** -31).all()
     within(o[:, :, 0], want.expand(b, group, 64), bound.expand(b, group, 64))
+
+
+# ---- waits that run out ------------------------------------------------------------------------------
+
+
+def test_a_wait_that_ran_out_reaches_a_program_that_only_decodes():
+    """An mbarrier nothing arrives at, 10 ms limit, no fault: the next call raises, the one after it is right again."""
+    from dcc_kv_b200 import _lib as L
+    g = gen(36)
+    cache, table = filled(g, "bf16", 1, 2, 64, 16, 400)
+    q = randn(g, 1, 8, 20, 64, dtype=torch.bfloat16)
+    want = dk.tree_attention(q, cache, table, lens(300))
+    cache.check()
+    for _ in range(2):
+        L.check(L.lib().dcc_debug_expire_wait(10_000_000, L.stream_ptr(dev())), "debug_expire_wait")
+        torch.cuda.synchronize()
+        with pytest.raises(L.DccError) as err:
+            dk.tree_attention(q, cache, table, lens(300))
+        assert err.value.status == L.DCC_ERR_TIMEOUT
+        got = dk.tree_attention(q, cache, table, lens(300))
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    L.check(L.lib().dcc_debug_expire_wait(10_000_000, L.stream_ptr(dev())), "debug_expire_wait")
+    with pytest.raises(L.DccError) as err:
+        cache.check()
+    assert err.value.status == L.DCC_ERR_TIMEOUT
+    cache.check()
+    got = dk.tree_attention(q, cache, table, lens(300))   # check() has reported and cleared it
+    assert torch.equal(got[0], want[0])
+
+
+def test_error_report_refusals():
+    from dcc_kv_b200 import _lib as L
+    word = torch.zeros(1, dtype=torch.int32)
+    assert L.lib().dcc_device_error_report(word.data_ptr()) in (L.DCC_ERR_INVALID_ARGUMENT, L.DCC_ERR_CUDA)
+    assert L.lib().dcc_device_error_report(word.cuda().data_ptr()) == L.DCC_ERR_INVALID_ARGUMENT
+
+
+def test_first_call_inside_a_capture():
+    """A process whose first attention is captured: nothing that a capture forbids is done."""
+    from dcc_kv_b200 import _lib as L
+    g = gen(37)
+    cache, table = filled(g, "int8", 1, 2, 64, 16, 400)
+    q, at = randn(g, 1, 8, 20, 64, dtype=torch.bfloat16), lens(300)
+    torch.cuda.synchronize()
+    saved = dict(L._reports)
+    L._reports.clear()
+    try:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            o, lse = dk.tree_attention(q, cache, table, at)
+        assert not L._reports
+    finally:
+        L._reports.update(saved)
+    graph.replay()
+    want = dk.tree_attention(q, cache, table, at)
+    assert torch.equal(o, want[0]) and torch.equal(lse, want[1])
+    cache.check()
