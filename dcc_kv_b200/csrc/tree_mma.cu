@@ -93,6 +93,13 @@ __device__ __forceinline__ void load_words(uint32_t a, uint32_t* w) {
   else
     asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];\n" : "=r"(w[0]), "=r"(w[1]) : "r"(a) : "memory");
 }
+template <int kWords>
+__device__ __forceinline__ void store_words(uint32_t a, const uint32_t* w) {
+  if constexpr (kWords == 4)
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(a), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+  else
+    asm volatile("st.shared.v2.b32 [%0], {%1, %2};\n" ::"r"(a), "r"(w[0]), "r"(w[1]) : "memory");
+}
 template <bool kHalf>
 __device__ __forceinline__ void mma(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
   if constexpr (kHalf)
@@ -557,9 +564,10 @@ __global__ void __launch_bounds__(Shape<kMode, kD, kNT>::kThreads, 1) tree_mma_k
         if (all) {
           weights(std::false_type{});
         } else {
-          if (!k8 && info.y + 15 >= 0 && guard) {
+          if (kMode != DCC_KV_INT8 && info.y + 15 >= 0 && guard) {
             // newest values that are not finite become zeros -- a row that does
             // not see them must not get 0 * inf --, and the rows that do, NaN
+            // (e4m3: the NaN code, which a pool may hold that was filled elsewhere)
             asm volatile("cp.async.wait_group %0;\n" ::"n"(2 * S - 2) : "memory");  // V of this chunk
             __syncwarp();
 #pragma unroll 1
@@ -568,15 +576,21 @@ __global__ void __launch_bounds__(Shape<kMode, kD, kNT>::kThreads, 1) tree_mma_k
               if (info.y + key < 0) continue;
               for (int c = 0; c < X::kVC; ++c) {
                 const uint32_t a = v_at[u & 1] + from + (u >> 1) * 8 * X::kRowBytes + 128 * c;
-                uint32_t x[4];
-                load_words<4>(a, x);
+                constexpr int kWords = X::kVB / 4;
+                uint32_t x[kWords];
+                load_words<kWords>(a, x);
+                const uint32_t was = broken;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  if ((x[e] & 0x7f80u) == 0x7f80u) x[e] &= 0xffff0000u, broken |= 1u << key;
-                  if ((x[e] & 0x7f800000u) == 0x7f800000u) x[e] &= 0x0000ffffu, broken |= 1u << key;
+                for (int e = 0; e < kWords; ++e) {
+                  if constexpr (k8) {
+                    const uint32_t nan = (((x[e] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;  // 1 in the bytes of 0x7f, 0xff
+                    if (nan) x[e] &= ~(nan * 255u), broken |= 1u << key;
+                  } else {
+                    if ((x[e] & 0x7f80u) == 0x7f80u) x[e] &= 0xffff0000u, broken |= 1u << key;
+                    if ((x[e] & 0x7f800000u) == 0x7f800000u) x[e] &= 0x0000ffffu, broken |= 1u << key;
+                  }
                 }
-                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(a), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3])
-                             : "memory");
+                if (broken != was) store_words<kWords>(a, x);
               }
             }
             broken = __reduce_or_sync(0xffffffffu, broken);

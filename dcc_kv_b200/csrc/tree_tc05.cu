@@ -439,11 +439,13 @@ __device__ __forceinline__ bool elected() {
 // bf16 value rows that do not exist hold whatever the page or the slot held,
 // and newest values that are not finite must not reach rows that do not see
 // them (0 * inf): both become zeros here; the softmax marks the rows that do
-// see the latter.  (8-bit codes are always finite.)
+// see the latter.  (int8 codes are always finite; e4m3 has a NaN code, which a
+// pool may hold that was filled elsewhere.)
 template <int kMode, int kD, bool kPair>
 __device__ __forceinline__ void clear_values(SmemOf<kMode, kD, kPair>& sm, uint32_t tile, int ring, bool newest, int64_t first,
                                              int lane) {
   constexpr int kPerRow = kD / 8, kRowsPer = 32 / kPerRow;
+  constexpr uint32_t kTop = kMode == DCC_KV_BF16 ? 0x7f80u : 0x7c00u;  // exponent of what is not finite, bf16 and fp16
   const int chunk = lane % kPerRow, sub = lane / kPerRow;
 #pragma unroll 1
   for (int r = sub; r < kTreeKeys; r += kRowsPer) {
@@ -456,8 +458,8 @@ __device__ __forceinline__ void clear_values(SmemOf<kMode, kD, kPair>& sm, uint3
       u[0] = v.x, u[1] = v.y, u[2] = v.z, u[3] = v.w;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        if ((u[c] & 0x7f80u) == 0x7f80u) u[c] &= 0xffff0000u;
-        if ((u[c] & 0x7f800000u) == 0x7f800000u) u[c] &= 0x0000ffffu;
+        if ((u[c] & kTop) == kTop) u[c] &= 0xffff0000u;
+        if ((u[c] & kTop << 16) == kTop << 16) u[c] &= 0x0000ffffu;
       }
     }
     st_shared_v4(a, u[0], u[1], u[2], u[3]);
@@ -508,13 +510,13 @@ __device__ __forceinline__ void issuer(const TreeParams& p, SmemOf<kMode, kD, kP
     tv.next(p, sm.span);
     wait_or_skip(ok, &sm.bar_full[X::kSlotsK + at_v.slot], at_v.use);
     const uint32_t tile = v0 + (uint32_t)at_v.slot * X::kTile;
-    if constexpr (!X::k8) {
+    if constexpr (kMode != DCC_KV_INT8) {
       const int ring = j % kRing;
       wait_or_skip(ok, &sm.bar_side[ring], (uint32_t)(j / kRing) & 1);
       const uint4 vis = *reinterpret_cast<const uint4*>(sm.vis[ring]);
       const int64_t first = (int64_t)tv.kt * kTreeKeys - tv.w.s.ctx;  // of the tile, behind the context
       const bool newest = guard && first + kTreeKeys > 0;
-      if ((vis.x & vis.y & vis.z & vis.w) != 0xffffffffu || newest)
+      if ((!X::k8 && (vis.x & vis.y & vis.z & vis.w) != 0xffffffffu) || newest)
         clear_values<kMode, kD, kPair>(sm, tile, ring, newest, first, lane);
     }
     return desc_at(tile, 16384);
@@ -677,21 +679,28 @@ __device__ __forceinline__ void softmax(const TreeParams& p, SmemOf<kMode, kD, k
           float bias = p.c.bias ? sm.side[ring][0][row] : 0.f;
           if (bias > -INFINITY && bias < INFINITY) bias = fminf(fmaxf(bias * kLog2e, -kMost), kMost);
           const int64_t i = i0 + row;
-          if (!X::k8 && guard && i >= 0 && i < w.s.cnt) {
+          float v_nan = 1.f;  // NaN for such an e4m3 row: a factor of its V scale
+          if (kMode != DCC_KV_INT8 && guard && i >= 0 && i < w.s.cnt) {
             // a newest value that is not finite: the rows that see it become NaN
-            // (8-bit rows that are not finite have a NaN scale)
+            // (a row that was not finite when it was quantised has a NaN scale)
             const PageWalk pages{p.q.page_table + w.b * p.q.table_stride, p.c.n_pages, p.c.page_size, p.q.max_pages};
             int off = 0;
             const int64_t page = pages.page_of(i + w.s.ctx, off);
             if (page >= 0) {
-              const uint4* v = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.c.v) +
-                                                              page_row(p.c, page, w.hk, off) * p.c.head_dim);
-              for (int c = 0; c < p.c.head_dim / 8; ++c) {
+              constexpr int kSize = X::k8 ? 1 : 2;
+              const uint4* v = reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(p.c.v) +
+                                                              page_row(p.c, page, w.hk, off) * p.c.head_dim * kSize);
+              for (int c = 0; c < p.c.head_dim * kSize / 16; ++c) {
                 const uint4 x = __ldg(v + c);
                 const uint32_t u[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  if ((u[e] & 0x7f80u) == 0x7f80u || (u[e] & 0x7f800000u) == 0x7f800000u) bias = __uint_as_float(0x7fc00000u);
+                for (int e = 0; e < 4; ++e) {
+                  if constexpr (X::k8) {
+                    if (((u[e] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) v_nan = __uint_as_float(0x7fc00000u);
+                  } else {
+                    if ((u[e] & 0x7f80u) == 0x7f80u || (u[e] & 0x7f800000u) == 0x7f800000u) bias = __uint_as_float(0x7fc00000u);
+                  }
+                }
               }
             }
           }
@@ -710,7 +719,7 @@ __device__ __forceinline__ void softmax(const TreeParams& p, SmemOf<kMode, kD, k
               v_exp = scale_exponent(fmaxf(fmaxf(sm.most[stream][0], sm.most[stream][1]), fmaxf(sm.most[stream][2], sm.most[stream][3])));
               if (row == 0) sm.up[stream] = v_exp;
             }
-            const float own_vs = sm.side[ring][2][row] * two_to(kWeightUp - v_exp), vs = fmaxf(own_vs, kLeastScale);
+            const float own_vs = sm.side[ring][2][row] * two_to(kWeightUp - v_exp) * v_nan, vs = fmaxf(own_vs, kLeastScale);
             sm.ks[stream][row] = sm.side[ring][1][row];
             sm.vs[stream][row] = own_vs < kLeastScale ? vs : own_vs;
             sm.lift[stream][row] = __log2f(vs) - kWeightUp + bias;

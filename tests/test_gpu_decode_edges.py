@@ -98,6 +98,30 @@ def test_a_nan_value_counts_however_small_its_weight(fmt, t, group, at, b):
     assert torch.isfinite(lse).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("t,group", ROWS[1:])
+@pytest.mark.parametrize("ctx,d", [(140, 64), (1000, 128), (129, 48)])
+def test_nan_codes_of_a_pool_filled_elsewhere(dtype, t, group, ctx, d):
+    """e4m3 has a NaN code, which write() never leaves: the newest rows that do not see it are unaffected."""
+    g = gen(38)
+    cache, table = filled(g, "e4m3", 1, 2, d, 16, ctx + t)
+    q = randn(g, 1, 2 * group, t, d, dtype=dtype)
+    mask = torch.eye(t, dtype=torch.bool, device=dev())
+    want = dk.tree_attention(q, cache, table, lens(ctx), tree=mask)
+    codes = cache.v.view(torch.uint8)
+    for at in (2, t - 1):
+        page, off = int(table[0, (ctx + at) // 16]), (ctx + at) % 16
+        keep = torch.tensor([i for i in range(t) if i != at], device=dev())
+        old = codes[page, :, off].clone()
+        for code, col in ((0x7f, 0), (0xff, 7), (0x7f, d - 1)):
+            codes[page, :, off, col] = code
+            got = dk.tree_attention(q, cache, table, lens(ctx), tree=mask)
+            assert torch.equal(got[0][:, :, keep], want[0][:, :, keep])
+            assert torch.equal(got[1][:, :, keep], want[1][:, :, keep])
+            assert torch.isnan(got[0][:, :, at, col]).all()
+            codes[page, :, off] = old
+
+
 # ---- attention: values of extreme size beside 8-bit codes, whose weights carry the V scale in fp16 ------
 
 
