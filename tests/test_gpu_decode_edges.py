@@ -186,6 +186,128 @@ def test_many_small_weights_add_up(fmt, group):
     within(o[:, :, 0], want.expand(b, group, 64), bound.expand(b, group, 64))
 
 
+# ---- attention: masks, for every number of rows at which another kernel takes the call --------------------
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "int8", "e4m3", "f32"])
+@pytest.mark.parametrize("t,group", ROWS[1:])
+@pytest.mark.parametrize("ctx", [140, 1000])
+def test_hidden_values_do_not_matter_for_any_number_of_rows(fmt, t, group, ctx):
+    """Rows behind the sequence, and drafted keys and values that a row does not see, in every kernel."""
+    g = gen(39)
+    hkv = 2
+    total = ctx + t + 54
+    cache, table = filled(g, fmt, 1, hkv, 64, 16, total)
+    q = randn(g, 1, hkv * group, t, 64, dtype=torch.bfloat16)
+    mask = torch.eye(t, dtype=torch.bool, device=dev())
+    want = dk.tree_attention(q, cache, table, lens(ctx), tree=mask)
+    ref.tree_close(want, ref.tree(q, cache, table, lens(ctx), mask=mask), 64, ctx + t)
+    poison = torch.full((1, hkv, 54, 64), math.nan, device=dev())
+    poison[:, :, ::2, 0] = math.inf
+    cache.write(poison, poison, table, ctx + t)
+    got = dk.tree_attention(q, cache, table, lens(ctx), tree=mask)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    for j in (2, t - 1):
+        keep = torch.tensor([i for i in range(t) if i != j], device=dev())
+        k0, v0 = cache.read(table, lens(ctx + j), 1, dtype=torch.float32)
+        for x in (math.nan, math.inf, -math.inf):
+            cache.write(torch.zeros(1, hkv, 1, 64, device=dev()), torch.full((1, hkv, 1, 64), x, device=dev()), table, ctx + j)
+            got = dk.tree_attention(q, cache, table, lens(ctx), tree=mask)
+            assert torch.equal(got[0][:, :, keep], want[0][:, :, keep])
+            assert not torch.isfinite(got[0][:, :, j]).any()
+            assert torch.equal(got[1][:, :, keep], want[1][:, :, keep])
+        cache.write(torch.full((1, hkv, 1, 64), math.nan, device=dev()), torch.zeros(1, hkv, 1, 64, device=dev()), table, ctx + j)
+        got = dk.tree_attention(q, cache, table, lens(ctx), tree=mask)
+        assert torch.equal(got[0][:, :, keep], want[0][:, :, keep]) and torch.isnan(got[0][:, :, j]).all()
+        cache.write(k0, v0, table, ctx + j)
+    assert_no_device_timeouts()
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "int8", "e4m3"])
+@pytest.mark.parametrize("t,group", [(1, 20), (1, 70), (1, 140), (1, 280)])
+def test_hidden_by_bias_for_any_number_of_rows(fmt, t, group):
+    """Single keys, whole tiles and all of them hidden by -inf or by the type's lowest value."""
+    g = gen(40)
+    lowest = torch.finfo(torch.float32).min
+    n = 900
+    cache, table = filled(g, fmt, 1, 1, 64, 16, n, bias=True)
+    q = randn(g, 1, group, 1, 64, dtype=torch.bfloat16)
+    k, v, b = cache.read(table, 0, n, dtype=torch.float32, logit_bias=True)
+    keep = b.clone()
+    at = lens(n - 1)
+    b[:, :, ::2] = lowest
+    cache.write(k, v, table, 0, logit_bias=b)
+    ref.tree_close(dk.tree_attention(q, cache, table, at), ref.tree(q, cache, table, at), 64, n)
+    b[:, :, ::2] = -math.inf
+    cache.write(k, v, table, 0, logit_bias=b)
+    seen = torch.arange(n, device=dev())[None] % 2 == 1
+    got = dk.tree_attention(q, cache, table, at)
+    cache.write(k, v, table, 0, logit_bias=torch.nan_to_num(b, neginf=0.0))
+    ref.tree_close(got, ref.tree(q, cache, table, at, seen_pos=seen), 64, n)
+    # only the first tiles hidden, or only the last
+    for lo, hi in ((0, 300), (128, 256), (600, n)):
+        for x in (lowest, -math.inf):
+            b = keep.clone()
+            b[:, :, lo:hi] = x
+            cache.write(k, v, table, 0, logit_bias=b)
+            got = dk.tree_attention(q, cache, table, at)
+            cache.write(k, v, table, 0, logit_bias=torch.nan_to_num(b, neginf=0.0))
+            s = torch.ones(1, n, dtype=torch.bool, device=dev())
+            if x == -math.inf:
+                s[:, lo:hi] = False
+            ref.tree_close(got, ref.tree(q, cache, table, at, seen_pos=s), 64, n)
+    b[:] = lowest
+    cache.write(k, v, table, 0, logit_bias=b)
+    o, lse = dk.tree_attention(q, cache, table, at)
+    vv = ref.cached(cache, table, 0, n)[1]
+    want, a = vv.mean(1), vv.abs().mean(1)
+    within(o[0, :, 0], want.expand(group, 64), ((n + 20) * ref.F32 + 2.0 ** -20) * a + 2 * ref.BF16 * a)
+    assert (lse == lowest).all()
+    b[:] = -math.inf
+    cache.write(k, v, table, 0, logit_bias=b)
+    o, lse = dk.tree_attention(q, cache, table, at)
+    assert (o == 0).all() and torch.isinf(lse).all()
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "int8", "e4m3"])
+@pytest.mark.parametrize("t,group", ROWS)
+@pytest.mark.parametrize("page", [16, 64, 24])
+def test_positions_without_a_page_for_any_number_of_rows(fmt, t, group, page):
+    g = gen(41)
+    n = 1200
+    cache, table = filled(g, fmt, 2, 2, 128, page, n)
+    per = table.shape[1]
+    q = randn(g, 2, 2 * group, t, 128, dtype=torch.bfloat16)
+    bad = table.clone()
+    bad[0, 2], bad[0, 9], bad[1, 0], bad[1, 5:8] = -1, cache.n_pages, 2147483647, -2147483648
+    seen = torch.ones(2, per * page, dtype=torch.bool, device=dev())
+    for s, i in ((0, 2), (0, 9), (1, 0), (1, 5), (1, 6), (1, 7)):
+        seen[s, i * page: (i + 1) * page] = False
+    ctx = lens(n - t, 701)
+    got = dk.tree_attention(q, cache, bad, ctx)
+    ref.tree_close(got, ref.tree(q, cache, table, ctx, seen_pos=seen), 128, n)
+    m = 3 * page
+    short = dk.tree_attention(q, cache, table[:, :3].contiguous(), lens(100, 48))
+    seen[:] = False
+    seen[:, :m] = True
+    ref.tree_close(short, ref.tree(q, cache, table, lens(100, 48), seen_pos=seen), 128, n)
+
+
+@pytest.mark.parametrize("fmt,dtype", [("bf16", torch.bfloat16), ("int8", torch.bfloat16), ("e4m3", torch.bfloat16), ("f32", torch.float32)])
+@pytest.mark.parametrize("t,group,b", [(4096, 8, 1), (1200, 16, 2)])
+@pytest.mark.parametrize("masked", [False, True])
+def test_more_row_tiles_than_a_grid_holds(fmt, dtype, t, group, b, masked):
+    """A prompt at once: every CTA takes several tiles of rows, one after the other."""
+    g = gen(42)
+    cache, table = filled(g, fmt, b, 1, 64, 16, 300 + t)
+    q = randn(g, b, group, t, 64, dtype=dtype)
+    mask = (torch.rand(t, t, generator=g, device=dev()) < 0.5) if masked else None
+    at = lens(*[300, 77][:b])
+    got = dk.tree_attention(q, cache, table, at, tree=mask)
+    ref.tree_close(got, ref.tree(q, cache, table, at, mask=mask), 64, 300 + t)
+    cache.check()
+
+
 # ---- waits that run out ------------------------------------------------------------------------------
 
 
