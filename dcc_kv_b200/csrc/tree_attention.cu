@@ -338,6 +338,8 @@ extern "C" int dcc_tree_attention(const dcc_kv_pages* cache, const dcc_tree_quer
   Workspace ws(workspace, workspace_bytes);
   tree_carve(p, ws);
   if (!workspace || !ws.ok()) return fail(DCC_ERR_WORKSPACE, "tree_attention: workspace too small");
+  if (reinterpret_cast<uintptr_t>(workspace) & 15u)  // the parts are stored and read 16 bytes at a time
+    return fail(DCC_ERR_INVALID_ARGUMENT, "tree_attention: the workspace must be 16-byte aligned");
   const int64_t items = (int64_t)q.n_seqs * cache->n_kv_heads * p.n_row_tiles;
   if (items > 2147483647LL) return fail(DCC_ERR_UNSUPPORTED, "tree_attention: too many sequences");
   cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -403,6 +403,7 @@ typedef struct dcc_tree_query {
   int32_t max_pages;
   int32_t reserved;
 } dcc_tree_query;
+/* The workspace starts on a 16-byte boundary. */
 size_t dcc_tree_attention_workspace_bytes(const dcc_kv_pages* cache, const dcc_tree_query* query, int dtype);
 int dcc_tree_attention(const dcc_kv_pages* cache, const dcc_tree_query* query, double scale, int dtype,
                        void* workspace, size_t workspace_bytes, void* stream);

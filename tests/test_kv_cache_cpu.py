@@ -37,3 +37,13 @@ def test_a_write_is_seen_by_a_backward_that_saved_the_pool(no_launch, fmt):
     assert all(x._version > n for x, n in zip(pools, before))
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.backward()
+
+
+def test_a_workspace_that_is_not_aligned_is_refused():
+    lib = L.lib()
+    pages = L.dcc_kv_pages(256, 256, 256, 256, None, 4, 16, 2, 64, L.DCC_KV_INT8)
+    query = L.dcc_tree_query(256, 256, None, 0, 0, 64, 0, 0, 64, 256, None, None, 0, 256, 4, 3, 1, 4, 4, 0)
+    need = lib.dcc_tree_attention_workspace_bytes(pages, query, L.DCC_BF16)
+    for at in (257, 264, 4096 + 4):
+        assert lib.dcc_tree_attention(pages, query, 0.125, L.DCC_BF16, at, need + 16, None) == L.DCC_ERR_INVALID_ARGUMENT
+        assert b"aligned" in lib.dcc_last_error()
