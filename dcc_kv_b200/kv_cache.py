@@ -131,7 +131,10 @@ class KvCache:
         written together."""
         b, t = self._check_rows(k, v)
         L.require_cuda(k, v, page_table)
-        k, v = (x.contiguous() if x.stride(3) != 1 else x for x in (k, v))
+        if k.stride(3) != 1:
+            k = k.contiguous()
+        if v.stride(3) != 1:
+            v = v.contiguous()
         if logit_bias is not None:
             if self.logit_bias is None:
                 raise ValueError("this cache holds no logit bias; make it with logit_bias=True")
@@ -139,12 +142,12 @@ class KvCache:
                 raise ValueError(f"logit_bias must be float32 {tuple(k.shape[:3])}")
             L.same_device(self.device, logit_bias=logit_bias)
             logit_bias = logit_bias.contiguous() if logit_bias.stride(2) != 1 else logit_bias
-        L.same_device(self.device, k=k, v=v)
-        with L.on_device(self.device):
+        dev = self.k.device
+        L.same_device(dev, k=k, v=v)
+        with L.on_device(dev):
             start = self._start(start, b)
             tok = self._tokens(k, v, logit_bias, page_table, start, counts, b, t)
-            L.check(L.lib().dcc_kv_cache_write(self._pages, tok, L.dtype_code(k), L.stream_ptr(self.device)),
-                    "kv_cache_write")
+            L.check(L.lib().dcc_kv_cache_write(self._pages, tok, L.dtype_code(k), L.stream_ptr(dev)), "kv_cache_write")
         L.written(self.k, self.v, self.k_scale, self.v_scale, self.logit_bias)
 
     def read(self, page_table: torch.Tensor, start: Union[int, torch.Tensor], length: int,

@@ -172,15 +172,19 @@ class Rotary:
         arr = (L.dcc_rotary_tensor * len(xs))()
         ys = []
         for i, x in enumerate(xs):
-            if x.stride(3) != 1 and d > 1:
+            sx = x.stride()
+            if sx[3] != 1 and d > 1:
                 x = x.contiguous()
+                sx = x.stride()
             if outs is not None:
-                y = outs[i]
+                y, sy = outs[i], sx
             else:
                 y = torch.empty_like(x)  # keeps the order of the axes, but not always a unit last stride of rows that overlap
-                if y.stride(3) != 1:
+                sy = y.stride()
+                if sy[3] != 1:
                     y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-            arr[i] = (x.data_ptr(), y.data_ptr(), *x.stride()[:3], *y.stride()[:3], x.shape[1])
+                    sy = y.stride()
+            arr[i] = (x.data_ptr(), y.data_ptr(), *sx[:3], *sy[:3], x.shape[1])
             ys.append(y)
         code = L.dtype_code(xs[0])
         ps = positions.stride() if positions.dim() == 2 else (0, positions.stride(0))
@@ -238,8 +242,13 @@ def _overlaps(x: torch.Tensor) -> bool:
 
 def _differentiated(xs) -> bool:
     """Autograd follows what happens to one of them, in reverse or forward mode."""
-    return (torch.is_grad_enabled() and any(x.requires_grad for x in xs)) or \
-        any(forward_ad.unpack_dual(x).tangent is not None for x in xs)
+    if torch.is_grad_enabled():
+        for x in xs:
+            if x.requires_grad:
+                return True
+    if forward_ad._current_level < 0:  # outside of every dual_level()
+        return False
+    return any(forward_ad.unpack_dual(x).tangent is not None for x in xs)
 
 
 class _RotaryFunction(torch.autograd.Function):
