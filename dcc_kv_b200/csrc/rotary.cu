@@ -6,10 +6,12 @@
 // formed in turns (position * turns_per_position, fp64) and reduced to
 // [-1/2, 1/2] turn before the fp32 sine and cosine: at position 2^20 an fp32
 // angle would be off by 0.06 rad, this one by 2e-7.
-// Measured: 32 + 8 heads of 128 in bf16, 32768 tokens, 112 us or 6.0 TB/s; in
-// fp32 with its gradient, 4097 tokens, 143 us or 4.7 TB/s (each way alone does not
-// outlast the launch of the next).  A single token of 64 sequences is bound by
-// its launch, 22 us with the Python call.
+// Measured: 32 + 8 heads of 128 in bf16, 32768 tokens, 112 us or 6.0 TB/s, with the
+// gradient 221; 2 x 4097 tokens with the gradient, in a graph, fp32 112 us or 6.0 TB/s,
+// bf16 68 or 5.0 (as calls 145 to 150, which is the host's part of autograd).  Rows that are
+// not 16-byte aligned, 20 heads of 32768 tokens: bf16 135 us (aligned 66), fp32 147
+// (118), fp64 220 (212).  A single token of 64 sequences takes 3 us in a graph, 21
+// with the Python call.
 #include <algorithm>
 #include <string>
 

@@ -13,11 +13,12 @@ constexpr int kSimtCtasPerSm = 6;
 
 // Online softmax over key tiles of 128: thread = key for the scores (q rows
 // from shared memory), thread = column for the values.  fp32 throughout.
-// Bound by instruction issue (2 fused multiply-adds per row, key and column);
-// it serves fp32 queries and caches and the head_dims and page sizes that the
+// Bound by its loads of keys: a warp's 32 lanes read single elements a row apart,
+// so that 2/3 of the time is waiting for them (19 % of the issue slots are used).
+// It serves fp32 queries and caches and the head_dims and page sizes that the
 // tensor-core kernels do not take.  16 sequences, 4 heads on each of 8 KV heads
-// of 128, 8k tokens: 1161 us beside a bf16 cache whose pages hold 12 tokens,
-// where 16-token pages take tree_mma.cu 105 us.
+// of 128, 8k tokens: 1110 us beside a bf16 cache whose pages hold 12 tokens or
+// one, where 16-token pages take tree_mma.cu 102 us; 1165 us beside fp32.
 template <typename T, int kFormat>
 __global__ void __launch_bounds__(kSimtThreads) tree_simt_kernel(const __grid_constant__ TreeParams p) {
   constexpr bool kScaled = kFormat == DCC_KV_INT8 || kFormat == DCC_KV_E4M3;
@@ -250,7 +251,8 @@ bool tree_tensor_supported(const dcc_kv_pages& c, const dcc_tree_query& q, int d
 // Which kernel takes a call, with how many query rows per KV head at a time.
 // Up to 16 rows the warps of tree_mma.cu, which pay per 8 rows, are ahead of
 // the tensor core tiles of tree_tc05.cu, which pay for 128 or 256 whatever the
-// number is; above they are behind (16 sequences, 8 KV heads of 128, us):
+// number is (beside 16 bf16 rows they are level); above they are behind (16
+// sequences, 8 KV heads of 128, us):
 //   rows  tokens  int8 mma / tc05   bf16 mma / tc05
 //      8    8192       82 / 159         107 / 115
 //     16    8192      112 / 160         116 / 114

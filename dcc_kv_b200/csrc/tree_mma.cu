@@ -22,16 +22,20 @@
 // range is under 2^-39 of that element.
 // Each warp keeps a running max that moves when a score passes it by 2^8, its
 // sums and O in registers; the warps are added up at the end of a piece.  P is
-// rounded once, to bf16 beside bf16 values (a relative 2^-9 of each weight), to
-// fp16 beside codes (2^-12): there P carries the V scale, so the max is taken
+// rounded once, to bf16 beside bf16 values (a relative 2^-8 of each weight), to
+// fp16 beside codes (2^-11): there P carries the V scale, so the max is taken
 // over score + log2(scale), in units that keep it below 2^14 (kWeightUp in
 // tree_attention.cuh; below 2^-20 of the largest fp16 is subnormal and holds P
 // to 2^-31 of that).
 // Measured: 16 sequences of 8192 tokens, 4 query heads on each of 8 KV heads of
-// 128: int8 75 us or 3.7 TB/s, e4m3 85 us, bf16 105 us or 5.1 TB/s; with 16 rows
-// per KV head 112 and 116 us.  8-bit codes are bound by the issue of their
-// widening, 560 to 600 instructions a warp and 16 keys; lines of 512 bytes a copy
-// instead of one row a lane took a quarter off.
+// 128: int8 73 us or 3.8 TB/s, e4m3 83 us, bf16 102 us or 5.3 TB/s; with 16 rows
+// per KV head int8 108, bf16 113 us.  Beside 8-bit codes the bound is the latency
+// of the widening's dependent chains with three warps a scheduler (the registers
+// allow no more, and 16 warps were slower, 81 against 75 us): 550 to 600
+// instructions a warp and 16 keys fill 51 to 56 % of the issue slots.  Lines of 512
+// bytes a copy instead of one row a lane took a quarter off; heads of 96, which
+// are copied row by row and padded to 128 columns, take 87 us (int8) and 86 (bf16)
+// for three quarters of the bytes, heads of 64 take 60 (int8).
 #include <string>
 #include <type_traits>
 

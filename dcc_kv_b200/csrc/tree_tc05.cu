@@ -30,14 +30,14 @@
 // and every role sees every use of the barriers that it waits on.
 // The running max of a row moves (with O and the sums rescaled) only when a
 // score passes it by 2^8.  P is rounded once for its MMA, to bf16 beside bf16
-// values (a relative 2^-9 of each weight) and to fp16 beside 8-bit ones (2^-12):
+// values (a relative 2^-8 of each weight) and to fp16 beside 8-bit ones (2^-11):
 // there P carries the V scale, so the max is taken over score + log2(scale), in
 // units that keep P below 2^14 (kWeightUp in tree_attention.cuh; below 2^-20 of
 // the largest fp16 is subnormal and holds P to 2^-31 of that).
 //
 // Measured (8 KV heads of 128, 4 query heads each): 64 tokens over 131072, bf16,
-// 193 us or 710 TFLOP/s; int8, 290 us; 13 tokens of 16 sequences over 4001, int8,
-// 100 us; bf16 77 us.  Neither memory nor tensor cores are full: what bounds it
+// 182 us or 756 TFLOP/s; int8, 292 us; 13 tokens of 16 sequences over 4001, int8,
+// 96 us; bf16 73 us.  Neither memory nor tensor cores are full: what bounds it
 // is the chain scores -> weights -> values -> next scores of a stream (its scores
 // and weights share TMEM) and the instruction cache, which all roles share.
 //

@@ -25,7 +25,7 @@ class KvCache:
     """Pages of ``page_size`` tokens of every KV head.  ``k``, ``v``
     [n_pages, H_kv, page_size, d] hold codes; int8 and e4m3 codes have one
     float32 scale per token and KV head in ``k_scale``, ``v_scale``
-    [n_pages, H_kv, page_size] (value = code * scale).  ``logit_bias``, of the
+    [n_pages, H_kv, page_size] (value = code * scale, scale >= 0).  ``logit_bias``, of the
     scales' shape, is added to the logits of a key, as for compact keys.
     Which pages a sequence owns is the caller's: every call takes a page table
     [B, max_pages] (int32), position p of a sequence being row p % page_size
@@ -153,8 +153,8 @@ class KvCache:
     def read(self, page_table: torch.Tensor, start: Union[int, torch.Tensor], length: int,
              counts: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.bfloat16,
              logit_bias: bool = False) -> Tuple[torch.Tensor, ...]:
-        """The values (code * scale, rounded once to ``dtype``, bfloat16 or
-        float32) of positions start[s] .. start[s] + length: (k, v)
+        """The values (code * scale in float32, then rounded to ``dtype``,
+        bfloat16 or float32) of positions start[s] .. start[s] + length: (k, v)
         [B, H_kv, length, d], and the logit bias [B, H_kv, length] when asked
         for.  Zeros where a sequence has no page and behind counts[s]."""
         if dtype not in (torch.bfloat16, torch.float32):

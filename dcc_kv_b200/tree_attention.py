@@ -45,9 +45,9 @@ def tree_attention(q: torch.Tensor, cache: KvCache, page_table: torch.Tensor, co
     reads KV head h // (H_q // H_kv); the cache's logit bias is added to the
     logits; ``scale`` defaults to 1 / sqrt(d).
 
-    Returns (O [B, H_q, T, d] in q's dtype, LSE [B, H_q, T] float32), as
-    :func:`~dcc_kv_b200.attention` does: :func:`~dcc_kv_b200.merge_lse` joins
-    it with attention over other keys.  A row that sees nothing, and the rows
+    Returns (O [B, H_q, T, d] in q's dtype, LSE [B, H_q, T] float32), without
+    gradients, as :func:`~dcc_kv_b200.attention` does:
+    :func:`~dcc_kv_b200.merge_lse` joins it with attention over other keys.  A row that sees nothing, and the rows
     behind counts[s], give O = 0 and LSE = -inf.
 
     Waits inside the kernels are bounded: one that gave up leaves the call's

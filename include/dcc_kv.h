@@ -328,8 +328,8 @@ int dcc_rotary(const dcc_rotary_tensor* tensors, int n_tensors, const void* posi
  *     rounded to nearest even and clamped to +-127
  *   DCC_KV_E4M3: scale = the smallest power of two >= amax / 448, at least
  *     2^-96, code = e4m3(x / scale), rounded to nearest even
- *   DCC_KV_BF16, DCC_KV_F32: code = x.
- * A quantised row with an infinity or NaN gets scale NaN and zero codes, so
+ *   DCC_KV_BF16, DCC_KV_F32: code = x (rounded to nearest even).
+ * Scales are not negative.  A quantised row with an infinity or NaN gets scale NaN and zero codes, so
  * all of it reads as NaN.  head_dim <= 128. */
 enum { DCC_KV_BF16 = 0, DCC_KV_F32 = 1, DCC_KV_INT8 = 2, DCC_KV_E4M3 = 3 };
 typedef struct dcc_kv_pages {
@@ -370,7 +370,7 @@ typedef struct dcc_kv_tokens {
 /* Quantises tokens into the cache.  Two tokens of one call at the same row
  * leave that row undefined.  tokens->bias NULL writes a zero bias. */
 int dcc_kv_cache_write(const dcc_kv_pages* cache, const dcc_kv_tokens* tokens, int dtype, void* stream);
-/* Reads tokens back: code * scale rounded once to `dtype`. */
+/* Reads tokens back: code * scale in float, then rounded to `dtype`. */
 int dcc_kv_cache_read(const dcc_kv_pages* cache, const dcc_kv_tokens* tokens, int dtype, void* stream);
 
 /* Attention of the T newest tokens of each sequence over its cached ones.
@@ -384,7 +384,8 @@ int dcc_kv_cache_read(const dcc_kv_pages* cache, const dcc_kv_tokens* tokens, in
  * `dtype` (DCC_BF16 or DCC_F32), lse [n_seqs, n_q_heads, T] contiguous or NULL.
  * Query head h reads KV head h / (n_q_heads / n_kv_heads).  T <= 4096.
  * A row that sees a key or value with an infinity or NaN is not finite;
- * rows that do not see it are unaffected. */
+ * rows that do not see it are unaffected.  Beside int8 and e4m3 codes and bf16
+ * queries, a sequence's V scales may differ by a factor of 2^90. */
 typedef struct dcc_tree_query {
   const void* q;
   void* o;
