@@ -61,12 +61,15 @@ __device__ __forceinline__ bool tree_sees(const TreeParams& p, int b, int64_t t,
 // Where weights are held in fp16 (beside 8-bit codes) they carry the V scale, in
 // units of 2^(e - 6) with e the exponent of the largest V scale of the first
 // keys of a part (0 where those have none): the first weights are below 2^7
-// whatever the values' size, also where the scores are so large (biases of the
-// type's lowest value) that a logarithm added to them is lost, and six bits
-// more of small weights are kept.  2^8 on, where the running max has to move,
-// fp16 still reaches.  (Scales of one sequence that differ by more than 2^90 are
-// beyond this.)
+// whatever the values' size, and six bits more of small weights are kept.  2^8
+// on, where the running max has to move, fp16 still reaches.  (Scales of one
+// sequence that differ by more than 2^90 are beyond this.)
+// Scores beyond kHuge, biases of a mask, do not hold a logarithm added to them (a
+// row of zeros has the scale 2^-96: -1e9 - 96 is -1e9 - 128 in fp32, and the weight
+// 2^128): there the max is taken of the scores alone, and of such a key's V scale
+// no more than kMostHuge counts, so that rows which see nothing else stay finite.
 constexpr int kWeightUp = 6;
+constexpr float kHuge = 16777216.f, kMostHuge = 8192.f;
 constexpr float kLeastScale = 5.048709793e-29f;  // 2^-94, in those units: rows that were never written have scale 0
 constexpr float kMostScale = 3.402823466e38f;
 __device__ __forceinline__ int scale_exponent(float largest) {

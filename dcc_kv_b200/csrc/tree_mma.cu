@@ -498,6 +498,7 @@ __global__ void __launch_bounds__(Shape<kMode, kD, kNT>::kThreads, 1) tree_mma_k
             ks[u] = load_one(ring_side + from + 64 + 32 * u + 4 * g);
             vs[u] = load_one(ring_side + from + 128 + 32 * u + 4 * g) * v_unit;
             vs[u] = vs[u] < kLeastScale ? kLeastScale : vs[u];
+            if (p.c.bias && fabsf(bias[u]) >= kHuge) vs[u] = vs[u] > kMostHuge ? kMostHuge : vs[u];
           }
         }
         uint32_t pr[kNT][2];
@@ -543,7 +544,8 @@ __global__ void __launch_bounds__(Shape<kMode, kD, kNT>::kThreads, 1) tree_mma_k
                 for (int u = 0; u < 2; ++u) {
                   float x = s[m][2 * u + h];
                   // (a NaN scale is not to move the max: it makes the row NaN by its product)
-                  if constexpr (k8) x += log2f(fminf(fmaxf(vs[u], kLeastScale), kMostScale)) - kWeightUp;
+                  if constexpr (k8)
+                    if (fabsf(x) < kHuge) x += log2f(fminf(fmaxf(vs[u], kLeastScale), kMostScale)) - kWeightUp;
                   if (seen(2 * u + h)) top = fmaxf(top, x);
                 }
 #pragma unroll

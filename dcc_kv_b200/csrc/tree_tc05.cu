@@ -721,8 +721,9 @@ __device__ __forceinline__ void softmax(const TreeParams& p, SmemOf<kMode, kD, k
             }
             const float own_vs = sm.side[ring][2][row] * two_to(kWeightUp - v_exp) * v_nan, vs = fmaxf(own_vs, kLeastScale);
             sm.ks[stream][row] = sm.side[ring][1][row];
-            sm.vs[stream][row] = own_vs < kLeastScale ? vs : own_vs;
-            sm.lift[stream][row] = __log2f(vs) - kWeightUp + bias;
+            const bool huge = fabsf(bias) >= kHuge;
+            sm.vs[stream][row] = own_vs < kLeastScale ? vs : huge && own_vs > kMostHuge ? kMostHuge : own_vs;
+            sm.lift[stream][row] = huge ? bias : __log2f(vs) - kWeightUp + bias;
           }
           group_sync(stream);
         }

@@ -146,6 +146,34 @@ def test_biases_at_the_lowest_value_beside_values_of_any_size(fmt, group, b, siz
     assert torch.isfinite(lse).all()
 
 
+@pytest.mark.parametrize("fmt", ["bf16", "int8", "e4m3"])
+@pytest.mark.parametrize("t,group", ROWS)
+@pytest.mark.parametrize("b", [1, 160])
+@pytest.mark.parametrize("low", [torch.finfo(torch.float32).min, -1e9, -1e8, -3e7, -1e4])
+@pytest.mark.parametrize("written", [True, False])
+def test_padding_of_zeros_hidden_by_a_large_bias(fmt, t, group, b, low, written):
+    """Padded keys whose values are zeros (or were never written: scale 0), whole tiles and single ones."""
+    g = gen(43)
+    n = 900
+    pad = torch.zeros(n, dtype=torch.bool, device=dev())
+    pad[:200] = pad[300:433] = pad[512:640] = pad[700:860:2] = True
+    k, v, bias = randn(g, 1, 1, n, 64), randn(g, 1, 1, n, 64) * 2.0 ** 12, randn(g, 1, 1, n)
+    v[:, :, pad] = 0
+    bias[:, :, pad] = low
+    cache, table = packed(g, fmt, b, 64, n, k, v, bias=bias)
+    if not written and cache.v_scale is not None:
+        cache.v_scale.view(-1)[:n][pad] = 0
+    q = randn(g, 1, group, t, 64, dtype=torch.bfloat16)
+    o, lse = dk.tree_attention(q.expand(b, group, t, 64), cache, table, lens(*[n - t] * b))
+    want = ref.tree(q, cache, table, lens(n - t))
+    for s in (0, b // 2, b - 1):
+        ref.tree_close((o[s: s + 1], lse[s: s + 1]), want, 64, n)
+    # only padding is seen: zeros, and the log-sum-exp of the padding
+    o, lse = dk.tree_attention(q.expand(b, group, t, 64), cache, table, lens(*[100] * b))
+    assert (o == 0).all() and torch.isfinite(lse).all()
+    within(lse, torch.full_like(lse, low).double(), 2.0 ** -23 * abs(low) + 100.0)
+
+
 @pytest.mark.parametrize("fmt", ["int8", "e4m3"])
 @pytest.mark.parametrize("t,group", ROWS)
 @pytest.mark.parametrize("b", [1, 160])
