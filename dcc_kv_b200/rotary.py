@@ -170,11 +170,12 @@ class Rotary:
         dev = xs[0].device
         b, _, t, d = xs[0].shape
         arr = (L.dcc_rotary_tensor * len(xs))()
-        ys = []
+        ys, held = [], []  # held: copies that the launch reads stay until it is made
         for i, x in enumerate(xs):
             sx = x.stride()
             if sx[3] != 1 and d > 1:
                 x = x.contiguous()
+                held.append(x)
                 sx = x.stride()
             if outs is not None:
                 y, sy = outs[i], sx

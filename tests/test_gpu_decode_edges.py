@@ -51,6 +51,23 @@ def test_hand_over_on_another_stream_behind_a_host_forward():
             assert torch.equal(got[0], want[nb - 1])
 
 
+# ---- rotary ------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("t", [1, 5, 300])
+def test_rotary_of_queries_with_another_last_stride(dtype, t):
+    """The copy that is made of them must live until the launch, beside results and copies of its size."""
+    g = gen(44)
+    rot = dk.Rotary(64)
+    pos = torch.arange(t, device=dev()) + 5000
+    for _ in range(8):
+        q = randn(g, 64, 2, 3, t, dtype=dtype).permute(1, 2, 3, 0)
+        for k in (randn(g, 2, 3, t, 64, dtype=dtype), randn(g, 64, 2, 3, t, dtype=dtype).permute(1, 2, 3, 0)):
+            a, b = rot(q, pos, k)
+            assert torch.equal(a, rot(q.contiguous(), pos)) and torch.equal(b, rot(k.contiguous(), pos))
+
+
 # ---- attention: values that are not finite -----------------------------------------------------------
 
 

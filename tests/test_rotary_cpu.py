@@ -140,3 +140,29 @@ def test_inplace_refuses_what_overlaps_itself(on_the_cpu):
                            ((2, 3, 4, 64), (768, 64, 192, 1))):
         x = torch.as_strided(base, shape, strides)
         assert rot(x, torch.arange(shape[2]), inplace=True) is x
+
+
+def test_copies_of_strided_inputs_live_until_the_launch(monkeypatch):
+    """Of queries with another last stride a copy is made; the results of the keys must not take its place."""
+    import ctypes as C
+    seen = []
+
+    class Library:
+        def dcc_rotary(self, arr, n, *rest):
+            seen.append([torch.frombuffer(bytearray(C.string_at(t.x, 4 * 64 * 5)), dtype=torch.float32) for t in arr])
+            for t in arr:  # what a launch does at once on the CPU
+                C.memset(t.y, 0, 4 * 64 * 5)
+            return L.DCC_OK
+
+    monkeypatch.setattr(L, "lib", Library)
+    monkeypatch.setattr(L, "require_cuda", lambda *tensors: None)
+    monkeypatch.setattr(L, "stream_ptr", lambda device: 0)
+    monkeypatch.setattr(L, "on_device", lambda device: torch.no_grad())
+    real = torch.empty_like
+    monkeypatch.setattr(torch, "empty_like", lambda x, **kw: real(x, **kw).fill_(-1))
+    rot = dk.Rotary(64)
+    for _ in range(8):
+        q, k = (torch.randn(64, 1, 1, 5).permute(1, 2, 3, 0) for _ in range(2))
+        rot(q, torch.arange(5), k)
+        for got, x in zip(seen[-1], (q, k)):
+            assert torch.equal(got, x.flatten())
