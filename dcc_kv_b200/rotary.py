@@ -25,7 +25,8 @@ _LAYOUTS = {"half": L.DCC_ROTARY_HALF, "interleaved": L.DCC_ROTARY_INTERLEAVED}
 # what each kind of scaling reads; the first ones may stand beside any of them
 _KEYS = {"": ("rope_type", "type", "rope_theta", "partial_rotary_factor", "original_max_position_embeddings"),
          "default": (), "linear": ("factor",), "ntk": ("factor",),
-         "yarn": ("factor", "beta_fast", "beta_slow", "truncate", "attention_factor", "mscale", "mscale_all_dim"),
+         # ("finetuned" says how a model was made, not how it turns)
+         "yarn": ("factor", "beta_fast", "beta_slow", "truncate", "attention_factor", "mscale", "mscale_all_dim", "finetuned"),
          "llama3": ("factor", "low_freq_factor", "high_freq_factor")}
 
 

@@ -353,6 +353,77 @@ def test_more_row_tiles_than_a_grid_holds(fmt, dtype, t, group, b, masked):
     cache.check()
 
 
+@pytest.mark.parametrize("fmt", ["bf16", "int8", "e4m3", "f32"])
+def test_pools_whose_offsets_pass_32_bits(fmt):
+    """Pages at the end of a pool of more than 2^32 elements hold, and give, what those of a small pool do."""
+    g = gen(45)
+    h, d, page, per = 8, 128, 16, 40
+    n_pages = 2 ** 32 // (h * d * page) + 2 * per
+    tables = [torch.arange(n, dtype=torch.int32, device=dev()).flip(0).view(2, per) for n in (2 * per,)]
+    tables.append(tables[0] + (n_pages - 2 * per))
+    caches = [dk.KvCache.empty(n, page, h, d, fmt, device=dev()) for n in (2 * per, n_pages)]
+    k, v = randn(g, 2, h, 600, d), randn(g, 2, h, 600, d)
+    q = randn(g, 2, 4 * h, 20, d, dtype=torch.bfloat16)
+    got = []
+    for cache, table in zip(caches, tables):
+        cache.write(k, v, table, lens(0, 20))
+        got.append([*cache.read(table, lens(0, 20), 600, dtype=torch.float32),
+                    *dk.tree_attention(q[:, :, :1], cache, table, lens(599, 300)),
+                    *dk.tree_attention(q, cache, table, lens(580, 300)),
+                    *dk.tree_attention(q[:, :, :2].float(), cache, table, lens(580, 300))])
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+
+
+def test_rotary_of_more_than_32_bits_of_bytes():
+    rot = dk.Rotary(128)
+    t = 2 ** 19 + 33
+    x = torch.empty(1, 34, t, 128, dtype=torch.bfloat16, device=dev()).normal_(generator=gen(46))
+    pos = torch.arange(t, device=dev())
+    y = rot(x, pos)
+    for cut in (slice(0, 7), slice(t - 7, t)):
+        assert torch.equal(y[:, :, cut], rot(x[:, :, cut].contiguous(), pos[cut]))
+
+
+# ---- together ----------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "int8"])
+def test_a_decoding_step_as_a_graph(fmt):
+    """Rotary positions, cache write and attention captured once; lengths and tokens change under the replays."""
+    g = gen(47)
+    b, hq, hkv, d = 3, 8, 2, 128
+    rot = dk.Rotary(d, theta=500000.0)
+    caches = [dk.KvCache.empty(60, 16, hkv, d, fmt, device=dev()) for _ in range(2)]
+    table = torch.randperm(60, generator=g, device=dev())[:45].to(torch.int32).view(b, 15)
+    k, v = (randn(g, b, hkv, 200, d, dtype=torch.bfloat16) for _ in range(2))
+    for cache in caches:
+        cache.write(k, v, table, 0)
+    x = [randn(g, b, h, 1, d, dtype=torch.bfloat16) for h in (hq, hkv, hkv)]
+    at = lens(200, 128, 77)
+
+    def step(cache):
+        q, k = rot(x[0], at[:, None], x[1])
+        cache.write(k, x[2], table, at)
+        return dk.tree_attention(q, cache, table, at)
+
+    graph = torch.cuda.CUDAGraph()
+    step(caches[0])
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        o, lse = step(caches[0])
+    for _ in range(5):
+        for t in x:
+            t.normal_(generator=g)
+        graph.replay()
+        want = step(caches[1])
+        assert torch.equal(o, want[0]) and torch.equal(lse, want[1])
+        at += 1
+    for a, c in zip(caches[0].read(table, 0, 240), caches[1].read(table, 0, 240)):
+        assert torch.equal(a, c)
+    caches[0].check()
+
+
 # ---- waits that run out ------------------------------------------------------------------------------
 
 
