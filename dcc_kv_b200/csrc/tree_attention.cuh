@@ -201,6 +201,53 @@ __device__ __forceinline__ T* tree_out_row(const TreeParams& p, int b, const Tre
   return static_cast<T*>(p.q.o) + b * p.q.o_seq_stride + r.h * p.q.o_head_stride + r.t * p.q.o_row_stride;
 }
 
+// ---- what both tensor-core kernels are made of ----
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, uint32_t size) {  // 16 bytes; of size < 16 the rest are zeros
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(size) : "memory");
+}
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <bool kHalf>
+__device__ __forceinline__ uint32_t pack(float lo, float hi) {
+  if constexpr (kHalf) {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  } else {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+}
+
+// int8 code in the low byte of each half, 0x64 above it and its sign flipped:
+// the fp16 number 1024 + 128 + code
+__device__ __forceinline__ uint32_t less_1152(uint32_t y) {
+  const __half2 off = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
+  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&y), off);
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t from_e4m3(uint32_t two) {
+  const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3);
+  return (uint32_t)r.x | (uint32_t)r.y << 16;
+}
+// Codes 0, 1 and 2, 3 of a word as two pairs of fp16.
+template <int kMode>
+__device__ __forceinline__ void widen_word(uint32_t w, uint32_t& b0, uint32_t& b1) {
+  if constexpr (kMode == DCC_KV_INT8) {
+    const uint32_t u = w ^ 0x80808080u;
+    b0 = less_1152(__byte_perm(u, 0x64646464u, 0x4140));
+    b1 = less_1152(__byte_perm(u, 0x64646464u, 0x4342));
+  } else {
+    b0 = from_e4m3(w & 0xffffu);
+    b1 = from_e4m3(w >> 16);
+  }
+}
+
 // The tensor-core kernels: bf16 queries, bf16 or 8-bit cache, head_dim a
 // multiple of 16, page_size of 8.  tree_mma.cu for up to 16 rows per KV head,
 // tree_tc05.cu for more.

@@ -84,12 +84,6 @@ struct Smem {
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
-__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, uint32_t size) {  // size < 16: zeros follow
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(size) : "memory");
-}
-__device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src) : "memory");
-}
 template <int kWords>
 __device__ __forceinline__ void load_words(uint32_t a, uint32_t* w) {
   if constexpr (kWords == 4)
@@ -127,45 +121,6 @@ __device__ __forceinline__ float load_one(uint32_t a) {
   float v;
   asm volatile("ld.shared.f32 %0, [%1];\n" : "=f"(v) : "r"(a) : "memory");
   return v;
-}
-__device__ __forceinline__ float exp2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-template <bool kHalf>
-__device__ __forceinline__ uint32_t pack(float lo, float hi) {
-  if constexpr (kHalf) {
-    const __half2 v = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&v);
-  } else {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&v);
-  }
-}
-
-// int8 code in the low byte of each half, 0x64 above it and its sign flipped:
-// the fp16 number 1024 + 128 + code
-__device__ __forceinline__ uint32_t less_1152(uint32_t y) {
-  const __half2 off = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
-  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&y), off);
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-__device__ __forceinline__ uint32_t from_e4m3(uint32_t two) {
-  const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3);
-  return (uint32_t)r.x | (uint32_t)r.y << 16;
-}
-// Codes 0, 1 and 2, 3 of a word as two pairs of fp16.
-template <int kMode>
-__device__ __forceinline__ void widen_word(uint32_t w, uint32_t& b0, uint32_t& b1) {
-  if constexpr (kMode == DCC_KV_INT8) {
-    const uint32_t u = w ^ 0x80808080u;
-    b0 = less_1152(__byte_perm(u, 0x64646464u, 0x4140));
-    b1 = less_1152(__byte_perm(u, 0x64646464u, 0x4342));
-  } else {
-    b0 = from_e4m3(w & 0xffffu);
-    b1 = from_e4m3(w >> 16);
-  }
 }
 // Code `q` of a and of b as a pair of fp16.
 template <int kMode>

@@ -143,27 +143,10 @@ __device__ __forceinline__ bool wait_all_lanes(uint64_t* bar, uint32_t parity) {
 __device__ __forceinline__ void wait_or_skip(bool& ok, uint64_t* bar, uint32_t parity) {
   if (ok) ok = wait_all_lanes(bar, parity);
 }
-__device__ __forceinline__ float exp2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<uint32_t*>(&v);
-}
-__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
-  __half2 v = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<uint32_t*>(&v);
-}
 __device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 3, 256;\n" ::: "memory"); }
 __device__ __forceinline__ void group_sync(int wg) { asm volatile("bar.sync %0, 128;\n" ::"r"(1 + wg) : "memory"); }
-template <int kBytes>
-__device__ __forceinline__ void cp_async(uint32_t dst, const void* src, uint32_t size) {  // size < kBytes: zeros follow
-  if constexpr (kBytes == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(size) : "memory");
-  else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(dst), "l"(src), "r"(size) : "memory");
+__device__ __forceinline__ void copy_async_word(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(dst), "l"(src) : "memory");
 }
 // Arrives (counted beforehand) once this thread's cp.async so far have landed.
 __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
@@ -173,27 +156,6 @@ __device__ __forceinline__ uint4 ld_shared_v4(uint32_t a) {
   uint4 v;
   asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
   return v;
-}
-
-// Four 8-bit codes to four fp16 (two per word), exactly.
-template <int kMode>
-__device__ __forceinline__ uint2 widen(uint32_t w) {
-  if constexpr (kMode == DCC_KV_INT8) {
-    const uint32_t u = w ^ 0x80808080u;  // code + 128
-    const __half2 off = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));  // 1152
-    uint32_t o[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const uint32_t y = __byte_perm(u, 0x64646464u, i ? 0x4342 : 0x4140);  // 0x6400 | u = 1024 + u
-      const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&y), off);
-      o[i] = *reinterpret_cast<const uint32_t*>(&r);
-    }
-    return make_uint2(o[0], o[1]);
-  } else {
-    const __half2_raw lo = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3);
-    const __half2_raw hi = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> 16), __NV_E4M3);
-    return make_uint2((uint32_t)lo.x | (uint32_t)lo.y << 16, (uint32_t)hi.x | (uint32_t)hi.y << 16);
-  }
 }
 
 // A place of the ring and the parity of its current use.
@@ -286,7 +248,7 @@ __device__ __forceinline__ void copies(const TreeParams& p, const TreeMaps& maps
       if (left[kFetch - 1] > 0) {
         const int s = pow2 ? pos >> shift : pos / p.c.page_size;
         add[kFetch - 1] = t.w.hk * p.c.page_size + pos - s * p.c.page_size;
-        cp_async<4>(smem_u32(&sm.pages[is_v][fetched % kFetch][lane]), p.q.page_table + (int64_t)t.w.b * p.q.table_stride + s, 4);
+        copy_async_word(smem_u32(&sm.pages[is_v][fetched % kFetch][lane]), p.q.page_table + (int64_t)t.w.b * p.q.table_stride + s);
       }
       ++fetched;
     }
@@ -330,10 +292,10 @@ __device__ __forceinline__ void copies(const TreeParams& p, const TreeMaps& maps
         const int eight = __shfl_sync(0xffffffffu, row, lane >> 1);
         const uint32_t to = smem_u32(&sm.side[ring][0][4 * lane]), size = eight >= 0 ? 16 : 0;
         const int from = eight >= 0 ? eight + 4 * (lane & 1) : 0;
-        if (p.c.bias) cp_async<16>(to, p.c.bias + from, size);
+        if (p.c.bias) copy_async(to, p.c.bias + from, size);
         if constexpr (X::k8) {
-          cp_async<16>(to + 512, p.c.k_scale + from, size);
-          cp_async<16>(to + 1024, p.c.v_scale + from, size);
+          copy_async(to + 512, p.c.k_scale + from, size);
+          copy_async(to + 1024, p.c.v_scale + from, size);
         }
         cp_async_arrive(&sm.bar_side[ring]);
       }
@@ -415,10 +377,14 @@ __device__ __forceinline__ void widen_tiles(const TreeParams& p, SmemOf<kMode, k
       __syncwarp();  // this warp alone reads and writes these rows
 #pragma unroll
       for (int s = 0; s < 2 * kTurn; ++s) {
-        const uint2 a = widen<kMode>(raw[s].x), b = widen<kMode>(raw[s].y), c = widen<kMode>(raw[s].z), d = widen<kMode>(raw[s].w);
+        uint32_t h[8];
+        widen_word<kMode>(raw[s].x, h[0], h[1]);
+        widen_word<kMode>(raw[s].y, h[2], h[3]);
+        widen_word<kMode>(raw[s].z, h[4], h[5]);
+        widen_word<kMode>(raw[s].w, h[6], h[7]);
         const uint32_t on = (s / kTurn + 2 * half) * 1024;
-        st_shared_v4(tile + to[s % kTurn][0] + on, a.x, a.y, b.x, b.y);
-        st_shared_v4(tile + to[s % kTurn][1] + on, c.x, c.y, d.x, d.y);
+        st_shared_v4(tile + to[s % kTurn][0] + on, h[0], h[1], h[2], h[3]);
+        st_shared_v4(tile + to[s % kTurn][1] + on, h[4], h[5], h[6], h[7]);
       }
     }
     fence_proxy_async_smem();
@@ -646,7 +612,7 @@ __device__ __forceinline__ void softmax(const TreeParams& p, SmemOf<kMode, kD, k
             const int up = top == 0 || top == 255 ? 0 : min(14 + 127 - (int)top, 120);
             const float f = __uint_as_float((uint32_t)(127 + up) << 23);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) h[e] = pack_half(__uint_as_float(h[e] << 16) * f, __uint_as_float(h[e] & 0xffff0000u) * f);
+            for (int e = 0; e < 4; ++e) h[e] = pack<true>(__uint_as_float(h[e] << 16) * f, __uint_as_float(h[e] & 0xffff0000u) * f);
             v[u] = make_uint4(h[0], h[1], h[2], h[3]);
             if (c == 0) sm.qf[rr] = __uint_as_float((uint32_t)(127 - up) << 23);
           }
@@ -862,12 +828,12 @@ __device__ __forceinline__ void softmax(const TreeParams& p, SmemOf<kMode, kD, k
                   v.z = (see >> (x + 2)) & 1 ? v.z : 0.f;
                   v.w = (see >> (x + 3)) & 1 ? v.w : 0.f;
                 }
-                h[x / 2] = pack_half(d[x] * v.x, d[x + 1] * v.y);
-                h[x / 2 + 1] = pack_half(d[x + 2] * v.z, d[x + 3] * v.w);
+                h[x / 2] = pack<true>(d[x] * v.x, d[x + 1] * v.y);
+                h[x / 2 + 1] = pack<true>(d[x + 2] * v.z, d[x + 3] * v.w);
               }
             } else {
 #pragma unroll
-              for (int x = 0; x < 32; x += 2) h[x / 2] = pack2(d[x], d[x + 1]);
+              for (int x = 0; x < 32; x += 2) h[x / 2] = pack<false>(d[x], d[x + 1]);
             }
             tmem_st16(s_col + 16 * c, h);  // over scores that have been read
           }
@@ -949,7 +915,8 @@ __device__ __forceinline__ void softmax(const TreeParams& p, SmemOf<kMode, kD, k
 #pragma unroll
           for (int x = 0; x < 32; x += 8) {
             if (32 * c + x >= p.c.head_dim) continue;
-            const uint4 h = make_uint4(pack2(d[x], d[x + 1]), pack2(d[x + 2], d[x + 3]), pack2(d[x + 4], d[x + 5]), pack2(d[x + 6], d[x + 7]));
+            const uint4 h = make_uint4(pack<false>(d[x], d[x + 1]), pack<false>(d[x + 2], d[x + 3]),
+                                       pack<false>(d[x + 4], d[x + 5]), pack<false>(d[x + 6], d[x + 7]));
             if (wide) {
               *reinterpret_cast<uint4*>(out + 32 * c + x) = h;
             } else {
